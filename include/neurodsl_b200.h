@@ -63,6 +63,12 @@
  *                       tensor-parallel reduction fused with :add + :layernorm)
  *   nd_gemm_allreduce_add_layernorm  the same, with the row-parallel :linear
  *                       before it in one launch
+ *   nd_window_attn_fwd  no reference counterpart (flash_attn_fwd! with a sliding
+ *                       window, sinks and grouped query heads)
+ *   nd_paged_decode_attn, nd_paged_kv_store, nd_paged_kv_evict  no reference
+ *                       counterpart (a key-value cache in pages)
+ *   nd_logits_penalty   no reference counterpart (between the LM head and the
+ *                       choice of a token)
  */
 #ifndef NEURODSL_B200_H
 #define NEURODSL_B200_H
@@ -462,6 +468,133 @@ int nd_gemm_allreduce_add_layernorm(void *stream, const void *A, const void *W, 
                                     int rows_max, int slot, const void *x, const float *bias,
                                     const float *gamma, const float *beta, void *s_out, void *y,
                                     int rows, int d, float eps);
+
+/*
+ * Attention prefill with a sliding window and sinks (no reference
+ * counterpart: flash_attn_fwd! with a mask and grouped query heads).
+ *   Q, O [B][H][Sq][64], K, V [B][Hkv][Sk][64] at element strides {row, head,
+ *   batch} as in nd_flash_attn_fwd_strided; H a multiple of Hkv, query head h
+ *   reads key head h / (H / Hkv).  1 <= Sq <= Sk: the queries are the last Sq
+ *   positions (a prompt's next chunk against the keys so far).  The query at
+ *   position p sees key j when j <= p and (j > p - window or j < sinks);
+ *   window >= 1 (Sk or more: plain causal attention), sinks >= 0, scale > 0.
+ *   Keys and values below Sk have to be finite: a masked one weighs exactly 0,
+ *   and 0 times an infinity is NaN.
+ *   lse, row_max [B][H][Sq] fp32 or NULL.  The weights are rounded to bf16
+ *   for the second product, whatever o_dtype.
+ */
+int nd_window_attn_fwd(void *stream, const void *Q, const int64_t *q_strides, const void *K,
+                       const int64_t *k_strides, const void *V, const int64_t *v_strides, void *O,
+                       const int64_t *o_strides, int o_dtype, float *lse, float *row_max, int B,
+                       int H, int Hkv, int Sq, int Sk, int D, float scale, int window, int sinks);
+
+/*
+ * A key-value cache in pages (no reference counterpart).  A pool is K and V of
+ * [n_pages][Hkv][page_size][64] bf16; position t of sequence b is row
+ * t % page_size of page table[b * table_ld + t / page_size], t / page_size <
+ * max_pages.  A contiguous cache [B][Hkv][L_max][64] is a pool of B pages with
+ * page_size L_max.  Tables and lengths are int32 on the device and are read
+ * when the kernel runs.  Two sequences may share pages that neither writes.
+ * A page number outside [0, n_pages) where a key is needed reads as zeros and
+ * takes no write; it, and a length that is negative or past the table (cut to
+ * fit, and nothing appended), set the device error word to 16
+ * (nd_device_error).  D must be 64; H a multiple of Hkv; page_size >= 1,
+ * max_pages * page_size < 2^30.
+ */
+
+/* Scratch bytes of nd_paged_decode_attn for at most max_len = max_pages *
+ * page_size keys; with_weights: for calls that accumulate weights.  The
+ * workspace must be zero-filled once before its first use, every call leaves
+ * it ready for the next, and calls that may run at the same time need one
+ * each. */
+int nd_paged_decode_workspace_size(int B, int H, int Hkv, int64_t max_len, int D,
+                                   int with_weights, size_t *bytes);
+
+/*
+ * Decode attention of one new token per sequence over a paged cache.
+ *   q [B][H][64] bf16; lens [B]: keys of each sequence, the new token
+ *   included; 0: a row of zeros with lse -inf.
+ *   k_new, v_new [B][Hkv][64] bf16 or both NULL: the token at position
+ *   lens[b] - 1, used for that key and written into its page (which no other
+ *   sequence may read or write in the same call).
+ *   window > 0: key j is seen when j >= lens[b] - window or j < sinks; 0: all.
+ *   Pages without a visible key are not read, and their table entries may
+ *   hold anything.
+ *   out [B][H][64] in o_dtype; lse [B][H] fp32 or NULL.
+ *   weights [B][Hkv][weights_ld] fp32 or NULL: weights[b][h][j] += the sum over
+ *   the group's query heads of exp(s_j - lse), for every visible key j
+ *   (weights_ld >= max_pages * page_size) — what nd_paged_kv_evict goes by.
+ *   workspace: nd_paged_decode_workspace_size bytes, required.
+ */
+int nd_paged_decode_attn(void *stream, const void *q, const void *k_new, const void *v_new,
+                         void *k_pages, void *v_pages, int n_pages, int page_size,
+                         const int32_t *table, int64_t table_ld, int max_pages,
+                         const int32_t *lens, void *out, int o_dtype, float *lse, float *weights,
+                         int64_t weights_ld, int B, int H, int Hkv, int D, int window, int sinks,
+                         float scale, void *workspace, size_t workspace_bytes);
+
+/*
+ * nd_kv_store into a paged cache: the K and V rows of token (b, s) at columns
+ * k_col and v_col of src [B*S][ld] bf16 go to position pos0 + s of sequence b
+ * (pos0_dev[b] + s if pos0_dev is not NULL).  lens [B] or NULL: tokens s >=
+ * lens[b] are padding and move nothing.  ld, k_col, v_col multiples of 8.
+ */
+int nd_paged_kv_store(void *stream, const void *src, int64_t ld, int k_col, int v_col,
+                      void *k_pages, void *v_pages, int n_pages, int page_size,
+                      const int32_t *table, int64_t table_ld, int max_pages, int B, int S, int Hkv,
+                      int pos0, const int32_t *pos0_dev, const int32_t *lens, int D);
+
+/*
+ * Eviction from a paged cache by accumulated attention weight.  For each
+ * (sequence, kv head) with more than `budget` keys, the first `sinks`, the
+ * last `recent` and, of those between, the budget - sinks - recent largest
+ * weights stay (the lowest positions among equals; NaN counts as the least);
+ * with at most `budget` keys all stay.  The kept rows are copied in order to
+ * positions 0, 1, ... of out_table's pages (max_out_pages a sequence), so
+ * shared source pages stay as they are; out_table's pages may not be among
+ * the source pages of any sequence nor occur twice.
+ *   weights [B][Hkv][weights_ld] fp32, weights_ld >= max_pages * page_size;
+ *   weights_out [B][Hkv][weights_out_ld] fp32, weights_out_ld >= budget: the
+ *   kept keys' weights, then zeros; may not overlap weights.
+ *   kept [B][Hkv][budget] int32: the positions that stay, then -1.
+ *   new_lens [B] int32: min(lens[b], budget).
+ *   budget >= 1, sinks + recent <= budget <= max_out_pages * page_size.
+ */
+int nd_paged_kv_evict(void *stream, void *k_pages, void *v_pages, int n_pages, int page_size,
+                      const int32_t *table, int64_t table_ld, int max_pages, const int32_t *lens,
+                      const float *weights, int64_t weights_ld, const int32_t *out_table,
+                      int64_t out_table_ld, int max_out_pages, float *weights_out,
+                      int64_t weights_out_ld, int32_t *kept, int32_t *new_lens, int B, int Hkv,
+                      int D, int budget, int sinks, int recent);
+
+/*
+ * Penalties, biases and a grammar mask on logits, and the greedy token (no
+ * reference counterpart; nd_argmax picks from unchanged logits).  Per row, for
+ * token v with c = its count in the row's history:
+ *   x = logits[v];  if c > 0: x = x > 0 ? x / repetition : x * repetition,
+ *   x = x - presence, x = x - frequency * c;  x = x + bias(v);
+ *   x = -inf where the mask's bit is 0
+ * each operation rounded to fp32, out [rows][V] in out_dtype.
+ *   logits [rows][V] in dtype, row stride ld; out may be logits (same dtype
+ *   and stride), and may otherwise not overlap it.
+ *   history [rows][history_ld] int32 or NULL: n_history entries a row, the
+ *   first history_lens[row] of them used (NULL: all), negative ones skipped.
+ *   repetition (> 0), presence, frequency [rows] fp32 or NULL (left out).
+ *   bias_ids, bias [rows][n_bias] or both NULL: negative ids are skipped, a
+ *   token listed twice takes both biases.
+ *   mask [rows][mask_ld] 32-bit words or NULL, mask_ld >= ceil(V / 32) (0: one
+ *   mask for all rows): bit v % 32 of word v / 32 allows token v.
+ *   idx [rows] int32 or NULL: the first index of the largest value of out's
+ *   row (NaN never wins over a number; 0 if nothing is allowed).
+ * A history or bias token >= V, or a history length outside [0, n_history],
+ * sets the device error word to 16; the token is skipped, the length cut.
+ */
+int nd_logits_penalty(void *stream, const void *logits, int dtype, int64_t ld, int rows, int V,
+                      const int32_t *history, int64_t history_ld, int n_history,
+                      const int32_t *history_lens, const float *repetition, const float *presence,
+                      const float *frequency, const int32_t *bias_ids, const float *bias,
+                      int n_bias, const uint32_t *mask, int64_t mask_ld, void *out, int out_dtype,
+                      int64_t out_ld, int32_t *idx);
 
 #ifdef __cplusplus
 }

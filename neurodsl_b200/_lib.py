@@ -86,6 +86,21 @@ SIGNATURES = {
     "nd_comm_free": (_i, [_vp]),
     "nd_allreduce_add_layernorm": (_i, [_vp, ctypes.POINTER(_vp), _i, _i, _sz, _i, _i, _vp, _vp,
                                         _vp, _vp, _vp, _vp, _i, _i, _f]),
+    "nd_window_attn_fwd": (_i, [_vp, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _i, _vp, _vp,
+                                _i, _i, _i, _i, _i, _i, _f, _i, _i]),
+    "nd_paged_decode_workspace_size": (_i, [_i, _i, _i, ctypes.c_int64, _i, _i,
+                                            ctypes.POINTER(_sz)]),
+    "nd_paged_decode_attn": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp, ctypes.c_int64, _i,
+                                  _vp, _vp, _i, _vp, _vp, ctypes.c_int64, _i, _i, _i, _i, _i, _i,
+                                  _f, _vp, _sz]),
+    "nd_paged_kv_store": (_i, [_vp, _vp, ctypes.c_int64, _i, _i, _vp, _vp, _i, _i, _vp,
+                               ctypes.c_int64, _i, _i, _i, _i, _i, _vp, _vp, _i]),
+    "nd_paged_kv_evict": (_i, [_vp, _vp, _vp, _i, _i, _vp, ctypes.c_int64, _i, _vp, _vp,
+                               ctypes.c_int64, _vp, ctypes.c_int64, _i, _vp, ctypes.c_int64, _vp,
+                               _vp, _i, _i, _i, _i, _i, _i]),
+    "nd_logits_penalty": (_i, [_vp, _vp, _i, ctypes.c_int64, _i, _i, _vp, ctypes.c_int64, _i, _vp,
+                               _vp, _vp, _vp, _vp, _vp, _i, _vp, ctypes.c_int64, _vp, _i,
+                               ctypes.c_int64, _vp]),
     "nd_gemm_allreduce_add_layernorm": (_i, [_vp, _vp, _vp, _i, ctypes.POINTER(_vp), _i, _i, _sz,
                                              _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _f]),
 }

@@ -23,7 +23,9 @@
 #include "launch.cuh"
 #include "elementwise.h"
 #include "layernorm.h"
+#include "logits.h"
 #include "model_ops.h"
+#include "paged_kv.h"
 #include "tp_comm.h"
 #include "tma.h"
 
@@ -297,18 +299,24 @@ void normalize_unit_strides(long long (&s)[3], int S, int H, int B) {
   }
 }
 
+// The window form's mask; null where the plain forms' `causal` says it all.
+struct FlashMask {
+  int window, sinks;
+};
+
 int flash_attn_common(const char* fn, void* stream, const void* Q, const void* K, const void* V,
                       void* O, int o_dtype, float* lse, float* row_max, int B, int H, int Sq,
-                      int Sk, int D, float scale, int causal, nd::FlashStrides st) {
+                      int Sk, int D, float scale, int causal, nd::FlashStrides st, int Hkv,
+                      const FlashMask* mask = nullptr) {
   normalize_unit_strides(st.q, Sq, H, B);
   normalize_unit_strides(st.o, Sq, H, B);
-  normalize_unit_strides(st.k, Sk, H, B);
-  normalize_unit_strides(st.v, Sk, H, B);
+  normalize_unit_strides(st.k, Sk, Hkv, B);
+  normalize_unit_strides(st.v, Sk, Hkv, B);
   if (B < 0 || H < 0 || Sq < 0 || Sk < 0)
     return fail(ND_ERR_INVALID_ARG, "%s: negative size (B=%d H=%d Sq=%d Sk=%d)", fn, B, H, Sq, Sk);
   if (D != 64) return fail(ND_ERR_UNSUPPORTED, "%s: head_dim %d not supported (64 only)", fn, D);
   if (!valid_dtype(o_dtype)) return fail(ND_ERR_UNSUPPORTED, "%s: bad o_dtype %d", fn, o_dtype);
-  if (causal && Sq != Sk)
+  if (mask == nullptr && causal && Sq != Sk)
     return fail(ND_ERR_SHAPE, "%s: causal attention needs Sq == Sk (got %d, %d)", fn, Sq, Sk);
   if (!causal && Sk == 0 && Sq > 0)
     return fail(ND_ERR_SHAPE, "%s: no keys (Sk = 0) for %d queries", fn, Sq);
@@ -335,11 +343,16 @@ int flash_attn_common(const char* fn, void* stream, const void* Q, const void* K
   int rc = check_current_device(nullptr);
   if (rc) return rc;
   const char* msg = nullptr;
-  cudaError_t e = nd::launch_flash_fwd(static_cast<cudaStream_t>(stream),
-                                       static_cast<const __nv_bfloat16*>(Q),
-                                       static_cast<const __nv_bfloat16*>(K),
-                                       static_cast<const __nv_bfloat16*>(V), O, o_dtype == ND_F32,
-                                       lse, row_max, B, H, Sq, Sk, scale, causal != 0, st, &msg);
+  const cudaStream_t cs = static_cast<cudaStream_t>(stream);
+  const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(Q);
+  const __nv_bfloat16* k = static_cast<const __nv_bfloat16*>(K);
+  const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(V);
+  cudaError_t e =
+      mask == nullptr
+          ? nd::launch_flash_fwd(cs, q, k, v, O, o_dtype == ND_F32, lse, row_max, B, H, Sq, Sk,
+                                 scale, causal != 0, st, &msg)
+          : nd::launch_window_fwd(cs, q, k, v, O, o_dtype == ND_F32, lse, row_max, B, H, Hkv, Sq,
+                                  Sk, scale, mask->window, mask->sinks, st, &msg);
   if (e != cudaSuccess) return cuda_fail(e, fn, msg);
   return ok();
 }
@@ -353,7 +366,7 @@ __attribute__((visibility("default"))) int nd_flash_attn_fwd(void* stream, const
                                                              int causal) {
   return flash_attn_common("nd_flash_attn_fwd", stream, Q, K, V, O, o_dtype, lse, row_max, B, H,
                            Sq, Sk, D, scale, causal,
-                           nd::flash_head_major_strides(H < 1 ? 1 : H, Sq, Sk));
+                           nd::flash_head_major_strides(H < 1 ? 1 : H, Sq, Sk), H);
 }
 
 __attribute__((visibility("default"))) int nd_flash_attn_fwd_strided(
@@ -370,7 +383,7 @@ __attribute__((visibility("default"))) int nd_flash_attn_fwd_strided(
     st.o[i] = o_strides[i];
   }
   return flash_attn_common("nd_flash_attn_fwd_strided", stream, Q, K, V, O, o_dtype, lse, row_max,
-                           B, H, Sq, Sk, D, scale, causal, st);
+                           B, H, Sq, Sk, D, scale, causal, st, H);
 }
 
 __attribute__((visibility("default"))) int nd_kv_decode_workspace_size(int B, int H, int L, int D,
@@ -1093,6 +1106,309 @@ __attribute__((visibility("default"))) int nd_gemm_allreduce_add_layernorm(
       static_cast<const __nv_bfloat16*>(x), bias, gamma, beta,
       static_cast<__nv_bfloat16*>(s_out), static_cast<__nv_bfloat16*>(y), rows, d, eps,
       nd::device_error_word());
+  if (e != cudaSuccess) return cuda_fail(e, fn);
+  return ok();
+}
+
+__attribute__((visibility("default"))) int nd_window_attn_fwd(
+    void* stream, const void* Q, const int64_t* q_strides, const void* K, const int64_t* k_strides,
+    const void* V, const int64_t* v_strides, void* O, const int64_t* o_strides, int o_dtype,
+    float* lse, float* row_max, int B, int H, int Hkv, int Sq, int Sk, int D, float scale,
+    int window, int sinks) {
+  const char* fn = "nd_window_attn_fwd";
+  if (!q_strides || !k_strides || !v_strides || !o_strides)
+    return fail(ND_ERR_INVALID_ARG, "%s: null strides", fn);
+  if (B < 0 || H < 0 || Hkv < 0 || Sq < 0 || Sk < 0)
+    return fail(ND_ERR_INVALID_ARG, "%s: negative size", fn);
+  if (H > 0 && (Hkv < 1 || H % Hkv != 0))
+    return fail(ND_ERR_SHAPE, "%s: %d query heads are no multiple of %d key heads", fn, H, Hkv);
+  if (Sq > Sk)
+    return fail(ND_ERR_SHAPE, "%s: %d queries are more than %d keys", fn, Sq, Sk);
+  if (window < 1 || sinks < 0)
+    return fail(ND_ERR_INVALID_ARG, "%s: need window >= 1 and sinks >= 0 (got %d, %d)", fn, window, sinks);
+  if (!(scale > 0.f) || !isfinite(scale))
+    return fail(ND_ERR_INVALID_ARG, "%s: scale must be positive and finite", fn);
+  if (Sk > (1 << 30)) return fail(ND_ERR_SHAPE, "%s: Sk = %d exceeds 2^30", fn, Sk);
+  nd::FlashStrides st;
+  for (int i = 0; i < 3; ++i) {
+    st.q[i] = q_strides[i];
+    st.k[i] = k_strides[i];
+    st.v[i] = v_strides[i];
+    st.o[i] = o_strides[i];
+  }
+  const FlashMask mask = {window, sinks};
+  return flash_attn_common(fn, stream, Q, K, V, O, o_dtype, lse, row_max, B, H, Sq, Sk, D, scale,
+                           1, st, Hkv, &mask);
+}
+
+namespace {
+constexpr long long kMaxPagedLen = 1LL << 30;   // positions are ints, a tile past the last included
+
+// What every paged entry point asks of a pool and its table.
+int check_pool(const char* fn, const void* k, const void* v, int n_pages, int page_size,
+               const void* table, int64_t table_ld, int max_pages, int B, int Hkv, int D,
+               bool empty) {
+  if (B < 0 || Hkv < 0 || max_pages < 0 || n_pages < 0)
+    return fail(ND_ERR_INVALID_ARG, "%s: negative size", fn);
+  if (D != 64) return fail(ND_ERR_UNSUPPORTED, "%s: head_dim %d not supported (64 only)", fn, D);
+  if (page_size < 1) return fail(ND_ERR_SHAPE, "%s: page_size %d must be at least 1", fn, page_size);
+  if (static_cast<long long>(max_pages) * page_size >= kMaxPagedLen)
+    return fail(ND_ERR_SHAPE, "%s: max_pages %d x page_size %d must be below 2^30", fn, max_pages, page_size);
+  if (table_ld < max_pages)
+    return fail(ND_ERR_SHAPE, "%s: table row stride %lld < max_pages %d", fn,
+                static_cast<long long>(table_ld), max_pages);
+  if (static_cast<long long>(B) * Hkv > 65535)
+    return fail(ND_ERR_SHAPE, "%s: B*Hkv = %lld exceeds 65535", fn, static_cast<long long>(B) * Hkv);
+  if (empty) return ND_OK;
+  if (n_pages < 1) return fail(ND_ERR_SHAPE, "%s: the pool has no pages", fn);
+  if (!k || !v || (!table && max_pages > 0))
+    return fail(ND_ERR_INVALID_ARG, "%s: null pool or table pointer", fn);
+  if (!aligned16(k) || !aligned16(v))
+    return fail(ND_ERR_ALIGNMENT, "%s: pools must be 16-byte aligned", fn);
+  return ND_OK;
+}
+
+nd::PagedPool make_pool(void* k, void* v, int n_pages, int Hkv, int page_size,
+                        const int32_t* table, int64_t table_ld, int max_pages) {
+  nd::PagedPool p;
+  p.k = static_cast<__nv_bfloat16*>(k);
+  p.v = static_cast<__nv_bfloat16*>(v);
+  p.n_pages = n_pages;
+  p.Hkv = Hkv;
+  p.page_size = page_size;
+  p.table = table;
+  p.table_ld = table_ld;
+  p.max_pages = max_pages;
+  return p;
+}
+}  // namespace
+
+__attribute__((visibility("default"))) int nd_paged_decode_workspace_size(int B, int H, int Hkv,
+                                                                          int64_t max_len, int D,
+                                                                          int with_weights,
+                                                                          size_t* bytes) {
+  const char* fn = "nd_paged_decode_workspace_size";
+  if (!bytes) return fail(ND_ERR_INVALID_ARG, "%s: bytes is NULL", fn);
+  if (B < 0 || H < 0 || Hkv < 0 || max_len < 0) return fail(ND_ERR_INVALID_ARG, "%s: negative size", fn);
+  if (D != 64) return fail(ND_ERR_UNSUPPORTED, "%s: head_dim %d not supported (64 only)", fn, D);
+  if (max_len >= kMaxPagedLen) return fail(ND_ERR_SHAPE, "%s: max_len must be below 2^30", fn);
+  if (H > 0 && (Hkv < 1 || H % Hkv != 0))
+    return fail(ND_ERR_SHAPE, "%s: %d query heads are no multiple of %d key heads", fn, H, Hkv);
+  *bytes = nd::paged_decode_workspace_bytes(B, H, Hkv, max_len, with_weights != 0);
+  return ok();
+}
+
+__attribute__((visibility("default"))) int nd_paged_decode_attn(
+    void* stream, const void* q, const void* k_new, const void* v_new, void* k_pages,
+    void* v_pages, int n_pages, int page_size, const int32_t* table, int64_t table_ld,
+    int max_pages, const int32_t* lens, void* out, int o_dtype, float* lse, float* weights,
+    int64_t weights_ld, int B, int H, int Hkv, int D, int window, int sinks, float scale,
+    void* workspace, size_t workspace_bytes) {
+  const char* fn = "nd_paged_decode_attn";
+  if (H < 0) return fail(ND_ERR_INVALID_ARG, "%s: negative size", fn);
+  const bool empty = B == 0 || H == 0;
+  int rc = check_pool(fn, k_pages, v_pages, n_pages, page_size, table, table_ld, max_pages, B, Hkv,
+                      D, empty);
+  if (rc) return rc;
+  if (H > 0 && (Hkv < 1 || H % Hkv != 0))
+    return fail(ND_ERR_SHAPE, "%s: %d query heads are no multiple of %d key heads", fn, H, Hkv);
+  if (static_cast<long long>(B) * H > 65535)
+    return fail(ND_ERR_SHAPE, "%s: B*H = %lld exceeds 65535", fn, static_cast<long long>(B) * H);
+  if (!valid_dtype(o_dtype)) return fail(ND_ERR_UNSUPPORTED, "%s: bad o_dtype %d", fn, o_dtype);
+  if ((k_new == nullptr) != (v_new == nullptr))
+    return fail(ND_ERR_INVALID_ARG, "%s: k_new and v_new must both be given or both NULL", fn);
+  if (window < 0 || sinks < 0)
+    return fail(ND_ERR_INVALID_ARG, "%s: window and sinks must not be negative (got %d, %d)", fn, window, sinks);
+  if (!isfinite(scale)) return fail(ND_ERR_INVALID_ARG, "%s: scale must be finite", fn);
+  if (weights != nullptr && weights_ld < static_cast<long long>(max_pages) * page_size)
+    return fail(ND_ERR_SHAPE, "%s: weights row stride %lld < max_pages * page_size", fn,
+                static_cast<long long>(weights_ld));
+  if (empty) return ok();
+  if (!q || !lens || !out) return fail(ND_ERR_INVALID_ARG, "%s: null tensor pointer", fn);
+  if (!aligned16(q) || !aligned16(out) || (k_new && (!aligned16(k_new) || !aligned16(v_new))))
+    return fail(ND_ERR_ALIGNMENT, "%s: tensors must be 16-byte aligned", fn);
+  const size_t need = nd::paged_decode_workspace_bytes(
+      B, H, Hkv, static_cast<long long>(max_pages) * page_size, weights != nullptr);
+  if (workspace == nullptr || workspace_bytes < need)
+    return fail(ND_ERR_WORKSPACE, "%s: workspace %zu bytes < %zu needed", fn,
+                workspace ? workspace_bytes : static_cast<size_t>(0), need);
+  if (!aligned16(workspace)) return fail(ND_ERR_ALIGNMENT, "%s: workspace must be 16-byte aligned", fn);
+  rc = check_current_device(nullptr);
+  if (rc) return rc;
+  nd::PagedDecode a = {};
+  a.q = static_cast<const __nv_bfloat16*>(q);
+  a.k_new = static_cast<const __nv_bfloat16*>(k_new);
+  a.v_new = static_cast<const __nv_bfloat16*>(v_new);
+  a.pool = make_pool(k_pages, v_pages, n_pages, Hkv, page_size, table, table_ld, max_pages);
+  a.lens = lens;
+  a.out = out;
+  a.out_f32 = o_dtype == ND_F32;
+  a.lse = lse;
+  a.weights = weights;
+  a.weights_ld = weights_ld;
+  a.B = B;
+  a.H = H;
+  a.window = window;
+  a.sinks = sinks;
+  a.scale = scale;
+  a.workspace = workspace;
+  const cudaError_t e =
+      nd::launch_paged_decode(static_cast<cudaStream_t>(stream), a, nd::device_error_word());
+  if (e != cudaSuccess) return cuda_fail(e, fn);
+  return ok();
+}
+
+__attribute__((visibility("default"))) int nd_paged_kv_store(
+    void* stream, const void* src, int64_t ld, int k_col, int v_col, void* k_pages, void* v_pages,
+    int n_pages, int page_size, const int32_t* table, int64_t table_ld, int max_pages, int B,
+    int S, int Hkv, int pos0, const int32_t* pos0_dev, const int32_t* lens, int D) {
+  const char* fn = "nd_paged_kv_store";
+  if (S < 0 || (pos0_dev == nullptr && pos0 < 0)) return fail(ND_ERR_INVALID_ARG, "%s: negative size", fn);
+  const bool empty = B == 0 || S == 0 || Hkv == 0;
+  int rc = check_pool(fn, k_pages, v_pages, n_pages, page_size, table, table_ld, max_pages, B, Hkv,
+                      D, empty);
+  if (rc) return rc;
+  if (pos0_dev == nullptr && lens == nullptr &&
+      static_cast<long long>(pos0) + S > static_cast<long long>(max_pages) * page_size)
+    return fail(ND_ERR_SHAPE, "%s: pos0 %d + S %d exceeds max_pages * page_size", fn, pos0, S);
+  if (ld % 8 || k_col % 8 || v_col % 8 || k_col < 0 || v_col < 0 ||
+      k_col + static_cast<long long>(Hkv) * 64 > ld || v_col + static_cast<long long>(Hkv) * 64 > ld)
+    return fail(ND_ERR_SHAPE, "%s: columns k=%d v=%d (+%d) must be multiples of 8 inside ld=%lld", fn,
+                k_col, v_col, Hkv * 64, static_cast<long long>(ld));
+  if (static_cast<long long>(B) * S * Hkv > (1LL << 36))
+    return fail(ND_ERR_SHAPE, "%s: too many rows", fn);
+  if (empty) return ok();
+  if (!src) return fail(ND_ERR_INVALID_ARG, "%s: null pointer", fn);
+  if (!aligned16(src)) return fail(ND_ERR_ALIGNMENT, "%s: src must be 16-byte aligned", fn);
+  rc = check_current_device(nullptr);
+  if (rc) return rc;
+  const cudaError_t e = nd::launch_paged_store(
+      static_cast<cudaStream_t>(stream), static_cast<const __nv_bfloat16*>(src), ld, k_col, v_col,
+      make_pool(k_pages, v_pages, n_pages, Hkv, page_size, table, table_ld, max_pages), B, S, pos0,
+      pos0_dev, lens, nd::device_error_word());
+  if (e != cudaSuccess) return cuda_fail(e, fn);
+  return ok();
+}
+
+__attribute__((visibility("default"))) int nd_paged_kv_evict(
+    void* stream, void* k_pages, void* v_pages, int n_pages, int page_size, const int32_t* table,
+    int64_t table_ld, int max_pages, const int32_t* lens, const float* weights, int64_t weights_ld,
+    const int32_t* out_table, int64_t out_table_ld, int max_out_pages, float* weights_out,
+    int64_t weights_out_ld, int32_t* kept, int32_t* new_lens, int B, int Hkv, int D, int budget,
+    int sinks, int recent) {
+  const char* fn = "nd_paged_kv_evict";
+  const bool empty = B == 0 || Hkv == 0;
+  int rc = check_pool(fn, k_pages, v_pages, n_pages, page_size, table, table_ld, max_pages, B, Hkv,
+                      D, empty);
+  if (rc) return rc;
+  if (budget < 1 || sinks < 0 || recent < 0 || static_cast<long long>(sinks) + recent > budget)
+    return fail(ND_ERR_INVALID_ARG, "%s: need budget >= 1 and sinks + recent <= budget (got %d, %d, %d)",
+                fn, budget, sinks, recent);
+  if (max_out_pages < 0 || out_table_ld < max_out_pages ||
+      static_cast<long long>(max_out_pages) * page_size < budget)
+    return fail(ND_ERR_SHAPE, "%s: %d output pages of %d do not hold the budget %d", fn,
+                max_out_pages, page_size, budget);
+  if (static_cast<long long>(max_out_pages) * page_size >= kMaxPagedLen)
+    return fail(ND_ERR_SHAPE, "%s: max_out_pages * page_size must be below 2^30", fn);
+  if (weights_ld < static_cast<long long>(max_pages) * page_size || weights_out_ld < budget)
+    return fail(ND_ERR_SHAPE, "%s: weights rows are too short", fn);
+  if (empty) return ok();
+  if (!lens || !weights || !out_table || !weights_out || !kept || !new_lens)
+    return fail(ND_ERR_INVALID_ARG, "%s: null pointer", fn);
+  const float* w_end = weights + static_cast<size_t>(B) * Hkv * weights_ld;
+  const float* wo_end = weights_out + static_cast<size_t>(B) * Hkv * weights_out_ld;
+  if (weights_out < w_end && weights < wo_end)
+    return fail(ND_ERR_INVALID_ARG, "%s: weights_out overlaps weights", fn);
+  rc = check_current_device(nullptr);
+  if (rc) return rc;
+  nd::PagedEvict a = {};
+  a.pool = make_pool(k_pages, v_pages, n_pages, Hkv, page_size, table, table_ld, max_pages);
+  a.lens = lens;
+  a.weights = weights;
+  a.weights_ld = weights_ld;
+  a.out_table = out_table;
+  a.out_table_ld = out_table_ld;
+  a.out_pages = max_out_pages;
+  a.B = B;
+  a.budget = budget;
+  a.sinks = sinks;
+  a.recent = recent;
+  a.weights_out = weights_out;
+  a.weights_out_ld = weights_out_ld;
+  a.kept = kept;
+  a.new_lens = new_lens;
+  const cudaError_t e =
+      nd::launch_paged_evict(static_cast<cudaStream_t>(stream), a, nd::device_error_word());
+  if (e != cudaSuccess) return cuda_fail(e, fn);
+  return ok();
+}
+
+__attribute__((visibility("default"))) int nd_logits_penalty(
+    void* stream, const void* logits, int dtype, int64_t ld, int rows, int V,
+    const int32_t* history, int64_t history_ld, int n_history, const int32_t* history_lens,
+    const float* repetition, const float* presence, const float* frequency,
+    const int32_t* bias_ids, const float* bias, int n_bias, const uint32_t* mask, int64_t mask_ld,
+    void* out, int out_dtype, int64_t out_ld, int32_t* idx) {
+  const char* fn = "nd_logits_penalty";
+  if (rows < 0 || V < 0 || n_history < 0 || n_bias < 0)
+    return fail(ND_ERR_INVALID_ARG, "%s: negative size", fn);
+  if (!valid_dtype(dtype) || !valid_dtype(out_dtype))
+    return fail(ND_ERR_UNSUPPORTED, "%s: bad dtype %d or %d", fn, dtype, out_dtype);
+  if (ld < V || out_ld < V)
+    return fail(ND_ERR_SHAPE, "%s: row stride %lld or %lld < V %d", fn, static_cast<long long>(ld),
+                static_cast<long long>(out_ld), V);
+  if (V > (1 << 30)) return fail(ND_ERR_SHAPE, "%s: V = %d exceeds 2^30", fn, V);
+  if (history != nullptr && history_ld < n_history)
+    return fail(ND_ERR_SHAPE, "%s: history row stride %lld < %d", fn,
+                static_cast<long long>(history_ld), n_history);
+  if ((bias_ids == nullptr) != (bias == nullptr))
+    return fail(ND_ERR_INVALID_ARG, "%s: bias_ids and bias must both be given or both NULL", fn);
+  if (history == nullptr && (history_lens || repetition || presence || frequency))
+    return fail(ND_ERR_INVALID_ARG, "%s: penalties need a history", fn);
+  if (mask != nullptr && mask_ld != 0 && mask_ld < (static_cast<long long>(V) + 31) / 32)
+    return fail(ND_ERR_SHAPE, "%s: mask row stride %lld < ceil(V / 32)", fn, static_cast<long long>(mask_ld));
+  if (rows == 0) return ok();
+  if (V == 0) return fail(ND_ERR_SHAPE, "%s: empty rows (V = 0)", fn);
+  if (!logits || !out) return fail(ND_ERR_INVALID_ARG, "%s: null pointer", fn);
+  if (logits == out) {
+    if (dtype != out_dtype || ld != out_ld)
+      return fail(ND_ERR_INVALID_ARG, "%s: out may be logits only with its dtype and stride", fn);
+  } else {
+    const char* x = static_cast<const char*>(logits);
+    const char* y = static_cast<const char*>(out);
+    const long long xn = ((rows - 1) * static_cast<long long>(ld) + V) * (dtype == ND_F32 ? 4 : 2);
+    const long long yn = ((rows - 1) * static_cast<long long>(out_ld) + V) * (out_dtype == ND_F32 ? 4 : 2);
+    if (x < y + yn && y < x + xn) return fail(ND_ERR_INVALID_ARG, "%s: out overlaps logits", fn);
+  }
+  const uintptr_t in_size = dtype == ND_F32 ? 4 : 2, out_size = out_dtype == ND_F32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(logits) % in_size || reinterpret_cast<uintptr_t>(out) % out_size)
+    return fail(ND_ERR_ALIGNMENT, "%s: logits and out must be aligned to their elements", fn);
+  int rc = check_current_device(nullptr);
+  if (rc) return rc;
+  nd::LogitsPenalty a = {};
+  a.logits = logits;
+  a.in_f32 = dtype == ND_F32;
+  a.ld = ld;
+  a.rows = rows;
+  a.V = V;
+  a.history = n_history > 0 ? history : nullptr;
+  a.history_ld = history_ld;
+  a.n_history = n_history;
+  a.history_lens = history_lens;
+  a.repetition = repetition;
+  a.presence = presence;
+  a.frequency = frequency;
+  a.bias_ids = n_bias > 0 ? bias_ids : nullptr;
+  a.bias = bias;
+  a.n_bias = n_bias;
+  a.mask = mask;
+  a.mask_ld = mask_ld;
+  a.out = out;
+  a.out_f32 = out_dtype == ND_F32;
+  a.out_ld = out_ld;
+  a.idx = idx;
+  const cudaError_t e =
+      nd::launch_logits_penalty(static_cast<cudaStream_t>(stream), a, nd::device_error_word());
   if (e != cudaSuccess) return cuda_fail(e, fn);
   return ok();
 }

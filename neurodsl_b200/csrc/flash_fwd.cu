@@ -38,6 +38,16 @@
 // the offset, so the final O/l is exact; the reported m is the true row max.  A row's output (O/l, lse, m) is
 // written during the first tile of its next item, before that item's first
 // P·V overwrites O, so no warp waits for the last P·V of an item.
+//
+// Window form (kWindow): query i sits at position p = Sk - Sq + i and sees
+// key j when j <= p and (j > p - window or j < sinks); K and V may have fewer
+// heads, each shared by `group` query heads.  An item streams only the K/V
+// tiles that hold a key one of its rows sees: the sinks' tiles, then the
+// window's.  The second query tile's window begins and ends one K/V tile
+// later than the first's, so each query tile leaves out one tile of the stream
+// it shares with the other.  Only tiles cut by a border of the visible range
+// are masked, by a bit mask per 32 columns (two instructions a score; the
+// comparisons it replaces would be four).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <limits.h>
@@ -239,11 +249,45 @@ struct WorkItem {
   int bh;         // batch * H + head
   int n_kv[kTiles];
   int n_total;    // K/V tiles streamed for the item (the last tile needs the most)
+  // window form: the stream is K/V tiles [0, n_sink), then lo, lo + 1, ...;
+  // query tile 1 leaves out the first `skip` (0 or 1) of the latter
+  int n_sink, lo, skip;
+  // K/V tile at stream position s, and stream position of query tile i's j-th
+  __device__ __forceinline__ int key_tile(int s) const { return s < n_sink ? s : lo + s - n_sink; }
+  __device__ __forceinline__ int stream_pos(int i, int j) const {
+    return (i == 1 && j >= n_sink) ? j + skip : j;
+  }
 };
 
-template <bool kCausal>
-__device__ __forceinline__ WorkItem decode_item(int k, int BH, int n_blk, int n_k) {
+// The window form's geometry: sizes of the visible range, the query heads of
+// a K/V head and the position of query 0.
+struct FlashWindow {
+  int window, sinks, group, off;
+};
+
+template <bool kCausal, bool kWindow>
+__device__ __forceinline__ WorkItem decode_item(int k, int BH, int n_blk, int n_k,
+                                                const FlashWindow& win) {
   WorkItem w;
+  if constexpr (kWindow) {
+    w.blk = n_blk - 1 - k / BH;
+    w.bh = k % BH;
+    const int p0 = win.off + w.blk * kRowsPerCta;        // position of the first row
+    const int lo0 = max(0, p0 - win.window + 1) / kBN;
+    const int hi0 = min((p0 + kBM - 1) / kBN, n_k - 1);
+    const int hi1 = min((p0 + 2 * kBM - 1) / kBN, n_k - 1);
+    // rows past Sq may have their whole window past Sk
+    const int lo1 = min(max(0, p0 + kBM - win.window + 1) / kBN, hi1);
+    const int sink_tiles = ceil_div(win.sinks, kBN);
+    w.lo = lo0;
+    w.n_sink = min(sink_tiles, lo0);
+    w.skip = sink_tiles > lo0 ? 0 : lo1 - lo0;
+    w.n_total = w.n_sink + hi1 - lo0 + 1;
+    w.n_kv[0] = w.n_total - (hi1 - hi0);
+    w.n_kv[1] = w.n_total - w.skip;
+    return w;
+  }
+  w.n_sink = w.lo = w.skip = 0;
   // Heavy items first: with a causal mask the last query rows see the most keys.
   w.blk = kCausal ? (n_blk - 1 - k / BH) : k / BH;
   w.bh = k % BH;
@@ -288,6 +332,7 @@ __device__ __forceinline__ int item_of(int n, int cta, int grid) {
 // item's first K/V tile, and the item's tile counts (nkv = 0: no more items).
 struct Cursor {
   int n, j, base, nkv, total;
+  int n_sink, skip;   // window form: as in WorkItem
 };
 
 // A row whose output is still to be written (the previous item's).
@@ -299,14 +344,14 @@ struct PendingRow {
 
 // kStrided: Q/K/V through 4-D maps and O through FlashLayout strides; the
 // contiguous head-major case keeps 3-D maps {64, S, B·H} and bh·S row offsets.
-template <bool kCausal, bool kOutF32, bool kStrided>
+template <bool kCausal, bool kOutF32, bool kStrided, bool kWindow>
 __global__ void __launch_bounds__(kThreads, 1)
     flash_fwd_kernel(const __grid_constant__ CUtensorMap tm_q,
                      const __grid_constant__ CUtensorMap tm_k,
                      const __grid_constant__ CUtensorMap tm_v,
                      const __grid_constant__ CUtensorMap tm_o, const FlashLayout lay,
                      float* __restrict__ lse_out, float* __restrict__ max_out, int BH, int Sq,
-                     int Sk, float scale_log2, int* __restrict__ err_word) {
+                     int Sk, float scale_log2, int* __restrict__ err_word, const FlashWindow win) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -373,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             return true;
           }
         }
-        const WorkItem w = decode_item<kCausal>(k, BH, n_blk, n_k);
+        const WorkItem w = decode_item<kCausal, kWindow>(k, BH, n_blk, n_k, win);
         const int h = kStrided ? w.bh % lay.H : 0, b = kStrided ? w.bh / lay.H : 0;
         mbar_arrive_expect_tx(&bars->q_full[qb], kTiles * kTileBytes);
         for (int i = 0; i < kTiles; ++i) {
@@ -389,9 +434,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       int n = 0;
       for (int k; ok && (k = item_of(n, cta, grid)) < n_items; ++n) {
-        const WorkItem w = decode_item<kCausal>(k, BH, n_blk, n_k);
+        const WorkItem w = decode_item<kCausal, kWindow>(k, BH, n_blk, n_k, win);
         while (ok && n_q <= n) ok = load_q(true);
-        const int h = kStrided ? w.bh % lay.H : 0, b = kStrided ? w.bh / lay.H : 0;
+        int h = kStrided ? w.bh % lay.H : 0;
+        const int b = kStrided ? w.bh / lay.H : 0;
+        int kv_bh = w.bh;
+        if constexpr (kWindow) {
+          h /= win.group;
+          kv_bh /= win.group;
+        }
         for (int j = 0; ok && j < w.n_total; ++j, ++kv_it) {
           // the next item's Q as soon as its buffer is free
           if (n_q == n + 1) ok = load_q(false);
@@ -401,14 +452,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = false;
           if (!ok) break;
           mbar_arrive_expect_tx(&bars->kv_full[s], 2 * kTileBytes);
+          const int key0 = (kWindow ? w.key_tile(j) : j) * kBN;
           if constexpr (kStrided) {
-            load_rows(&tm_k, &bars->kv_full[s], smem + kOffK + s * kTileBytes, j * kBN, h, b,
+            load_rows(&tm_k, &bars->kv_full[s], smem + kOffK + s * kTileBytes, key0, h, b,
                       lay.kv_token_major);
-            load_rows(&tm_v, &bars->kv_full[s], smem + kOffV + s * kTileBytes, j * kBN, h, b,
+            load_rows(&tm_v, &bars->kv_full[s], smem + kOffV + s * kTileBytes, key0, h, b,
                       lay.kv_token_major);
           } else {
-            tma_load_3d(&tm_k, &bars->kv_full[s], smem + kOffK + s * kTileBytes, 0, j * kBN, w.bh);
-            tma_load_3d(&tm_v, &bars->kv_full[s], smem + kOffV + s * kTileBytes, 0, j * kBN, w.bh);
+            tma_load_3d(&tm_k, &bars->kv_full[s], smem + kOffK + s * kTileBytes, 0, key0, kv_bh);
+            tma_load_3d(&tm_v, &bars->kv_full[s], smem + kOffV + s * kTileBytes, 0, key0, kv_bh);
           }
         }
       }
@@ -433,13 +485,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         c.base = base;
         const int k = item_of(n, cta, grid);
         if (k < n_items) {
-          const WorkItem w = decode_item<kCausal>(k, BH, n_blk, n_k);
+          const WorkItem w = decode_item<kCausal, kWindow>(k, BH, n_blk, n_k, win);
           c.nkv = i == 0 ? w.n_kv[0] : w.n_kv[1];
           c.total = w.n_total;
+          c.n_sink = w.n_sink;
+          c.skip = i == 1 ? w.skip : 0;
         } else {
           c.nkv = 0;
           c.total = 0;
+          c.n_sink = 0;
+          c.skip = 0;
         }
+      };
+      // ring position of the cursor's tile
+      auto ring_pos = [&](const Cursor& c) {
+        if constexpr (kWindow) return c.base + c.j + (c.j >= c.n_sink ? c.skip : 0);
+        return c.base + c.j;
       };
       auto advance = [&](Cursor& c) {
         if (++c.j == c.nkv) start(c, c.n + 1, c.base + c.total);
@@ -471,7 +532,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       while (ok && (c.nkv != 0 || p.nkv != 0)) {
         if (c.nkv != 0) {
           // S = Q·K^T into TMEM once the softmax has read the previous S
-          const int pos = c.base + c.j;
+          const int pos = ring_pos(c);
+          // window form: query tile 1 leaves out the position before this
+          // one; the wait below sees a later position landed, which releases it
+          if constexpr (kWindow) {
+            if (c.skip != 0 && c.j == c.n_sink) skipped = pos - 1;
+          }
           if (s_cnt > 0 && !mbar_wait(&bars->s_free[i], (s_cnt - 1) & 1, abort_flag)) { ok = false; break; }
           if (c.j == 0 && !mbar_wait(&bars->q_full[c.n & 1], (c.n >> 1) & 1, abort_flag)) { ok = false; break; }
           if (!mbar_wait(&bars->kv_full[pos % kStages], (pos / kStages) & 1, abort_flag)) { ok = false; break; }
@@ -494,7 +560,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           // O (+)= P·V once the softmax has written P
           if (!mbar_wait(&bars->p_full[i], pv_cnt & 1, abort_flag)) { ok = false; break; }
           tc_fence_after();
-          const int pos = p.base + p.j;   // landed: its S product waited for it
+          const int pos = ring_pos(p);   // landed: its S product waited for it
           const int s = pos % kStages;
 #pragma unroll
           for (int kk = 0; kk < kBN / 16; ++kk) {
@@ -506,7 +572,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           umma_commit(&bars->o_done[i]);
           ++pv_cnt;
           umma_commit(&bars->kv_empty[s]);
-          if (p.j + 1 == p.nkv && p.nkv < p.total) {
+          if (p.j + 1 == p.nkv && p.nkv + (kWindow ? p.skip : 0) < p.total) {
             skipped = p.base + p.nkv;
             release_skipped();
           }
@@ -599,7 +665,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     PendingRow pend;
     pend.valid = false;
     for (int n = 0, k; ok && (k = item_of(n, cta, grid)) < n_items; ++n) {
-      const WorkItem w = decode_item<kCausal>(k, BH, n_blk, n_k);
+      const WorkItem w = decode_item<kCausal, kWindow>(k, BH, n_blk, n_k, win);
       const int q_idx = w.blk * kRowsPerCta + tile * kBM + row;
       const int nkv = tile == 0 ? w.n_kv[0] : w.n_kv[1];
       float m_used = -INFINITY;  // offset of the exponentials (log2 units)
@@ -617,8 +683,29 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_before();
         mbar_arrive(&bars->s_free[tile]);
         float* sv = reinterpret_cast<float*>(sr);
-        const bool last = (j == nkv - 1);
-        if (last) {
+        bool last = (j == nkv - 1);
+        if constexpr (kWindow) {
+          // `last`: whether a border of the visible range cuts this tile
+          const int k0 = w.key_tile(w.stream_pos(tile, j)) * kBN;
+          const int p_min = win.off + w.blk * kRowsPerCta + tile * kBM, p_max = p_min + kBM - 1;
+          last = k0 + kBN - 1 > p_min || (k0 <= p_max - win.window && k0 + kBN > win.sinks);
+          if (last) {
+            const int hi = p_min + row - k0;          // columns up to hi are not in the future,
+            const int lo = hi - win.window + 1;       // from lo on in the window,
+            const int sk = win.sinks - k0;            // below sk sinks
+#pragma unroll
+            for (int q = 0; q < kBN / 32; ++q) {
+              const int h32 = hi - 32 * q, l32 = lo - 32 * q, s32 = sk - 32 * q;
+              const uint32_t past = h32 < 0 ? 0u : h32 >= 31 ? ~0u : (2u << h32) - 1u;
+              const uint32_t near = l32 <= 0 ? ~0u : l32 > 31 ? 0u : ~0u << l32;
+              const uint32_t sink = s32 <= 0 ? 0u : s32 > 31 ? ~0u : (1u << s32) - 1u;
+              const uint32_t seen = past & (near | sink);
+#pragma unroll
+              for (int c = 0; c < 32; ++c)
+                if (!(seen & (1u << c))) sv[32 * q + c] = -INFINITY;
+            }
+          }
+        } else if (last) {
           const int k0 = j * kBN;
 #pragma unroll
           for (int c = 0; c < kBN; ++c) {
@@ -644,7 +731,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           const bool up = t > m_used + kRescaleThreshold;
           if (!__any_sync(0xffffffffu, up)) return true;
           const float m_new = up ? t : m_used;
-          const float alpha = fast_exp2(m_used - m_new);   // 1 where the offset stays
+          float alpha = fast_exp2(m_used - m_new);   // 1 where the offset stays
+          if constexpr (kWindow) {
+            if (m_used == m_new) alpha = 1.f;          // also while a row has seen no key (-inf)
+          }
           m_used = m_new;
           l *= alpha;
           if (j > 0 || half_stored) {
@@ -677,6 +767,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           return true;
         };
+        // minus the offset; a row that has seen no key yet (a window's first
+        // tile may hold none of its keys) has p = 2^-inf = 0 against any offset
+        auto neg_offset = [&]() -> uint64_t {
+          float nm = -m_used;
+          if constexpr (kWindow) nm = m_used == -INFINITY ? 0.f : nm;
+          return f2_pack(nm, nm);
+        };
         uint32_t pk[kBN / 4];   // half a row of packed probabilities
         // ---- first half of the keys: its max, then its exponentials
         const float t_a = half_max<0>(sv) * scale_log2;
@@ -685,7 +782,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         float sum_a;
         {
           uint64_t acc[4] = {0, 0, 0, 0};
-          exp_cols<0, kBN / 2>(last, sv, scale2, f2_pack(-m_used, -m_used), pk, acc);
+          exp_cols<0, kBN / 2>(last, sv, scale2, neg_offset(), pk, acc);
           sum_a = f2_sum4(acc);
         }
         // second half's max: independent of the exponentials above
@@ -698,7 +795,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!raise_offset(t_b, true)) { ok = false; break; }
         {
           uint64_t acc[4] = {0, 0, 0, 0};
-          exp_cols<kBN / 2, kBN>(last, sv, scale2, f2_pack(-m_used, -m_used), pk, acc);
+          exp_cols<kBN / 2, kBN>(last, sv, scale2, neg_offset(), pk, acc);
           l += f2_sum4(acc);
         }
         tmem_st32(p_addr + 32, *reinterpret_cast<const uint32_t(*)[32]>(pk));
@@ -739,11 +836,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-template <bool kCausal, bool kOutF32, bool kStrided>
+template <bool kCausal, bool kOutF32, bool kStrided, bool kWindow = false>
 cudaError_t launch_typed(cudaStream_t stream, const CUtensorMap& tq, const CUtensorMap& tk,
                          const CUtensorMap& tv, const CUtensorMap& to, const FlashLayout& lay,
-                         float* lse, float* mx, int BH, int Sq, int Sk, float scale_log2) {
-  auto kern = flash_fwd_kernel<kCausal, kOutF32, kStrided>;
+                         float* lse, float* mx, int BH, int Sq, int Sk, float scale_log2,
+                         const FlashWindow& win = {}) {
+  auto kern = flash_fwd_kernel<kCausal, kOutF32, kStrided, kWindow>;
   cudaError_t e =
       cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
   if (e != cudaSuccess) return e;
@@ -756,7 +854,7 @@ cudaError_t launch_typed(cudaStream_t stream, const CUtensorMap& tq, const CUten
   const int n_items = ceil_div(Sq, kRowsPerCta) * BH;
   dim3 grid(n_items < sms ? n_items : sms);
   kern<<<grid, kThreads, kSmemBytes, stream>>>(tq, tk, tv, to, lay, lse, mx, BH, Sq, Sk, scale_log2,
-                                               device_error_word());
+                                               device_error_word(), win);
   return cudaGetLastError();
 }
 
@@ -797,6 +895,60 @@ cudaError_t make_rows_map(CUtensorMap* map, const void* base, int S, int H, int 
 }
 }  // namespace
 
+namespace {
+// The tensor maps of Q, K, V and O for H query heads and Hkv key/value heads;
+// *strided: whether the 4-D form is needed.
+cudaError_t make_maps(const __nv_bfloat16* Q, const __nv_bfloat16* K, const __nv_bfloat16* V,
+                      void* O, bool out_f32, int B, int H, int Hkv, int Sq, int Sk,
+                      const FlashStrides& st, CUtensorMap* tq, CUtensorMap* tk, CUtensorMap* tv,
+                      CUtensorMap* to, FlashLayout* lay, bool* is_strided, const char** err_msg) {
+  lay->H = H;
+  lay->q_token_major = lay->kv_token_major = lay->o_token_major = 0;
+  const FlashStrides hm = flash_head_major_strides(H, Sq, Sk);
+  const FlashStrides hm_kv = flash_head_major_strides(Hkv, Sq, Sk);
+  bool strided = false;
+  for (int i = 0; i < 3; ++i)
+    strided = strided || st.q[i] != hm.q[i] || st.k[i] != hm_kv.k[i] || st.v[i] != hm_kv.v[i] ||
+              st.o[i] != hm.o[i];
+  *is_strided = strided;
+  cudaError_t e = cudaSuccess;
+  if (strided) {
+    int k_tok = 0, v_tok = 0;
+    e = make_rows_map(tq, Q, Sq, H, B, st.q, kBM, false, &lay->q_token_major, err_msg);
+    if (e == cudaSuccess) e = make_rows_map(tk, K, Sk, Hkv, B, st.k, kBM, false, &k_tok, err_msg);
+    if (e == cudaSuccess) e = make_rows_map(tv, V, Sk, Hkv, B, st.v, kBM, false, &v_tok, err_msg);
+    if (e == cudaSuccess)
+      e = make_rows_map(to, O, Sq, H, B, st.o, 32, out_f32, &lay->o_token_major, err_msg);
+    if (e != cudaSuccess) return e;
+    if (k_tok != v_tok) {
+      if (err_msg) *err_msg = "K and V must share one layout (both head-major or both token-major)";
+      return cudaErrorInvalidValue;
+    }
+    lay->kv_token_major = k_tok;
+  } else {
+    // contiguous head-major: 3-D maps {64, S, B·H}, so a ragged S is
+    // zero-filled per head, never read from the next head
+    const uint32_t box[3] = {kD, kBM, 1};
+    const uint64_t qdims[3] = {kD, static_cast<uint64_t>(Sq), static_cast<uint64_t>(B) * H};
+    const uint64_t qstr[2] = {kD * 2, static_cast<uint64_t>(Sq) * kD * 2};
+    const uint64_t kdims[3] = {kD, static_cast<uint64_t>(Sk), static_cast<uint64_t>(B) * Hkv};
+    const uint64_t kstr[2] = {kD * 2, static_cast<uint64_t>(Sk) * kD * 2};
+    e = make_tmap_bf16_sw128(tq, Q, 3, qdims, qstr, box, err_msg);
+    if (e == cudaSuccess) e = make_tmap_bf16_sw128(tk, K, 3, kdims, kstr, box, err_msg);
+    if (e == cudaSuccess) e = make_tmap_bf16_sw128(tv, V, 3, kdims, kstr, box, err_msg);
+    // O: boxes of 32 rows x 128 bytes (64 bf16, or 32 of 64 fp32)
+    const uint64_t esz = out_f32 ? 4 : 2;
+    const uint32_t obox[3] = {static_cast<uint32_t>(128 / esz), 32, 1};
+    const uint64_t ostr[2] = {kD * esz, static_cast<uint64_t>(Sq) * kD * esz};
+    if (e == cudaSuccess)
+      e = make_tmap_sw128(to, out_f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                          static_cast<int>(esz), O, 3, qdims, ostr, obox, err_msg);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+}  // namespace
+
 cudaError_t launch_flash_fwd(cudaStream_t stream, const __nv_bfloat16* Q, const __nv_bfloat16* K,
                              const __nv_bfloat16* V, void* O, bool out_f32, float* lse,
                              float* row_max, int B, int H, int Sq, int Sk, float scale,
@@ -805,47 +957,10 @@ cudaError_t launch_flash_fwd(cudaStream_t stream, const __nv_bfloat16* Q, const 
   if (BH == 0 || Sq == 0) return cudaSuccess;
   CUtensorMap tq, tk, tv, to;
   FlashLayout lay;
-  lay.H = H;
-  lay.q_token_major = lay.kv_token_major = lay.o_token_major = 0;
-  const FlashStrides hm = flash_head_major_strides(H, Sq, Sk);
   bool strided = false;
-  for (int i = 0; i < 3; ++i)
-    strided = strided || st.q[i] != hm.q[i] || st.k[i] != hm.k[i] || st.v[i] != hm.v[i] ||
-              st.o[i] != hm.o[i];
-  cudaError_t e = cudaSuccess;
-  if (strided) {
-    int k_tok = 0, v_tok = 0;
-    e = make_rows_map(&tq, Q, Sq, H, B, st.q, kBM, false, &lay.q_token_major, err_msg);
-    if (e == cudaSuccess) e = make_rows_map(&tk, K, Sk, H, B, st.k, kBM, false, &k_tok, err_msg);
-    if (e == cudaSuccess) e = make_rows_map(&tv, V, Sk, H, B, st.v, kBM, false, &v_tok, err_msg);
-    if (e == cudaSuccess)
-      e = make_rows_map(&to, O, Sq, H, B, st.o, 32, out_f32, &lay.o_token_major, err_msg);
-    if (e != cudaSuccess) return e;
-    if (k_tok != v_tok) {
-      if (err_msg) *err_msg = "K and V must share one layout (both head-major or both token-major)";
-      return cudaErrorInvalidValue;
-    }
-    lay.kv_token_major = k_tok;
-  } else {
-    // contiguous head-major: 3-D maps {64, S, B·H}, so a ragged S is
-    // zero-filled per head, never read from the next head
-    const uint32_t box[3] = {kD, kBM, 1};
-    const uint64_t qdims[3] = {kD, static_cast<uint64_t>(Sq), static_cast<uint64_t>(BH)};
-    const uint64_t qstr[2] = {kD * 2, static_cast<uint64_t>(Sq) * kD * 2};
-    const uint64_t kdims[3] = {kD, static_cast<uint64_t>(Sk), static_cast<uint64_t>(BH)};
-    const uint64_t kstr[2] = {kD * 2, static_cast<uint64_t>(Sk) * kD * 2};
-    e = make_tmap_bf16_sw128(&tq, Q, 3, qdims, qstr, box, err_msg);
-    if (e == cudaSuccess) e = make_tmap_bf16_sw128(&tk, K, 3, kdims, kstr, box, err_msg);
-    if (e == cudaSuccess) e = make_tmap_bf16_sw128(&tv, V, 3, kdims, kstr, box, err_msg);
-    // O: boxes of 32 rows x 128 bytes (64 bf16, or 32 of 64 fp32)
-    const uint64_t esz = out_f32 ? 4 : 2;
-    const uint32_t obox[3] = {static_cast<uint32_t>(128 / esz), 32, 1};
-    const uint64_t ostr[2] = {kD * esz, static_cast<uint64_t>(Sq) * kD * esz};
-    if (e == cudaSuccess)
-      e = make_tmap_sw128(&to, out_f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
-                          static_cast<int>(esz), O, 3, qdims, ostr, obox, err_msg);
-    if (e != cudaSuccess) return e;
-  }
+  const cudaError_t e = make_maps(Q, K, V, O, out_f32, B, H, H, Sq, Sk, st, &tq, &tk, &tv, &to,
+                                  &lay, &strided, err_msg);
+  if (e != cudaSuccess) return e;
   const float sl2 = scale * kLog2e;
 #define ND_FLASH_LAUNCH(C, F, S_)                                                              \
   launch_typed<C, F, S_>(stream, tq, tk, tv, to, lay, lse, row_max, BH, Sq, Sk, sl2)
@@ -856,6 +971,32 @@ cudaError_t launch_flash_fwd(cudaStream_t stream, const __nv_bfloat16* Q, const 
   if (causal) return out_f32 ? ND_FLASH_LAUNCH(true, true, false) : ND_FLASH_LAUNCH(true, false, false);
   return out_f32 ? ND_FLASH_LAUNCH(false, true, false) : ND_FLASH_LAUNCH(false, false, false);
 #undef ND_FLASH_LAUNCH
+}
+
+cudaError_t launch_window_fwd(cudaStream_t stream, const __nv_bfloat16* Q, const __nv_bfloat16* K,
+                              const __nv_bfloat16* V, void* O, bool out_f32, float* lse,
+                              float* row_max, int B, int H, int Hkv, int Sq, int Sk, float scale,
+                              int window, int sinks, const FlashStrides& st,
+                              const char** err_msg) {
+  const int BH = B * H;
+  if (BH == 0 || Sq == 0) return cudaSuccess;
+  CUtensorMap tq, tk, tv, to;
+  FlashLayout lay;
+  bool strided = false;
+  const cudaError_t e = make_maps(Q, K, V, O, out_f32, B, H, Hkv, Sq, Sk, st, &tq, &tk, &tv, &to,
+                                  &lay, &strided, err_msg);
+  if (e != cudaSuccess) return e;
+  FlashWindow win;
+  win.window = window < Sk ? window : Sk;
+  win.sinks = sinks < Sk ? sinks : Sk;
+  win.group = H / Hkv;
+  win.off = Sk - Sq;
+  const float sl2 = scale * kLog2e;
+#define ND_WINDOW_LAUNCH(F, S_)                                                                   \
+  launch_typed<true, F, S_, true>(stream, tq, tk, tv, to, lay, lse, row_max, BH, Sq, Sk, sl2, win)
+  if (strided) return out_f32 ? ND_WINDOW_LAUNCH(true, true) : ND_WINDOW_LAUNCH(false, true);
+  return out_f32 ? ND_WINDOW_LAUNCH(true, false) : ND_WINDOW_LAUNCH(false, false);
+#undef ND_WINDOW_LAUNCH
 }
 
 }  // namespace nd

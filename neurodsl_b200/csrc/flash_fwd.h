@@ -25,4 +25,12 @@ cudaError_t launch_flash_fwd(cudaStream_t stream, const __nv_bfloat16* Q, const 
                              float* row_max, int B, int H, int Sq, int Sk, float scale,
                              bool causal, const FlashStrides& st, const char** err_msg);
 
+// Sliding window with sinks: query i is at position p = Sk - Sq + i (Sq <= Sk)
+// and sees key j when j <= p and (j > p - window or j < sinks).  K and V have
+// Hkv heads, query head h reads head h / (H / Hkv).  window >= 1, sinks >= 0.
+cudaError_t launch_window_fwd(cudaStream_t stream, const __nv_bfloat16* Q, const __nv_bfloat16* K,
+                              const __nv_bfloat16* V, void* O, bool out_f32, float* lse,
+                              float* row_max, int B, int H, int Hkv, int Sq, int Sk, float scale,
+                              int window, int sinks, const FlashStrides& st, const char** err_msg);
+
 }  // namespace nd

@@ -564,6 +564,345 @@ def add_layernorm(x, p, bias=None, gamma=None, beta=None, eps=1e-5, s_out=None, 
     return s_out, out
 
 
+# ---- sliding window, paged cache and logits penalties -------------------------
+def _same_device(first, name, **tensors):
+    """Every given tensor is a CUDA tensor on the device of `first`."""
+    if not isinstance(first, torch.Tensor) or not first.is_cuda:
+        raise TypeError(f"{name} must be a CUDA tensor")
+    dev = first.device
+    for n, t in tensors.items():
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise TypeError(f"{n} must be a CUDA tensor")
+        if t.device != dev:
+            raise ValueError(f"{n} is on {t.device}, {name} on {dev}")
+    return dev
+
+
+class _on:
+    """Makes the tensors' device current for a call and names its stream: the
+    caller's, which must be one of that device, or that device's current one."""
+
+    def __init__(self, dev, stream):
+        if stream is not None and stream.device != dev:
+            raise ValueError(f"stream is on {stream.device}, the tensors on {dev}")
+        self.dev, self.stream, self.prev = dev, stream, -1
+
+    def __enter__(self):
+        cur = torch.cuda.current_device()
+        if self.dev.index != cur:
+            self.prev = cur
+            torch.cuda.set_device(self.dev)
+        s = self.stream if self.stream is not None else torch.cuda.current_stream(self.dev)
+        return s.cuda_stream
+
+    def __exit__(self, *exc):
+        if self.prev >= 0:
+            torch.cuda.set_device(self.prev)
+        return False
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
+def window_attn_fwd(Q, K, V, window, sinks=0, scale=None, out=None, out_dtype=torch.bfloat16,
+                    lse=None, row_max=None, stream=None):
+    """Causal attention with a sliding window and sinks (nd_window_attn_fwd):
+    Q [B][H][Sq][64], K and V [B][Hkv][Sk][64] bf16, H a multiple of Hkv,
+    Sq <= Sk; the queries are the last Sq positions, and the query at position
+    p sees key j when j <= p and (j > p - window or j < sinks).
+
+    Returns (O, lse, row_max) like flash_attn_fwd, and like there Q, K, V and
+    `out` may be strided views (a fused projection, a longer cache)."""
+    for n, t in (("Q", Q), ("K", K), ("V", V)):
+        _need(t, n, torch.bfloat16, 4, contiguous=False)
+    dev = _same_device(Q, "Q", K=K, V=V, out=out, lse=lse, row_max=row_max)
+    B, H, Sq, D = Q.shape
+    Hkv, Sk = K.shape[1], K.shape[2]
+    if K.shape != (B, Hkv, Sk, D) or V.shape != K.shape:
+        raise ValueError(f"shape mismatch Q{tuple(Q.shape)} K{tuple(K.shape)} V{tuple(V.shape)}")
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    if out is None:
+        out = torch.empty((B, H, Sq, D), dtype=out_dtype, device=dev)
+    if out.dtype not in _DT or out.shape != Q.shape:
+        raise ValueError(f"out must be float32 or bfloat16 {tuple(Q.shape)}")
+    stats = []
+    for n, t in (("lse", lse), ("row_max", row_max)):
+        if t is None:
+            t = torch.empty((B, H, Sq), dtype=torch.float32, device=dev)
+        _need(t, n, torch.float32)
+        if t.numel() != B * H * Sq:
+            raise ValueError(f"{n} must have B*H*Sq = {B * H * Sq} values")
+        stats.append(t)
+    with _on(dev, stream) as st:
+        check(_lib.load().nd_window_attn_fwd(
+            st, _addr(Q), _row_strides(Q, "Q"), _addr(K), _row_strides(K, "K"), _addr(V),
+            _row_strides(V, "V"), _addr(out), _row_strides(out, "out"), _DT[out.dtype],
+            _addr(stats[0]), _addr(stats[1]), B, H, Hkv, Sq, Sk, D, float(scale), int(window),
+            int(sinks)))
+    return out, stats[0], stats[1]
+
+
+def _need_pool(k_pages, v_pages, block_table, B):
+    _need(k_pages, "k_pages", torch.bfloat16, 4)
+    _need(v_pages, "v_pages", torch.bfloat16, 4)
+    if v_pages.shape != k_pages.shape:
+        raise ValueError("k_pages and v_pages differ in shape")
+    _need_table(block_table, "block_table", B)
+
+
+def _need_table(table, name, B):
+    _need(table, name, torch.int32, 2, contiguous=False)
+    if table.shape[0] != B or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError(f"{name} must be [{B}][pages] with contiguous rows")
+
+
+def _table_ld(table):
+    return table.stride(0) if table.shape[0] > 1 else table.shape[1]
+
+
+def _need_lens(t, name, B):
+    _need(t, name, torch.int32, 1)
+    if t.numel() != B:
+        raise ValueError(f"{name} must have {B} values")
+
+
+def paged_decode_workspace_size(B, H, Hkv, max_len, weights=False, D=64):
+    n = ctypes.c_size_t(0)
+    check(_lib.load().nd_paged_decode_workspace_size(B, H, Hkv, int(max_len), D,
+                                                     int(bool(weights)), ctypes.byref(n)))
+    return n.value
+
+
+def paged_decode_workspace(B, H, Hkv, max_len, weights=False, device=None):
+    """A zero-filled workspace for paged_decode_attn calls of up to these
+    sizes (max_len: pages a sequence times page_size; weights: for calls that
+    accumulate them).  Every call leaves it ready for the next; calls that may
+    run at the same time, two captured graphs' among them, need one each."""
+    n = paged_decode_workspace_size(B, H, Hkv, max_len, weights)
+    return torch.zeros(n, dtype=torch.uint8, device=device if device is not None else "cuda")
+
+
+def paged_decode_attn(q, k_pages, v_pages, block_table, lens, k_new=None, v_new=None, window=0,
+                      sinks=0, scale=None, out=None, out_dtype=torch.bfloat16, lse=None,
+                      want_lse=True, weights=None, workspace=None, stream=None):
+    """Decode attention of one new token per sequence over a paged cache
+    (nd_paged_decode_attn): q [B][H][64], pages [n_pages][Hkv][page_size][64]
+    bf16, block_table [B][max_pages] and lens [B] int32 on the device.
+
+    With k_new / v_new [B][Hkv][64] the token at lens - 1 is appended in the
+    same pass.  window > 0 sees the last `window` keys and the first `sinks`.
+    weights [B][Hkv][>= max_pages * page_size] fp32 gains every visible key's
+    attention weight, summed over its group's query heads.  workspace: from
+    paged_decode_workspace, kept by the caller from call to call; without one
+    each call makes its own.  Returns (out [B][H][64], lse [B][H] or None)."""
+    _need(q, "q", torch.bfloat16, 3)
+    B, H, D = q.shape
+    _need_pool(k_pages, v_pages, block_table, B)
+    dev = _same_device(q, "q", k_pages=k_pages, v_pages=v_pages, block_table=block_table,
+                       lens=lens, k_new=k_new, v_new=v_new, out=out, lse=lse, weights=weights,
+                       workspace=workspace)
+    n_pages, Hkv, page_size, Dk = k_pages.shape
+    max_pages = block_table.shape[1]
+    if Dk != D:
+        raise ValueError(f"q has head_dim {D}, the pages {Dk}")
+    _need_lens(lens, "lens", B)
+    if (k_new is None) != (v_new is None):
+        raise ValueError("k_new and v_new go together")
+    if k_new is not None:
+        for n, t in (("k_new", k_new), ("v_new", v_new)):
+            _need(t, n, torch.bfloat16, 3)
+            if t.shape != (B, Hkv, D):
+                raise ValueError(f"{n} must be {(B, Hkv, D)}, got {tuple(t.shape)}")
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    if out is None:
+        out = torch.empty((B, H, D), dtype=out_dtype, device=dev)
+    _need(out, "out")
+    if out.shape != q.shape or out.dtype not in _DT:
+        raise ValueError(f"out must be float32 or bfloat16 {tuple(q.shape)}")
+    if lse is None and want_lse:
+        lse = torch.empty((B, H), dtype=torch.float32, device=dev)
+    if lse is not None:
+        _need(lse, "lse", torch.float32)
+        if lse.numel() != B * H:
+            raise ValueError(f"lse must have {B * H} values")
+    weights_ld = 0
+    if weights is not None:
+        _need(weights, "weights", torch.float32, 3)
+        if weights.shape[:2] != (B, Hkv):
+            raise ValueError(f"weights must be [{B}][{Hkv}][keys], got {tuple(weights.shape)}")
+        weights_ld = weights.shape[2]
+    if workspace is not None:
+        _need(workspace, "workspace")
+    with _on(dev, stream) as st:
+        if workspace is None:
+            # made on the call's stream, so that its memory is reused only after the call
+            with torch.cuda.stream(stream if stream is not None else torch.cuda.current_stream(dev)):
+                workspace = paged_decode_workspace(B, H, Hkv, max_pages * page_size,
+                                                   weights is not None, device=dev)
+        check(_lib.load().nd_paged_decode_attn(
+            st, _addr(q), _addr(k_new), _addr(v_new), _addr(k_pages), _addr(v_pages), n_pages,
+            page_size, _addr(block_table), _table_ld(block_table), max_pages, _addr(lens),
+            _addr(out), _DT[out.dtype], _addr(lse), _addr(weights), weights_ld, B, H, Hkv, D,
+            int(window), int(sinks), float(scale), _addr(workspace),
+            workspace.numel() * workspace.element_size()))
+    return out, lse
+
+
+def paged_kv_store(src, k_col, v_col, k_pages, v_pages, block_table, B, S, pos0=0, lens=None,
+                   stream=None):
+    """K/V rows of a [B*S][ld] bf16 projection into a paged cache
+    (nd_paged_kv_store): token (b, s) goes to position pos0 + s of sequence b.
+    pos0: an int, or int32 [B] on the device; lens: int32 [B] tokens of each
+    sequence, the rest being padding (None: all S)."""
+    _need(src, "src", torch.bfloat16, 2, contiguous=False)
+    if src.shape[1] > 1 and src.stride(1) != 1:
+        raise ValueError("src rows must be contiguous")
+    if src.shape[0] != B * S:
+        raise ValueError(f"src must have B*S = {B * S} rows, got {src.shape[0]}")
+    _need_pool(k_pages, v_pages, block_table, B)
+    pos_dev = pos0 if isinstance(pos0, torch.Tensor) else None
+    dev = _same_device(src, "src", k_pages=k_pages, v_pages=v_pages, block_table=block_table,
+                       pos0=pos_dev, lens=lens)
+    if pos_dev is not None:
+        _need_lens(pos_dev, "pos0", B)
+    if lens is not None:
+        _need_lens(lens, "lens", B)
+    n_pages, Hkv, page_size, D = k_pages.shape
+    if max(k_col, v_col) + Hkv * D > src.shape[1]:
+        raise ValueError("k_col / v_col: the heads' columns do not fit src")
+    with _on(dev, stream) as st:
+        check(_lib.load().nd_paged_kv_store(
+            st, _addr(src), src.stride(0) if src.shape[0] > 1 else src.shape[1], int(k_col),
+            int(v_col), _addr(k_pages), _addr(v_pages), n_pages, page_size, _addr(block_table),
+            _table_ld(block_table), block_table.shape[1], int(B), int(S), Hkv,
+            0 if pos_dev is not None else int(pos0), _addr(pos_dev), _addr(lens), D))
+
+
+def paged_kv_evict(k_pages, v_pages, block_table, lens, weights, out_table, budget, sinks=0,
+                   recent=0, weights_out=None, kept=None, new_lens=None, stream=None):
+    """Cut every (sequence, kv head) of a paged cache to `budget` keys by
+    accumulated attention weight (nd_paged_kv_evict): the first `sinks`, the
+    last `recent` and the largest weights between stay, copied in order to
+    out_table's pages, which must be none of the source pages.
+
+    weights [B][Hkv][keys] fp32 as paged_decode_attn accumulates them.
+    Returns (kept [B][Hkv][budget] int32 positions, -1 past the last;
+    new_lens [B]; weights_out [B][Hkv][keys], the kept keys' weights first,
+    zeros behind them)."""
+    _need(lens, "lens", torch.int32, 1)
+    B = lens.numel()
+    _need_pool(k_pages, v_pages, block_table, B)
+    _need_table(out_table, "out_table", B)
+    dev = _same_device(k_pages, "k_pages", v_pages=v_pages, block_table=block_table, lens=lens,
+                       weights=weights, out_table=out_table, weights_out=weights_out, kept=kept,
+                       new_lens=new_lens)
+    n_pages, Hkv, page_size, D = k_pages.shape
+    _need(weights, "weights", torch.float32, 3)
+    if weights.shape[:2] != (B, Hkv):
+        raise ValueError(f"weights must be [{B}][{Hkv}][keys], got {tuple(weights.shape)}")
+    if weights_out is None:
+        weights_out = torch.empty_like(weights)
+    _need(weights_out, "weights_out", torch.float32, 3)
+    if weights_out.shape[:2] != (B, Hkv):
+        raise ValueError(f"weights_out must be [{B}][{Hkv}][keys]")
+    if kept is None:
+        kept = torch.empty((B, Hkv, max(0, int(budget))), dtype=torch.int32, device=dev)
+    _need(kept, "kept", torch.int32)
+    if kept.numel() != B * Hkv * budget:
+        raise ValueError(f"kept must have B*Hkv*budget = {B * Hkv * budget} values")
+    if new_lens is None:
+        new_lens = torch.empty((B,), dtype=torch.int32, device=dev)
+    _need_lens(new_lens, "new_lens", B)
+    with _on(dev, stream) as st:
+        check(_lib.load().nd_paged_kv_evict(
+            st, _addr(k_pages), _addr(v_pages), n_pages, page_size, _addr(block_table),
+            _table_ld(block_table), block_table.shape[1], _addr(lens), _addr(weights),
+            weights.shape[2], _addr(out_table), _table_ld(out_table), out_table.shape[1],
+            _addr(weights_out), weights_out.shape[2], _addr(kept), _addr(new_lens), B, Hkv, D,
+            int(budget), int(sinks), int(recent)))
+    return kept, new_lens, weights_out
+
+
+def logits_penalty(logits, history=None, history_lens=None, repetition=None, presence=None,
+                   frequency=None, bias_ids=None, bias=None, mask=None, out=None, out_dtype=None,
+                   idx=None, greedy=True, stream=None):
+    """Penalties, biases and a grammar mask on logits [rows][V], and the greedy
+    token (nd_logits_penalty, which gives the order of the operations).
+
+    history int32 [rows][n] (negative: no token), of which the first
+    history_lens [rows] count; repetition, presence, frequency fp32 [rows];
+    bias_ids int32 / bias fp32 [rows][n_bias]; mask int32 [rows][>= V/32] or
+    [>= V/32] for all rows, bit v % 32 of word v / 32 allowing token v.  `out`
+    may be `logits` itself.  Returns (out, idx int32 [rows], or None with
+    greedy=False)."""
+    _need(logits, "logits", None, 2, contiguous=False)
+    if logits.dtype not in _DT:
+        raise TypeError(f"logits dtype {logits.dtype} not supported")
+    rows, V = logits.shape
+    dev = _same_device(logits, "logits", history=history, history_lens=history_lens,
+                       repetition=repetition, presence=presence, frequency=frequency,
+                       bias_ids=bias_ids, bias=bias, mask=mask, out=out, idx=idx)
+    if out is None:
+        out = torch.empty((rows, V), dtype=out_dtype or logits.dtype, device=dev)
+    if out.dtype not in _DT or out.shape != logits.shape:
+        raise ValueError(f"out must be float32 or bfloat16 {(rows, V)}")
+    for n, t in (("logits", logits), ("out", out)):
+        if V > 1 and t.stride(1) != 1:
+            raise ValueError(f"{n} rows must be contiguous")
+        if rows > 1 and t.stride(0) < V:
+            raise ValueError(f"{n} rows overlap")
+    ld = lambda t: t.stride(0) if rows > 1 else max(V, 1)
+    n_hist = hist_ld = 0
+    if history is not None:
+        _need(history, "history", torch.int32, 2, contiguous=False)
+        n_hist = history.shape[1]
+        if history.shape[0] != rows or (n_hist > 1 and history.stride(1) != 1):
+            raise ValueError(f"history must be [{rows}][tokens] with contiguous rows")
+        hist_ld = history.stride(0) if rows > 1 else n_hist
+    if history_lens is not None:
+        _need_lens(history_lens, "history_lens", rows)
+    for n, t in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
+        if t is not None:
+            _need(t, n, torch.float32, 1)
+            if t.numel() != rows:
+                raise ValueError(f"{n} must have {rows} values")
+    n_bias = 0
+    if (bias_ids is None) != (bias is None):
+        raise ValueError("bias_ids and bias go together")
+    if bias_ids is not None:
+        _need(bias_ids, "bias_ids", torch.int32, 2)
+        _need(bias, "bias", torch.float32, 2)
+        if bias_ids.shape != bias.shape or bias.shape[0] != rows:
+            raise ValueError(f"bias_ids and bias must be [{rows}][n]")
+        n_bias = bias.shape[1]
+    mask_ld = 0
+    if mask is not None:
+        if mask.dtype not in (torch.int32, torch.uint32):
+            raise TypeError(f"mask must be int32 or uint32 words, got {mask.dtype}")
+        if mask.dim() not in (1, 2) or (mask.shape[-1] > 1 and mask.stride(-1) != 1):
+            raise ValueError("mask must be [words] or [rows][words] with contiguous rows")
+        if mask.shape[-1] < (V + 31) // 32 or (mask.dim() == 2 and mask.shape[0] != rows):
+            raise ValueError(f"mask must have {rows} rows (or one) of at least {(V + 31) // 32} words")
+        if mask.dim() == 2:
+            mask_ld = mask.stride(0) if rows > 1 else mask.shape[1]
+    if idx is None and greedy:
+        idx = torch.empty((rows,), dtype=torch.int32, device=dev)
+    if idx is not None:
+        _need_lens(idx, "idx", rows)
+    with _on(dev, stream) as st:
+        check(_lib.load().nd_logits_penalty(
+            st, _addr(logits), _DT[logits.dtype], ld(logits), rows, V, _addr(history), hist_ld,
+            n_hist, _addr(history_lens), _addr(repetition), _addr(presence), _addr(frequency),
+            _addr(bias_ids), _addr(bias), n_bias, _addr(mask), mask_ld, _addr(out),
+            _DT[out.dtype], ld(out), _addr(idx)))
+    return out, idx
+
+
 # ---- tensor-parallel reduction over NVLink peer memory ----------------------
 def comm_region_bytes(rows_max, d):
     n = ctypes.c_size_t(0)
