@@ -22,15 +22,23 @@
 // workspace, and the CTA that draws the head's last ticket joins them in
 // range order, so the result does not depend on timing.
 //
-// Inside a CTA each of four warps takes 16 keys of a tile and keeps its own
-// running max and sum; the warps join through shared memory at a head's end.
-// Keys and values go from global memory to a ring of per-lane shared-memory
-// slots by cp.async (a lane reads back only what it copied, so the ring needs
-// no barrier and has no bank conflicts) and feed mma.m16n8k16 directly: the
-// 64 dims of Q and K are assigned to fragment slots by one permutation that
-// lets a lane read 16 contiguous bytes, and V rows are paired along keys with
-// byte permutes.  The matrix unit runs far below its rate here; what counts
-// is that one instruction serves the whole group of query heads.
+// Inside a CTA a producer warp keeps a ring of tiles filled, running ahead over
+// the range whatever heads its tiles belong to, and four warps take 16 keys
+// of a tile each, with their own running max and sum; they join through shared
+// memory at a head's end while the next head's tiles are already arriving.
+// Two producers, by the page size: where a page holds whole groups of 16 rows,
+// one TMA box per group (or per tile, from 64 rows on) with the 128-byte
+// swizzle; else 16-byte cp.async pieces into the same layout.
+//
+// S = Q K^T takes Q as the 16-row operand of mma.m16n8k16 (query head = row)
+// and K's rows as they lie (ldmatrix).  The scores' fragment is then, packed to
+// bf16, the column operand of O^T = V^T P^T as it stands, with V^T by
+// transposing ldmatrix: no data moves between lanes but the row max.  The
+// matrix unit runs far below its rate; what counts is that one instruction
+// serves the whole group of query heads and that a warp's chain per tile is
+// short (an earlier form in which each lane copied its own keys by cp.async
+// spent 350 instructions per 16 keys: 85 us for the ragged batch below).
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <stdint.h>
 
@@ -38,22 +46,27 @@
 #include "model_ops.h"
 #include "paged_kv.h"
 #include "ptx.cuh"
+#include "tma.h"
 
 namespace nd {
 namespace {
 
 constexpr int kD = 64;
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
+constexpr int kWarps = 4;                       // consumer warps
+constexpr int kConsumers = kWarps * 32;
+constexpr int kThreads = kConsumers + 32;       // + the producer warp
 constexpr int kKeysPerWarp = 16;
 constexpr int kTile = kWarps * kKeysPerWarp;    // keys per tile
 constexpr int kStages = 4;                      // ring depth, in tiles
-constexpr int kStageBytes = 4096;               // one warp's 16 keys, K and V
+constexpr int kRowBytes = kD * 2;
+constexpr int kTileBytes = kTile * kRowBytes;   // K or V of a tile
+constexpr int kStageBytes = 2 * kTileBytes;
 constexpr int kMaxCtas = 512;                   // CTAs of one launch
 constexpr int kMaxRows = 16;                    // query heads of one pass
 constexpr int kPartialRow = kD + 2;             // acc[64], max, sum
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kDevErrTimeoutPaged = 6;          // a tile did not arrive in time
 
 struct Params {
   const __nv_bfloat16* q;
@@ -66,34 +79,39 @@ struct Params {
   const int* lens;
   void* out;
   float* lse;
-  float* scores;       // [B][H][cap], log2 units, or null
+  float* scores;       // [B][H][scores_ld], log2 units, or null
+  long long scores_ld; // the table's keys, rounded up to whole tiles
   float* lse2;         // [B][H], log2 units, with scores
   float* partials;
   unsigned int* tickets;
   int* err_word;
   int B, H, Hkv, G, parts;   // parts: passes of up to 16 query heads per kv head
   int n_pages, page_size, page_shift, max_pages;
+  int box;             // rows of a TMA box
   int window, sinks, min_tiles;
   float scale_log2;
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool pred) {
-  const int n = pred ? 16 : 0;   // 0: the slot is filled with zeros
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
+  const int n = there ? 16 : 0;   // 0: the piece is filled with zeros
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n)
                : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// This thread's copies so far arrive on `bar` when they have landed.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ uint4 ld_shared_v4(uint32_t a) {
-  uint4 r;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
-               : "r"(a)
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
                : "memory");
-  return r;
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
 }
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                          uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -120,207 +138,245 @@ struct Span {
   int lo;       // first tile of the window
   int n;        // tiles in all
 };
-__device__ __forceinline__ Span span_of(const Params& p, int b) {
+__device__ __forceinline__ Span make_span(const Params& p, int L) {
   Span s;
-  const long long cap = static_cast<long long>(p.max_pages) * p.page_size;
-  int L = p.lens[b];
+  const int cap = p.max_pages * p.page_size;
   s.ok = L >= 0 && L <= cap;
-  if (!s.ok) {
-    if (p.err_word && blockIdx.x == 0) atomicCAS(p.err_word, 0, kModelErrIndex);
-    L = L < 0 ? 0 : static_cast<int>(cap);
-  }
+  if (!s.ok) L = L < 0 ? 0 : cap;
   s.L = L;
   s.start = (p.window > 0 && p.window < L) ? L - p.window : 0;
   s.lo = s.start / kTile;
-  const int sinks = p.sinks < s.start ? p.sinks : s.start;
+  const int sinks = min(p.sinks, s.start);
   s.n_sink = min((sinks + kTile - 1) / kTile, s.lo);
   s.n = max(1, s.n_sink + (L + kTile - 1) / kTile - s.lo);
   return s;
 }
-__device__ __forceinline__ int key_tile(const Span& s, int j) {
-  return j < s.n_sink ? j : s.lo + j - s.n_sink;
+__device__ __forceinline__ bool visible(const Params& p, const Span& s, int key) {
+  return key < s.L && (key >= s.start || key < p.sinks);
+}
+// Whether the n keys from key0 on hold a visible one / are all visible.  The
+// table is read only for the former: a page below the window may have been
+// given back.
+__device__ __forceinline__ bool any_visible(const Params& p, const Span& s, int key0, int n) {
+  return key0 < s.L && (key0 + n > s.start || key0 < p.sinks);
+}
+__device__ __forceinline__ bool all_visible(const Params& p, const Span& s, int key0, int n) {
+  return key0 + n <= s.L && (key0 >= s.start || key0 + n <= p.sinks);
 }
 
 // A place in the row of all tiles: tile j of pass `hp` (kv head and group of
 // query heads) of sequence b.
 struct Cursor {
   int b, hp, j;
+  int next_len;     // of sequence b + 1, read well before it is needed
   Span s;
+  __device__ __forceinline__ int key_tile() const {
+    return j < s.n_sink ? j : s.lo + j - s.n_sink;
+  }
+};
+__device__ __forceinline__ void next_tile(const Params& p, int heads, Cursor& c) {
+  if (++c.j < c.s.n) return;
+  c.j = 0;
+  if (++c.hp < heads) return;
+  c.hp = 0;
+  if (++c.b >= p.B) return;
+  c.s = make_span(p, c.next_len);
+  if (c.b + 1 < p.B) c.next_len = p.lens[c.b + 1];
+}
+
+// What every warp works out for itself: the tiles of all heads, how many CTAs
+// share them, and this CTA's range of them.  (No barrier: the five warps of a
+// CTA read the same few lengths.)
+struct Plan {
+  long long total, n_cta, lo, hi;
+};
+__device__ __forceinline__ Plan make_plan(const Params& p, int heads, Cursor& c) {
+  const int lane = threadIdx.x & 31;
+  const int per = (p.B + 31) / 32;
+  const int b0 = lane * per, b1 = min(p.B, b0 + per);
+  long long mine = 0;
+  for (int b = b0; b < b1; ++b) {
+    const Span s = make_span(p, p.lens[b]);
+    if (!s.ok && p.err_word && blockIdx.x == 0) atomicCAS(p.err_word, 0, kModelErrIndex);
+    mine += s.n;
+  }
+  long long upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += x;
+  }
+  Plan r;
+  r.total = __shfl_sync(0xffffffffu, upto, 31) * heads;
+  r.n_cta = (r.total + p.min_tiles - 1) / p.min_tiles;
+  if (r.n_cta > gridDim.x) r.n_cta = gridDim.x;
+  r.lo = r.hi = 0;
+  if (static_cast<long long>(blockIdx.x) >= r.n_cta) return r;
+  r.lo = r.total * blockIdx.x / r.n_cta;
+  r.hi = r.total * (blockIdx.x + 1) / r.n_cta;
+  // the sequence of the range's first tile
+  long long at = upto - mine;
+  const bool here = at * heads <= r.lo && r.lo < upto * heads;
+  int b = b0;
+  if (here)
+    for (int n; r.lo >= (at + (n = make_span(p, p.lens[b]).n)) * heads; ++b) at += n;
+  const int src = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+  c.b = __shfl_sync(0xffffffffu, b, src);
+  const long long in = r.lo - __shfl_sync(0xffffffffu, at, src) * heads;
+  c.s = make_span(p, p.lens[c.b]);
+  c.next_len = c.b + 1 < p.B ? p.lens[c.b + 1] : 0;
+  c.hp = static_cast<int>(in / c.s.n);
+  c.j = static_cast<int>(in - static_cast<long long>(c.hp) * c.s.n);
+  return r;
+}
+
+// The row of a key in the pool; -1 (and the error word) if its page is none of
+// the pool's.
+__device__ __forceinline__ long long pool_row(const Params& p, int b, int h, int key) {
+  const int page = p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
+  const int id = p.table[b * p.table_ld + page];
+  if (id < 0 || id >= p.n_pages) {
+    if (p.err_word) atomicCAS(p.err_word, 0, kModelErrIndex);
+    return -1;
+  }
+  return (static_cast<long long>(id) * p.Hkv + h) * p.page_size + (key - page * p.page_size);
+}
+
+struct Bars {
+  uint64_t full[kStages];    // a tile has landed
+  uint64_t empty[kStages];   // the four consumer warps have read it
+  int abort_flag;
 };
 
-template <int kRows, bool kOutF32, bool kWholePage>
-__global__ void __launch_bounds__(kThreads, kRows == 8 ? 3 : 2) paged_decode_kernel(const Params p) {
-  extern __shared__ __align__(16) uint8_t ring[];
-  __shared__ long long sm_sum[kThreads];
-  __shared__ long long sm_first;   // tiles before the CTA's first sequence
-  __shared__ int sm_b;
+// ---- the producer warp: every tile of the range into the ring, in order.
+// Rows without a visible key are not copied (their stage bytes are whatever was
+// there; the consumers mask them), rows of a page outside the pool are zeros.
+template <bool kTma>
+__device__ __forceinline__ void produce(const Params& p, const CUtensorMap* tm_k,
+                                        const CUtensorMap* tm_v, int heads, Cursor c, int n_tiles,
+                                        uint8_t* ring, Bars* bars) {
+  const int lane = threadIdx.x & 31;
+  volatile int* abort_flag = &bars->abort_flag;
+  // what a lane fetches: with TMA, box `lane` of the tile; else rows lane and
+  // lane + 32.  Looked up one tile ahead.
+  long long row[2] = {-2, -2};     // -2: nothing to copy, -1: zeros
+  auto look_up = [&](const Cursor& x) {
+    const int key0 = x.key_tile() * kTile, h = x.hp / p.parts;
+    if constexpr (kTma) {
+      const int key = key0 + lane * p.box;
+      row[0] = lane * p.box < kTile && any_visible(p, x.s, key, p.box) ? pool_row(p, x.b, h, key) : -2;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int key = key0 + lane + 32 * i;
+        row[i] = visible(p, x.s, key) ? pool_row(p, x.b, h, key) : -2;
+      }
+    }
+  };
+  look_up(c);
+  bool ok = true;
+  int it = 0;
+  for (; it < n_tiles; ++it) {
+    const int s = it % kStages;
+    if (it >= kStages && !warp_wait(&bars->empty[s], ((it / kStages) - 1) & 1, abort_flag)) {
+      ok = false;
+      break;
+    }
+    uint8_t* dst = ring + s * kStageBytes;
+    if constexpr (kTma) {
+      const bool go = row[0] != -2;
+      const unsigned n = __popc(__ballot_sync(0xffffffffu, go));
+      if (lane == 0) mbar_arrive_expect_tx(&bars->full[s], n * p.box * 2 * kRowBytes);
+      if (go) {
+        // a box that starts past the pool's last row reads as zeros
+        const int r = static_cast<int>(row[0] < 0 ? static_cast<long long>(p.n_pages) * p.Hkv * p.page_size
+                                                  : row[0]);
+        tma_load_2d(tm_k, &bars->full[s], dst + lane * p.box * kRowBytes, 0, r);
+        tma_load_2d(tm_v, &bars->full[s], dst + kTileBytes + lane * p.box * kRowBytes, 0, r);
+      }
+    } else {
+      const int piece = lane & 7;
+#pragma unroll 4
+      for (int i = 0; i < kTile / 4; ++i) {
+        const int r = 4 * i + (lane >> 3);
+        const long long src = __shfl_sync(0xffffffffu, i < kTile / 8 ? row[0] : row[1], r & 31);
+        if (src == -2) continue;
+        const size_t off = static_cast<size_t>(src < 0 ? 0 : src) * kD + piece * 8;
+        const uint32_t to = smem_u32(dst) + r * kRowBytes + ((piece ^ (r & 7)) << 4);
+        cp_async16(to, p.k + off, src >= 0);
+        cp_async16(to + kTileBytes, p.v + off, src >= 0);
+      }
+      cp_async_arrive(&bars->full[s]);
+    }
+    if (it + 1 < n_tiles) {
+      next_tile(p, heads, c);
+      look_up(c);
+    }
+  }
+  if (!ok) {
+    raise_abort(abort_flag, p.err_word, kDevErrTimeoutPaged);
+    // what was issued lands before the CTA may exit
+    for (int i = it > kStages ? it - kStages : 0; i < it; ++i)
+      (void)warp_wait(&bars->full[i % kStages], (i / kStages) & 1, abort_flag);
+  }
+}
+
+template <int kRows, bool kOutF32, bool kTma>
+__global__ void __launch_bounds__(kThreads, kRows == 8 ? 3 : 2)
+    paged_decode_kernel(const Params p, const __grid_constant__ CUtensorMap tm_k,
+                        const __grid_constant__ CUtensorMap tm_v) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ Bars bars;
   __shared__ float sm_m[kWarps][kRows], sm_l[kWarps][kRows];
   __shared__ float sm_o[kWarps][kRows][kD + 4];
   __shared__ unsigned int sm_ticket;
+  uint8_t* ring = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g = lane >> 2, q4 = lane & 3;
   const int heads = p.Hkv * p.parts;
-
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&bars.full[s], kTma ? 1 : 32);
+      mbar_init(&bars.empty[s], kWarps);
+    }
+    bars.abort_flag = 0;
+    fence_barrier_init();
+  }
   pdl_wait();
   pdl_trigger();
-
-  // ---- this CTA's range: sum every sequence's tiles, deal them out evenly
-  const int per = (p.B + kThreads - 1) / kThreads;
-  {
-    long long mine = 0;
-    for (int b = threadIdx.x * per; b < min(p.B, (static_cast<int>(threadIdx.x) + 1) * per); ++b)
-      mine += span_of(p, b).n;
-    sm_sum[threadIdx.x] = mine;
-  }
-  __syncthreads();
-  // inclusive scan by the first warp, four sums a lane
-  if (warp == 0) {
-    long long v[4], run = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      run += sm_sum[lane * 4 + i];
-      v[i] = run;
-    }
-    long long base = run;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long x = __shfl_up_sync(0xffffffffu, base, o);
-      if (lane >= o) base += x;
-    }
-    base -= run;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) sm_sum[lane * 4 + i] = base + v[i];
-  }
-  __syncthreads();
-  const long long total = sm_sum[kThreads - 1] * heads;
-  long long n_cta = (total + p.min_tiles - 1) / p.min_tiles;
-  if (n_cta > gridDim.x) n_cta = gridDim.x;
-  if (static_cast<long long>(blockIdx.x) >= n_cta) return;
-  const long long cta = blockIdx.x;
-  const long long lo = total * cta / n_cta, hi = total * (cta + 1) / n_cta;
-  {
-    const long long before = threadIdx.x == 0 ? 0 : sm_sum[threadIdx.x - 1];
-    if (before * heads <= lo && lo < sm_sum[threadIdx.x] * heads) {
-      long long at = before;
-      int b = threadIdx.x * per;
-      for (int n; lo >= (at + (n = span_of(p, b).n)) * heads; ++b) at += n;
-      sm_b = b;
-      sm_first = at;
-    }
-  }
   __syncthreads();
 
-  Cursor c;                 // the tile being computed
-  c.b = sm_b;
-  c.s = span_of(p, c.b);
-  long long head_start;     // first tile of the head being computed
-  {
-    const long long in = lo - sm_first * heads;
-    c.hp = static_cast<int>(in / c.s.n);
-    c.j = static_cast<int>(in - static_cast<long long>(c.hp) * c.s.n);
-    head_start = lo - c.j;
+  Cursor c;
+  const Plan plan = make_plan(p, heads, c);
+  const long long lo = plan.lo, hi = plan.hi, n_cta = plan.n_cta;
+  if (lo == hi) return;
+  if (warp == kWarps) {
+    if constexpr (kTma) {
+      // rows written by earlier kernels' ordinary stores, read by bulk copies
+      asm volatile("fence.proxy.async.global;" ::: "memory");
+    }
+    produce<kTma>(p, &tm_k, &tm_v, heads, c, static_cast<int>(hi - lo), ring, &bars);
+    return;
   }
-  auto advance = [&](Cursor& x) {
-    if (++x.j == x.s.n) {
-      x.j = 0;
-      if (++x.hp == heads) {
-        x.hp = 0;
-        if (++x.b < p.B) x.s = span_of(p, x.b);
-      }
-    }
-  };
 
-  // ---- the ring: issue() copies this warp's 16 keys of a tile into a stage
-  const uint32_t my_ring = smem_u32(ring) + warp * (kStages * kStageBytes) + lane * 16;
-  auto visible = [&](const Span& s, int key) -> bool {
-    return key < s.L && (key >= s.start || key < p.sinks);
-  };
-  auto page_of = [&](int key) -> int {
-    return p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
-  };
-  // the row of a key in the pool, -1 if its page is none of the pool's
-  auto row_of = [&](int b, int h, int key, int id) -> long long {
-    const int row = key - page_of(key) * p.page_size;
-    if (id < 0 || id >= p.n_pages) {
-      if (p.err_word) atomicCAS(p.err_word, 0, kModelErrIndex);
-      return -1;
-    }
-    return (static_cast<long long>(id) * p.Hkv + h) * p.page_size + row;
-  };
-  // Whether this warp's keys from key0 hold a visible one: the table is read
-  // only for those (a page below the window may have been given back).
-  auto any_visible = [&](const Span& s, int key0) -> bool {
-    return key0 < s.L && (key0 + kKeysPerWarp > s.start || key0 < p.sinks);
-  };
-  auto page_id = [&](const Cursor& x) -> int {   // of this warp's keys (kWholePage)
-    const int key = key_tile(x.s, x.j) * kTile + warp * kKeysPerWarp;
-    return any_visible(x.s, key) ? p.table[x.b * p.table_ld + page_of(key)] : 0;
-  };
-  auto issue = [&](const Cursor& x, int stage, int id) {
-    const int key0 = key_tile(x.s, x.j) * kTile + warp * kKeysPerWarp;
-    const int h = x.hp / p.parts;
-    const uint32_t dst = my_ring + stage * kStageBytes;
-    long long row0 = 0;    // whole page: the row of key0; else the row of key0 + lane
-    if constexpr (kWholePage) {
-      if (any_visible(x.s, key0)) row0 = row_of(x.b, h, key0, id);
-    } else {
-      const int key = key0 + (lane & 15);
-      row0 = visible(x.s, key)
-                 ? row_of(x.b, h, key, p.table[x.b * p.table_ld + page_of(key)]) : -1;
-    }
-    const bool app = p.k_new != nullptr && x.s.ok && x.s.L - 1 >= key0 && x.s.L - 1 < key0 + kKeysPerWarp;
-    const size_t new_off = (static_cast<size_t>(x.b) * p.Hkv + h) * kD;
-    auto copy = [&](const __nv_bfloat16* pool, const __nv_bfloat16* fresh, __nv_bfloat16* pool_w,
-                    int r, int piece, uint32_t slot) {
-      const int key = key0 + r;
-      long long row;
-      if constexpr (kWholePage)
-        row = row0 < 0 ? -1 : row0 + r;
-      else
-        row = __shfl_sync(0xffffffffu, row0, r);
-      const __nv_bfloat16* src = pool + (row < 0 ? 0 : row) * kD + piece * 8;
-      bool there = row >= 0 && visible(x.s, key);
-      if (app && key == x.s.L - 1) {   // the new token: from k_new / v_new, and into its page
-        src = fresh + new_off + piece * 8;
-        if (row >= 0 && x.hp % p.parts == 0)
-          *reinterpret_cast<uint4*>(pool_w + row * kD + piece * 8) =
-              *reinterpret_cast<const uint4*>(src);
-        there = true;
-      }
-      cp_async16(dst + slot * 512, src, there);
-    };
+  // ---- consumers
+  const int g = lane >> 2, q4 = lane & 3;
+  volatile int* abort_flag = &bars.abort_flag;
+  // ldmatrix: lane's row of the warp's 16 and its 16-byte piece, swizzled;
+  // matrices 0/1: keys 0-7, pieces 2s and 2s + 1; matrices 2/3: keys 8-15
+  uint32_t mat[4];
+  {
+    const uint32_t r = (lane & 7) + ((lane >> 4) << 3);
+    const uint32_t base = smem_u32(ring) + (warp * kKeysPerWarp + r) * kRowBytes;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int c2 = 0; c2 < 2; ++c2) copy(p.k, p.k_new, p.k, g + 8 * t, q4 + 4 * c2, t * 2 + c2);
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) copy(p.v, p.v_new, p.v, 8 * t + 2 * q4 + e, g, 4 + t * 2 + e);
-  };
-
-  Cursor pre = c;           // the next tile to copy
-  long long pre_at = lo;
-  int pre_id = 0;
-  if constexpr (kWholePage) pre_id = page_id(pre);
-  auto issue_next = [&](int stage) {
-    if (pre_at < hi) {
-      issue(pre, stage, pre_id);
-      ++pre_at;
-      if (pre_at < hi) {
-        advance(pre);
-        if constexpr (kWholePage) pre_id = page_id(pre);
-      }
-    }
-    cp_async_commit();
-  };
-#pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) issue_next(s);
-
-  // ---- heads of the range, one after the other
+    for (int s = 0; s < 4; ++s) mat[s] = base + (((2 * s + ((lane >> 3) & 1)) ^ (lane & 7)) << 4);
+  }
+  constexpr int kR = kRows > 8 ? 2 : 1;       // rows per lane: g, g + 8
+  bool ok = true;          // after a lost tile the rest runs on without waiting
+  int it = 0;              // tiles taken from the ring
   long long at = lo;
-  int stage = 0;
+  long long head_start = lo - c.j;
   while (at < hi) {
     const long long head_end = head_start + c.s.n;
     const long long seg_end = head_end < hi ? head_end : hi;
@@ -328,139 +384,184 @@ __global__ void __launch_bounds__(kThreads, kRows == 8 ? 3 : 2) paged_decode_ker
     const int rows = min(p.G - row_base, kRows);
     const int head0 = h * p.G + row_base;       // query head of row 0
 
-    // Q fragments: rows g and g + 8, dims in the order K is read
-    uint32_t qa[2][8];
+    // Q fragments: rows g and g + 8; k step s takes dims 16 s + 2 q4 and + 8
+    uint32_t qa[kR][8];
 #pragma unroll
-    for (int r = 0; r < (kRows > 8 ? 2 : 1); ++r) {
-      uint4 x0 = make_uint4(0, 0, 0, 0), x1 = x0;
-      if (g + 8 * r < rows) {
-        const uint4* src = reinterpret_cast<const uint4*>(
-            p.q + (static_cast<size_t>(c.b) * p.H + head0 + g + 8 * r) * kD);
-        x0 = src[q4];
-        x1 = src[q4 + 4];
-      }
-      qa[r][0] = x0.x; qa[r][1] = x0.y; qa[r][2] = x0.z; qa[r][3] = x0.w;
-      qa[r][4] = x1.x; qa[r][5] = x1.y; qa[r][6] = x1.z; qa[r][7] = x1.w;
+    for (int r = 0; r < kR; ++r) {
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(
+          p.q + (static_cast<size_t>(c.b) * p.H + head0 + g + 8 * r) * kD);
+#pragma unroll
+      for (int s = 0; s < 8; ++s) qa[r][s] = g + 8 * r < rows ? src[4 * s + q4] : 0u;
     }
-    constexpr int kR = kRows > 8 ? 2 : 1;       // rows per lane
-    float m[kR], l[kR], o[8][4];
+    // o[r][i] holds, of rows 8 r + 2 q4 and 8 r + 2 q4 + 1, the dims 16 i + g
+    // and 16 i + 8 + g (the C fragment of O^T)
+    float m[kR], l[kR], o[kR][4][4];
 #pragma unroll
     for (int r = 0; r < kR; ++r) {
       m[r] = -INFINITY;
       l[r] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[r][i][e] = 0.f;
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
 
-    for (; at < seg_end; ++at) {
-      issue_next((stage + kStages - 1) % kStages);
-      cp_async_wait<kStages - 1>();
-      const uint32_t src = my_ring + stage * kStageBytes;
-      stage = (stage + 1) % kStages;
-      const int key0 = key_tile(c.s, c.j) * kTile + warp * kKeysPerWarp;
+    const int n = static_cast<int>(seg_end - at);
+    for (int k = 0; k < n; ++k, ++it) {
+      const int st = it % kStages;
+      const uint32_t off = st * kStageBytes;
+      const int key0 = c.key_tile() * kTile + warp * kKeysPerWarp;
+      if (k + 1 < n) ++c.j;
+      ok = ok && warp_wait(&bars.full[st], (it / kStages) & 1, abort_flag);
+      const bool full = all_visible(p, c.s, key0, kKeysPerWarp);
+      const int fresh = c.s.L - 1 - key0;          // the new token's row of the 16
+      const bool app = p.k_new != nullptr && c.s.ok && fresh >= 0 && fresh < kKeysPerWarp;
+      if (!full || app) {
+        // The border of the visible range: values of keys outside it become
+        // zeros (their weight is zero, but 0 * NaN is not), and the new token
+        // goes into the tile and into its page.
+        uint8_t* kt = ring + off + warp * kKeysPerWarp * kRowBytes;
+        uint8_t* vt = kt + kTileBytes;
+        const int piece = lane & 7;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = 4 * i + (lane >> 3);
+          if (!visible(p, c.s, key0 + r))
+            *reinterpret_cast<uint4*>(vt + r * kRowBytes + ((piece ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+        }
+        if (app && lane < 16) {
+          const __nv_bfloat16* src = (lane < 8 ? p.k_new : p.v_new) +
+                                     (static_cast<size_t>(c.b) * p.Hkv + h) * kD + piece * 8;
+          const uint4 x = *reinterpret_cast<const uint4*>(src);
+          *reinterpret_cast<uint4*>((lane < 8 ? kt : vt) + fresh * kRowBytes + ((piece ^ (fresh & 7)) << 4)) = x;
+          if (c.hp % p.parts == 0) {
+            const long long row = pool_row(p, c.b, h, c.s.L - 1);
+            if (row >= 0)
+              *reinterpret_cast<uint4*>((lane < 8 ? p.k : p.v) + row * kD + piece * 8) = x;
+          }
+        }
+        fence_async_shared();   // before the stage's next bulk copy
+        __syncwarp();
+      }
 
-      // S = Q K^T: two tiles of 8 keys, four steps of 16 dims
+      uint32_t kf[4][4], vf[4][4];
+#pragma unroll
+      for (int s = 0; s < 4; ++s) ldmatrix4(kf[s], mat[s] + off);
+#pragma unroll
+      for (int s = 0; s < 4; ++s) ldmatrix4_trans(vf[s], mat[s] + off + kTileBytes);
+      // S = Q K^T: two tiles of 8 keys, four steps of 16 dims; in log2 units
       float sc[2][4];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const uint4 k0 = ld_shared_v4(src + (t * 2) * 512), k1 = ld_shared_v4(src + (t * 2 + 1) * 512);
-        sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.f;
-        const uint32_t z = 0;
-        mma_bf16(sc[t], qa[0][0], kR > 1 ? qa[1][0] : z, qa[0][1], kR > 1 ? qa[1][1] : z, k0.x, k0.y);
-        mma_bf16(sc[t], qa[0][2], kR > 1 ? qa[1][2] : z, qa[0][3], kR > 1 ? qa[1][3] : z, k0.z, k0.w);
-        mma_bf16(sc[t], qa[0][4], kR > 1 ? qa[1][4] : z, qa[0][5], kR > 1 ? qa[1][5] : z, k1.x, k1.y);
-        mma_bf16(sc[t], qa[0][6], kR > 1 ? qa[1][6] : z, qa[0][7], kR > 1 ? qa[1][7] : z, k1.z, k1.w);
+      for (int t = 0; t < 2; ++t) sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.f;
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          mma_bf16(sc[t], qa[0][2 * s], kR > 1 ? qa[kR - 1][2 * s] : 0u, qa[0][2 * s + 1],
+                   kR > 1 ? qa[kR - 1][2 * s + 1] : 0u, kf[s][2 * t], kf[s][2 * t + 1]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.empty[st]);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 2 * kR; ++e) sc[t][e] *= p.scale_log2;
+      if (!full) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 2 * kR; ++e)
+            if (!visible(p, c.s, key0 + 8 * t + 2 * q4 + (e & 1))) sc[t][e] = -INFINITY;
       }
-      bool vis[2][2];
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) vis[t][e] = visible(c.s, key0 + 8 * t + 2 * q4 + e);
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int r = 0; r < kR; ++r)
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            sc[t][2 * r + e] = vis[t][e] ? sc[t][2 * r + e] * p.scale_log2 : -INFINITY;
       if (p.scores != nullptr) {
-        const long long cap = static_cast<long long>(p.max_pages) * p.page_size;
+        // whole tiles: a row of scores has room for them
 #pragma unroll
         for (int r = 0; r < kR; ++r)
           if (g + 8 * r < rows) {
-            float* dst = p.scores + (static_cast<size_t>(c.b) * p.H + head0 + g + 8 * r) * cap;
+            float* dst = p.scores + (static_cast<size_t>(c.b) * p.H + head0 + g + 8 * r) * p.scores_ld +
+                         key0 + 2 * q4;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
-#pragma unroll
-              for (int e = 0; e < 2; ++e)
-                if (vis[t][e]) dst[key0 + 8 * t + 2 * q4 + e] = sc[t][2 * r + e];
+              *reinterpret_cast<float2*>(dst + 8 * t) = make_float2(sc[t][2 * r], sc[t][2 * r + 1]);
           }
       }
       // running max; the accumulators follow where it rose
+      float up[kR];
+      bool rose = false;
 #pragma unroll
       for (int r = 0; r < kR; ++r) {
         float x = fmaxf(fmaxf(sc[0][2 * r], sc[0][2 * r + 1]), fmaxf(sc[1][2 * r], sc[1][2 * r + 1]));
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-        const float m_new = fmaxf(m[r], x);
-        const float base = m_new == -INFINITY ? 0.f : m_new;   // no key yet: every p is 2^-inf
-        const float alpha = exp2f(m[r] - base);
-        m[r] = m_new;
-        l[r] *= alpha;
+        up[r] = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+        rose = rose || up[r] > m[r];
+      }
+      if (__any_sync(0xffffffffu, rose)) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          o[i][2 * r] *= alpha;
-          o[i][2 * r + 1] *= alpha;
+        for (int r = 0; r < kR; ++r) {
+          const float m_new = fmaxf(m[r], up[r]);
+          const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m[r] - m_new);
+          m[r] = m_new;
+          l[r] *= alpha;
+          const float a0 = __shfl_sync(0xffffffffu, alpha, 8 * q4);        // row 2 q4
+          const float a1 = __shfl_sync(0xffffffffu, alpha, 8 * q4 + 4);    // row 2 q4 + 1
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            o[r][i][0] *= a0;
+            o[r][i][1] *= a1;
+            o[r][i][2] *= a0;
+            o[r][i][3] *= a1;
+          }
         }
+      }
+#pragma unroll
+      for (int r = 0; r < kR; ++r) {
+        const float base = m[r] == -INFINITY ? 0.f : m[r];   // no key yet: every p is 2^-inf
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float pr = exp2f(sc[t][2 * r + e] - base);
+            const float pr = fast_exp2(sc[t][2 * r + e] - base);
             sc[t][2 * r + e] = pr;
             l[r] += pr;
           }
       }
-      // O += P V.  P goes to the matrix unit in bf16 (relative error 2^-9 a
-      // weight, below the bf16 output's own rounding); an fp32 output takes
-      // P as three bf16 terms, which carry all 24 bits.
-      uint4 v0 = ld_shared_v4(src + 4 * 512), v1 = ld_shared_v4(src + 5 * 512);
-      uint4 v2 = ld_shared_v4(src + 6 * 512), v3 = ld_shared_v4(src + 7 * 512);
-      const uint32_t va[4][4] = {{v0.x, v0.y, v0.z, v0.w}, {v1.x, v1.y, v1.z, v1.w},
-                                 {v2.x, v2.y, v2.z, v2.w}, {v3.x, v3.y, v3.z, v3.w}};
+      // O^T += V^T P^T.  P goes to the matrix unit in bf16 (relative error
+      // 2^-9 a weight, below the bf16 output's own rounding).  An fp32 output
+      // takes P as three bf16 terms, which carry all 24 bits, and adds each
+      // step's product in fp32 arithmetic: the matrix unit's own accumulation
+      // cuts off low bits, a bias that grows with the number of steps.
+      uint32_t pb[kR][kOutF32 ? 3 : 1][2];
 #pragma unroll
-      for (int term = 0; term < (kOutF32 ? 3 : 1); ++term) {
-        uint32_t pa[2][2];   // [key half][row]
+      for (int r = 0; r < kR; ++r)
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            if (r >= kR) {
-              pa[t][r] = 0;
-              continue;
-            }
+          for (int x = 0; x < (kOutF32 ? 3 : 1); ++x) {
             const uint32_t w = pack_bf16x2(sc[t][2 * r], sc[t][2 * r + 1]);
-            pa[t][r] = w;
-            if constexpr (kOutF32) {   // what the rounding left
-              sc[t][2 * r] -= __uint_as_float(w << 16);
-              sc[t][2 * r + 1] -= __uint_as_float(w & 0xFFFF0000u);
-            }
+            pb[r][x][t] = w;
+            sc[t][2 * r] -= __uint_as_float(w << 16);     // what the rounding left
+            sc[t][2 * r + 1] -= __uint_as_float(w & 0xFFFF0000u);
           }
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          mma_bf16(o[2 * w], pa[0][0], pa[0][1], pa[1][0], pa[1][1],
-                   __byte_perm(va[0][w], va[1][w], 0x5410), __byte_perm(va[2][w], va[3][w], 0x5410));
-          mma_bf16(o[2 * w + 1], pa[0][0], pa[0][1], pa[1][0], pa[1][1],
-                   __byte_perm(va[0][w], va[1][w], 0x7632), __byte_perm(va[2][w], va[3][w], 0x7632));
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int r = 0; r < kR; ++r) {
+          if constexpr (kOutF32) {
+            float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int y = 2; y >= 0; --y)
+              mma_bf16(x, vf[i][0], vf[i][1], vf[i][2], vf[i][3], pb[r][y][0], pb[r][y][1]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[r][i][e] += x[e];
+          } else {
+            mma_bf16(o[r][i], vf[i][0], vf[i][1], vf[i][2], vf[i][3], pb[r][0][0], pb[r][0][1]);
+          }
         }
       }
-      if (at + 1 < seg_end) ++c.j;
     }
+    at = seg_end;
 
     // ---- the head's end in this range: join the warps
-    __syncthreads();   // the previous head's readers are done
+    named_bar_sync(1, kConsumers);   // the previous head's readers are done
 #pragma unroll
     for (int r = 0; r < kR; ++r) {
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
@@ -470,16 +571,30 @@ __global__ void __launch_bounds__(kThreads, kRows == 8 ? 3 : 2) paged_decode_ker
         sm_l[warp][g + 8 * r] = l[r];
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {    // lane q4 holds dims 16 q4 + i and 16 q4 + 8 + i
-        sm_o[warp][g + 8 * r][16 * q4 + i] = o[i][2 * r];
-        sm_o[warp][g + 8 * r][16 * q4 + 8 + i] = o[i][2 * r + 1];
-      }
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          sm_o[warp][8 * r + 2 * q4 + (e & 1)][16 * i + 8 * (e >> 1) + g] = o[r][i][e];
     }
-    __syncthreads();
+    named_bar_sync(1, kConsumers);
     const bool whole = head_start >= lo && head_end <= hi;
+    auto finish = [&](int r, int d, float mm, float ll, float oo) {
+      const size_t row = static_cast<size_t>(c.b) * p.H + head0 + r;
+      const float y = ll > 0.f ? oo / ll : 0.f;
+      if constexpr (kOutF32)
+        static_cast<float*>(p.out)[row * kD + d] = y;
+      else
+        static_cast<__nv_bfloat16*>(p.out)[row * kD + d] = __float2bfloat16_rn(y);
+      if (d == 0) {
+        const float lse2 = ll > 0.f ? mm + log2f(ll) : -INFINITY;
+        if (p.lse) p.lse[row] = lse2 * kLn2;
+        if (p.scores) p.lse2[row] = lse2;
+      }
+    };
     // slot 1 of the range where the head begins, slot 0 of every later one
-    float* part = p.partials + (cta * 2 + (head_start >= lo ? 1 : 0)) * kRows * kPartialRow;
-    for (int i = threadIdx.x; i < rows * kD; i += kThreads) {
+    float* part = p.partials + (static_cast<size_t>(blockIdx.x) * 2 + (head_start >= lo ? 1 : 0)) *
+                                   kRows * kPartialRow;
+    for (int i = threadIdx.x; i < rows * kD; i += kConsumers) {
       const int r = i / kD, d = i % kD;
       float mm = -INFINITY;
 #pragma unroll
@@ -492,17 +607,7 @@ __global__ void __launch_bounds__(kThreads, kRows == 8 ? 3 : 2) paged_decode_ker
         oo += sm_o[w][r][d] * f;
       }
       if (whole) {
-        const size_t row = static_cast<size_t>(c.b) * p.H + head0 + r;
-        const float y = ll > 0.f ? oo / ll : 0.f;
-        if constexpr (kOutF32)
-          static_cast<float*>(p.out)[row * kD + d] = y;
-        else
-          static_cast<__nv_bfloat16*>(p.out)[row * kD + d] = __float2bfloat16_rn(y);
-        if (d == 0) {
-          const float lse2 = ll > 0.f ? mm + log2f(ll) : -INFINITY;
-          if (p.lse) p.lse[row] = lse2 * kLn2;
-          if (p.scores) p.lse2[row] = lse2;
-        }
+        finish(r, d, mm, ll, oo);
       } else {
         part[r * kPartialRow + d] = oo;
         if (d == 0) {
@@ -514,45 +619,37 @@ __global__ void __launch_bounds__(kThreads, kRows == 8 ? 3 : 2) paged_decode_ker
     if (!whole) {
       // The barrier orders this CTA's partial before thread 0's ticket, whose
       // release publishes it; the last ticket's acquire sees all of them.
-      const long long c0 = ((head_start + 1) * n_cta + total - 1) / total - 1;
-      const long long c1 = (head_end * n_cta + total - 1) / total - 1;
-      __syncthreads();
+      const long long c0 = ((head_start + 1) * n_cta + plan.total - 1) / plan.total - 1;
+      const long long c1 = (head_end * n_cta + plan.total - 1) / plan.total - 1;
+      named_bar_sync(1, kConsumers);
       if (threadIdx.x == 0) sm_ticket = atom_add_acq_rel_gpu(&p.tickets[c0], 1u);
-      __syncthreads();
+      named_bar_sync(1, kConsumers);
       if (sm_ticket == static_cast<unsigned int>(c1 - c0)) {
-        auto slot = [&](long long cc) {
-          return p.partials + (cc * 2 + (cc == c0 ? 1 : 0)) * kRows * kPartialRow;
+        const int n_part = static_cast<int>(c1 - c0) + 1;
+        auto slot = [&](int x) {   // partials in range order
+          return p.partials + (static_cast<size_t>(c0 + x) * 2 + (x == 0 ? 1 : 0)) * kRows * kPartialRow;
         };
-        for (int i = threadIdx.x; i < rows * kD; i += kThreads) {
+        for (int i = threadIdx.x; i < rows * kD; i += kConsumers) {
           const int r = i / kD, d = i % kD;
           float mm = -INFINITY;
-          for (long long cc = c0; cc <= c1; ++cc)
-            mm = fmaxf(mm, __ldcg(slot(cc) + r * kPartialRow + kD));
+#pragma unroll 8
+          for (int x = 0; x < n_part; ++x) mm = fmaxf(mm, __ldcg(slot(x) + r * kPartialRow + kD));
           float ll = 0.f, oo = 0.f;
-          for (long long cc = c0; cc <= c1; ++cc) {
-            const float* x = slot(cc) + r * kPartialRow;
-            const float pm = __ldcg(x + kD);
+#pragma unroll 4
+          for (int x = 0; x < n_part; ++x) {
+            const float* s = slot(x) + r * kPartialRow;
+            const float pm = __ldcg(s + kD);
             const float f = pm == -INFINITY ? 0.f : exp2f(pm - mm);
-            ll += __ldcg(x + kD + 1) * f;
-            oo += __ldcg(x + d) * f;
+            ll += __ldcg(s + kD + 1) * f;
+            oo += __ldcg(s + d) * f;
           }
-          const size_t row = static_cast<size_t>(c.b) * p.H + head0 + r;
-          const float y = ll > 0.f ? oo / ll : 0.f;
-          if constexpr (kOutF32)
-            static_cast<float*>(p.out)[row * kD + d] = y;
-          else
-            static_cast<__nv_bfloat16*>(p.out)[row * kD + d] = __float2bfloat16_rn(y);
-          if (d == 0) {
-            const float lse2 = ll > 0.f ? mm + log2f(ll) : -INFINITY;
-            if (p.lse) p.lse[row] = lse2 * kLn2;
-            if (p.scores) p.lse2[row] = lse2;
-          }
+          finish(r, d, mm, ll, oo);
         }
         if (threadIdx.x == 0) p.tickets[c0] = 0u;   // ready for the next call
       }
     }
     if (at < hi) {
-      advance(c);
+      next_tile(p, heads, c);
       head_start = head_end;
     }
   }
@@ -569,8 +666,7 @@ __global__ void __launch_bounds__(kWeightThreads)
   pdl_wait();
   pdl_trigger();
   const int b = blockIdx.y / p.Hkv, h = blockIdx.y % p.Hkv;
-  const Span s = span_of(p, b);
-  const long long cap = static_cast<long long>(p.max_pages) * p.page_size;
+  const Span s = make_span(p, p.lens[b]);
   float* w = weights + static_cast<size_t>(blockIdx.y) * weights_ld;
   const size_t row0 = static_cast<size_t>(b) * p.H + h * p.G;
   for (int i = 0; i < kWeightKeys; i += kWeightThreads) {
@@ -578,7 +674,7 @@ __global__ void __launch_bounds__(kWeightThreads)
     if (key >= s.L || (key < s.start && key >= p.sinks)) continue;
     float x = 0.f;
     for (int g = 0; g < p.G; ++g)
-      x += exp2f(p.scores[(row0 + g) * cap + key] - p.lse2[row0 + g]);
+      x += exp2f(p.scores[(row0 + g) * p.scores_ld + key] - p.lse2[row0 + g]);
     w[key] += x;
   }
 }
@@ -590,17 +686,21 @@ size_t partials_bytes(int G) {
   return round256(static_cast<size_t>(kMaxCtas) * 2 * rows * kPartialRow * sizeof(float));
 }
 
-template <int kRows, bool kOutF32, bool kWholePage>
-cudaError_t launch_typed(cudaStream_t stream, const Params& p, long long max_tiles) {
-  auto kern = paged_decode_kernel<kRows, kOutF32, kWholePage>;
-  constexpr int smem = kWarps * kStages * kStageBytes;
+template <int kRows, bool kOutF32, bool kTma>
+cudaError_t launch_typed(cudaStream_t stream, const Params& p, long long max_tiles,
+                         const CUtensorMap& tk, const CUtensorMap& tv) {
+  auto kern = paged_decode_kernel<kRows, kOutF32, kTma>;
+  constexpr int smem = kStages * kStageBytes + 1024;   // + alignment
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   long long grid = static_cast<long long>(current_sm_count()) * (kRows == 8 ? 3 : 2);
   if (grid > kMaxCtas) grid = kMaxCtas;
   if (grid > max_tiles) grid = max_tiles;
-  return launch_ex(kern, dim3(static_cast<unsigned>(grid)), dim3(kThreads), smem, stream, 1, true, p);
+  return launch_ex(kern, dim3(static_cast<unsigned>(grid)), dim3(kThreads), smem, stream, 1, true, p,
+                   tk, tv);
 }
+
+long long scores_ld(long long max_len) { return (max_len + kTile - 1) / kTile * kTile; }
 
 }  // namespace
 
@@ -609,7 +709,7 @@ size_t paged_decode_workspace_bytes(int B, int H, int Hkv, long long max_len, bo
   size_t n = tickets_bytes() + partials_bytes(G);
   if (weights) {
     const size_t rows = static_cast<size_t>(B) * H;
-    n += round256(rows * sizeof(float)) + rows * static_cast<size_t>(max_len) * sizeof(float);
+    n += round256(rows * sizeof(float)) + rows * static_cast<size_t>(scores_ld(max_len)) * sizeof(float);
   }
   return n;
 }
@@ -647,18 +747,31 @@ cudaError_t launch_paged_decode(cudaStream_t stream, const PagedDecode& a, int* 
   ws += tickets_bytes();
   p.partials = reinterpret_cast<float*>(ws);
   ws += partials_bytes(p.G);
-  if (a.weights) {
+  if (a.weights != nullptr && a.pool.max_pages > 0) {
     p.lse2 = reinterpret_cast<float*>(ws);
     p.scores = reinterpret_cast<float*>(ws + round256(static_cast<size_t>(a.B) * a.H * sizeof(float)));
   }
   const long long cap = static_cast<long long>(p.max_pages) * p.page_size;
+  p.scores_ld = scores_ld(cap);
   const long long per_head = cap > 0 ? (cap + kTile - 1) / kTile : 1;
   const long long max_tiles = static_cast<long long>(a.B) * p.Hkv * p.parts * per_head;
-  const bool whole_page = p.page_size % kKeysPerWarp == 0;
-  cudaError_t e;
+  // TMA boxes need whole groups of 16 rows in a page and row numbers in 31 bits
+  const long long pool_rows = static_cast<long long>(p.n_pages) * p.Hkv * p.page_size;
+  const bool tma = p.page_size % kKeysPerWarp == 0 && pool_rows < (1LL << 31);
+  p.box = p.page_size % 64 == 0 ? 64 : p.page_size % 32 == 0 ? 32 : 16;
+  CUtensorMap tk = {}, tv = {};
+  cudaError_t e = cudaSuccess;
+  if (tma) {
+    const uint64_t dims[2] = {kD, static_cast<uint64_t>(pool_rows)};
+    const uint64_t strides[1] = {kRowBytes};
+    const uint32_t box[2] = {kD, static_cast<uint32_t>(p.box)};
+    e = make_tmap_bf16_sw128(&tk, p.k, 2, dims, strides, box, nullptr);
+    if (e == cudaSuccess) e = make_tmap_bf16_sw128(&tv, p.v, 2, dims, strides, box, nullptr);
+    if (e != cudaSuccess) return e;
+  }
 #define ND_PAGED(R, F)                                                        \
-  e = whole_page ? launch_typed<R, F, true>(stream, p, max_tiles)             \
-                 : launch_typed<R, F, false>(stream, p, max_tiles)
+  e = tma ? launch_typed<R, F, true>(stream, p, max_tiles, tk, tv)            \
+          : launch_typed<R, F, false>(stream, p, max_tiles, tk, tv)
   if (p.G <= 8) {
     if (a.out_f32) ND_PAGED(8, true); else ND_PAGED(8, false);
   } else {
