@@ -63,7 +63,8 @@ constexpr int kTileBytes = kTile * kRowBytes;   // K or V of a tile
 constexpr int kStageBytes = 2 * kTileBytes;
 constexpr int kMaxCtas = 512;                   // CTAs of one launch
 constexpr int kMaxRows = 16;                    // query heads of one pass
-constexpr int kPartialRow = kD + 2;             // acc[64], max, sum
+constexpr int kPartialRow = kD + 4;             // acc[64], max, sum (16-byte rows)
+constexpr int kMaxSplit = 128;                  // ranges that share a head, at most (about)
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kDevErrTimeoutPaged = 6;          // a tile did not arrive in time
@@ -188,8 +189,14 @@ __device__ __forceinline__ void next_tile(const Params& p, int heads, Cursor& c)
 // share them, and this CTA's range of them.  (No barrier: the five warps of a
 // CTA read the same few lengths.)
 struct Plan {
-  long long total, n_cta, lo, hi;
+  long long total, lo, hi;
+  int n_cta;
 };
+// a / b; in 32 bits where that holds both (a 64-bit division is a long call)
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  if ((a | b) >> 32 == 0) return static_cast<unsigned>(a) / static_cast<unsigned>(b);
+  return a / b;
+}
 __device__ __forceinline__ Plan make_plan(const Params& p, int heads, Cursor& c) {
   const int lane = threadIdx.x & 31;
   const int per = (p.B + 31) / 32;
@@ -208,12 +215,13 @@ __device__ __forceinline__ Plan make_plan(const Params& p, int heads, Cursor& c)
   }
   Plan r;
   r.total = __shfl_sync(0xffffffffu, upto, 31) * heads;
-  r.n_cta = (r.total + p.min_tiles - 1) / p.min_tiles;
-  if (r.n_cta > gridDim.x) r.n_cta = gridDim.x;
+  long long n_cta = (r.total + p.min_tiles - 1) / p.min_tiles;
+  n_cta = min(n_cta, static_cast<long long>(kMaxSplit) * p.B * heads);
+  r.n_cta = static_cast<int>(min(n_cta, static_cast<long long>(gridDim.x)));
   r.lo = r.hi = 0;
-  if (static_cast<long long>(blockIdx.x) >= r.n_cta) return r;
-  r.lo = r.total * blockIdx.x / r.n_cta;
-  r.hi = r.total * (blockIdx.x + 1) / r.n_cta;
+  if (static_cast<int>(blockIdx.x) >= r.n_cta) return r;
+  r.lo = quotient(r.total * blockIdx.x, r.n_cta);
+  r.hi = quotient(r.total * (blockIdx.x + 1), r.n_cta);
   // the sequence of the range's first tile
   long long at = upto - mine;
   const bool here = at * heads <= r.lo && r.lo < upto * heads;
@@ -225,7 +233,7 @@ __device__ __forceinline__ Plan make_plan(const Params& p, int heads, Cursor& c)
   const long long in = r.lo - __shfl_sync(0xffffffffu, at, src) * heads;
   c.s = make_span(p, p.lens[c.b]);
   c.next_len = c.b + 1 < p.B ? p.lens[c.b + 1] : 0;
-  c.hp = static_cast<int>(in / c.s.n);
+  c.hp = static_cast<int>(quotient(in, c.s.n));
   c.j = static_cast<int>(in - static_cast<long long>(c.hp) * c.s.n);
   return r;
 }
@@ -328,7 +336,7 @@ __global__ void __launch_bounds__(kThreads, kRows == 8 ? 3 : 2)
   extern __shared__ uint8_t smem_raw[];
   __shared__ Bars bars;
   __shared__ float sm_m[kWarps][kRows], sm_l[kWarps][kRows];
-  __shared__ float sm_o[kWarps][kRows][kD + 4];
+  __shared__ __align__(16) float sm_o[kWarps][kRows][kD + 4];
   __shared__ unsigned int sm_ticket;
   uint8_t* ring = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -343,13 +351,17 @@ __global__ void __launch_bounds__(kThreads, kRows == 8 ? 3 : 2)
     bars.abort_flag = 0;
     fence_barrier_init();
   }
+  if (kTma && threadIdx.x == kConsumers) {
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
   pdl_wait();
   pdl_trigger();
   __syncthreads();
 
   Cursor c;
   const Plan plan = make_plan(p, heads, c);
-  const long long lo = plan.lo, hi = plan.hi, n_cta = plan.n_cta;
+  const long long lo = plan.lo, hi = plan.hi;
   if (lo == hi) return;
   if (warp == kWarps) {
     if constexpr (kTma) {
@@ -373,6 +385,21 @@ __global__ void __launch_bounds__(kThreads, kRows == 8 ? 3 : 2)
     for (int s = 0; s < 4; ++s) mat[s] = base + (((2 * s + ((lane >> 3) & 1)) ^ (lane & 7)) << 4);
   }
   constexpr int kR = kRows > 8 ? 2 : 1;       // rows per lane: g, g + 8
+  // Q fragments: rows g and g + 8; k step s takes dims 16 s + 2 q4 and + 8.
+  // A head's are read while the head before it is computed.
+  uint32_t qa[kR][8], qn[kR][8];
+  auto load_q = [&](int b, int hp) {
+    const int base = (hp % p.parts) * kMaxRows;
+#pragma unroll
+    for (int r = 0; r < kR; ++r) {
+      const int row = base + g + 8 * r;
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(
+          p.q + (static_cast<size_t>(b) * p.H + (hp / p.parts) * p.G + row) * kD);
+#pragma unroll
+      for (int s = 0; s < 8; ++s) qn[r][s] = row < p.G ? src[4 * s + q4] : 0u;
+    }
+  };
+  load_q(c.b, c.hp);
   bool ok = true;          // after a lost tile the rest runs on without waiting
   int it = 0;              // tiles taken from the ring
   long long at = lo;
@@ -384,14 +411,20 @@ __global__ void __launch_bounds__(kThreads, kRows == 8 ? 3 : 2)
     const int rows = min(p.G - row_base, kRows);
     const int head0 = h * p.G + row_base;       // query head of row 0
 
-    // Q fragments: rows g and g + 8; k step s takes dims 16 s + 2 q4 and + 8
-    uint32_t qa[kR][8];
 #pragma unroll
-    for (int r = 0; r < kR; ++r) {
-      const uint32_t* src = reinterpret_cast<const uint32_t*>(
-          p.q + (static_cast<size_t>(c.b) * p.H + head0 + g + 8 * r) * kD);
+    for (int r = 0; r < kR; ++r)
 #pragma unroll
-      for (int s = 0; s < 8; ++s) qa[r][s] = g + 8 * r < rows ? src[4 * s + q4] : 0u;
+      for (int s = 0; s < 8; ++s) qa[r][s] = qn[r][s];
+    if (seg_end < hi) load_q(c.hp + 1 < heads ? c.b : c.b + 1, c.hp + 1 < heads ? c.hp + 1 : 0);
+    // The new token's K (lanes 0-7) and V (lanes 8-15), and its row in the
+    // pool, in hand before the head's last tile is.
+    const bool append = p.k_new != nullptr && c.s.ok && c.s.L > 0 && seg_end == head_end;
+    uint4 fresh_kv = make_uint4(0, 0, 0, 0);
+    long long fresh_row = -1;
+    if (append && lane < 16) {
+      fresh_kv = *reinterpret_cast<const uint4*>((lane < 8 ? p.k_new : p.v_new) +
+                                                 (static_cast<size_t>(c.b) * p.Hkv + h) * kD + (lane & 7) * 8);
+      if (c.hp % p.parts == 0) fresh_row = pool_row(p, c.b, h, c.s.L - 1);
     }
     // o[r][i] holds, of rows 8 r + 2 q4 and 8 r + 2 q4 + 1, the dims 16 i + g
     // and 16 i + 8 + g (the C fragment of O^T)
@@ -415,7 +448,7 @@ __global__ void __launch_bounds__(kThreads, kRows == 8 ? 3 : 2)
       ok = ok && warp_wait(&bars.full[st], (it / kStages) & 1, abort_flag);
       const bool full = all_visible(p, c.s, key0, kKeysPerWarp);
       const int fresh = c.s.L - 1 - key0;          // the new token's row of the 16
-      const bool app = p.k_new != nullptr && c.s.ok && fresh >= 0 && fresh < kKeysPerWarp;
+      const bool app = append && fresh >= 0 && fresh < kKeysPerWarp;
       if (!full || app) {
         // The border of the visible range: values of keys outside it become
         // zeros (their weight is zero, but 0 * NaN is not), and the new token
@@ -430,15 +463,9 @@ __global__ void __launch_bounds__(kThreads, kRows == 8 ? 3 : 2)
             *reinterpret_cast<uint4*>(vt + r * kRowBytes + ((piece ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
         }
         if (app && lane < 16) {
-          const __nv_bfloat16* src = (lane < 8 ? p.k_new : p.v_new) +
-                                     (static_cast<size_t>(c.b) * p.Hkv + h) * kD + piece * 8;
-          const uint4 x = *reinterpret_cast<const uint4*>(src);
-          *reinterpret_cast<uint4*>((lane < 8 ? kt : vt) + fresh * kRowBytes + ((piece ^ (fresh & 7)) << 4)) = x;
-          if (c.hp % p.parts == 0) {
-            const long long row = pool_row(p, c.b, h, c.s.L - 1);
-            if (row >= 0)
-              *reinterpret_cast<uint4*>((lane < 8 ? p.k : p.v) + row * kD + piece * 8) = x;
-          }
+          *reinterpret_cast<uint4*>((lane < 8 ? kt : vt) + fresh * kRowBytes + ((piece ^ (fresh & 7)) << 4)) = fresh_kv;
+          if (fresh_row >= 0)
+            *reinterpret_cast<uint4*>((lane < 8 ? p.k : p.v) + fresh_row * kD + piece * 8) = fresh_kv;
         }
         fence_async_shared();   // before the stage's next bulk copy
         __syncwarp();
@@ -578,73 +605,121 @@ __global__ void __launch_bounds__(kThreads, kRows == 8 ? 3 : 2)
     }
     named_bar_sync(1, kConsumers);
     const bool whole = head_start >= lo && head_end <= hi;
-    auto finish = [&](int r, int d, float mm, float ll, float oo) {
-      const size_t row = static_cast<size_t>(c.b) * p.H + head0 + r;
-      const float y = ll > 0.f ? oo / ll : 0.f;
-      if constexpr (kOutF32)
-        static_cast<float*>(p.out)[row * kD + d] = y;
-      else
-        static_cast<__nv_bfloat16*>(p.out)[row * kD + d] = __float2bfloat16_rn(y);
-      if (d == 0) {
-        const float lse2 = ll > 0.f ? mm + log2f(ll) : -INFINITY;
-        if (p.lse) p.lse[row] = lse2 * kLn2;
-        if (p.scores) p.lse2[row] = lse2;
-      }
-    };
-    // slot 1 of the range where the head begins, slot 0 of every later one
-    float* part = p.partials + (static_cast<size_t>(blockIdx.x) * 2 + (head_start >= lo ? 1 : 0)) *
-                                   kRows * kPartialRow;
-    for (int i = threadIdx.x; i < rows * kD; i += kConsumers) {
-      const int r = i / kD, d = i % kD;
-      float mm = -INFINITY;
+    // The warps' shares of value d of row r, joined.
+    auto joined = [&](int r, int d, float& mm, float& ll, float& oo) {
+      mm = -INFINITY;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, sm_m[w][r]);
-      float ll = 0.f, oo = 0.f;
+      ll = oo = 0.f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float f = sm_m[w][r] == -INFINITY ? 0.f : exp2f(sm_m[w][r] - mm);
-        ll += sm_l[w][r] * f;
-        oo += sm_o[w][r][d] * f;
+        const float x = sm_m[w][r];
+        const float f = x == -INFINITY ? 0.f : fast_exp2(x - mm);
+        if (x != -INFINITY) {   // a share without keys may not even be written
+          ll += sm_l[w][r] * f;
+          oo += sm_o[w][r][d] * f;
+        }
       }
-      if (whole) {
-        finish(r, d, mm, ll, oo);
-      } else {
+    };
+    auto finish = [&]() {
+      for (int i = threadIdx.x; i < rows * kD; i += kConsumers) {
+        const int r = i / kD, d = i % kD;
+        float mm, ll, oo;
+        joined(r, d, mm, ll, oo);
+        const size_t row = static_cast<size_t>(c.b) * p.H + head0 + r;
+        const float y = ll > 0.f ? oo / ll : 0.f;
+        if constexpr (kOutF32)
+          static_cast<float*>(p.out)[row * kD + d] = y;
+        else
+          static_cast<__nv_bfloat16*>(p.out)[row * kD + d] = __float2bfloat16_rn(y);
+        if (d == 0) {
+          const float lse2 = ll > 0.f ? mm + log2f(ll) : -INFINITY;
+          if (p.lse) p.lse[row] = lse2 * kLn2;
+          if (p.scores) p.lse2[row] = lse2;
+        }
+      }
+    };
+    if (whole) {
+      finish();
+    } else {
+      // slot 1 of the range where the head begins, slot 0 of every later one
+      float* part = p.partials + (static_cast<size_t>(blockIdx.x) * 2 + (head_start >= lo ? 1 : 0)) *
+                                     kRows * kPartialRow;
+      for (int i = threadIdx.x; i < rows * kD; i += kConsumers) {
+        const int r = i / kD, d = i % kD;
+        float mm, ll, oo;
+        joined(r, d, mm, ll, oo);
         part[r * kPartialRow + d] = oo;
         if (d == 0) {
           part[r * kPartialRow + kD] = mm;
           part[r * kPartialRow + kD + 1] = ll;
         }
       }
-    }
-    if (!whole) {
       // The barrier orders this CTA's partial before thread 0's ticket, whose
       // release publishes it; the last ticket's acquire sees all of them.
-      const long long c0 = ((head_start + 1) * n_cta + plan.total - 1) / plan.total - 1;
-      const long long c1 = (head_end * n_cta + plan.total - 1) / plan.total - 1;
+      const int c0 = static_cast<int>(quotient((head_start + 1) * plan.n_cta + plan.total - 1, plan.total)) - 1;
+      const int c1 = static_cast<int>(quotient(head_end * plan.n_cta + plan.total - 1, plan.total)) - 1;
       named_bar_sync(1, kConsumers);
       if (threadIdx.x == 0) sm_ticket = atom_add_acq_rel_gpu(&p.tickets[c0], 1u);
       named_bar_sync(1, kConsumers);
       if (sm_ticket == static_cast<unsigned int>(c1 - c0)) {
-        const int n_part = static_cast<int>(c1 - c0) + 1;
-        auto slot = [&](int x) {   // partials in range order
-          return p.partials + (static_cast<size_t>(c0 + x) * 2 + (x == 0 ? 1 : 0)) * kRows * kPartialRow;
-        };
-        for (int i = threadIdx.x; i < rows * kD; i += kConsumers) {
-          const int r = i / kD, d = i % kD;
-          float mm = -INFINITY;
-#pragma unroll 8
-          for (int x = 0; x < n_part; ++x) mm = fmaxf(mm, __ldcg(slot(x) + r * kPartialRow + kD));
-          float ll = 0.f, oo = 0.f;
-#pragma unroll 4
-          for (int x = 0; x < n_part; ++x) {
-            const float* s = slot(x) + r * kPartialRow;
-            const float pm = __ldcg(s + kD);
-            const float f = pm == -INFINITY ? 0.f : exp2f(pm - mm);
-            ll += __ldcg(s + kD + 1) * f;
-            oo += __ldcg(s + d) * f;
+        // Join the ranges' partials in an order that only their number sets.
+        // Eight groups of 16 threads (four values each): `per` rows at a time,
+        // 8 / per groups to a row, eight partials in flight a group; the
+        // groups' shares then go the way of the warps'.
+        const int n_part = c1 - c0 + 1;
+        const int group = threadIdx.x >> 4, l16 = threadIdx.x & 15;
+        const int per = rows <= 2 ? 2 : rows <= 4 ? 4 : 8;
+        const int share = group / per, shares = 8 / per;
+        for (int r = group % per; r < rows; r += per) {
+          float mm = -INFINITY, ll = 0.f;
+          float4 oo = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int x0 = share; x0 < n_part; x0 += 8 * shares) {
+            float pm[8], pl[8];
+            float4 po[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+              const int x = x0 + u * shares;
+              pm[u] = -INFINITY;
+              pl[u] = 0.f;
+              po[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (x < n_part) {
+                const float* s = p.partials + ((static_cast<size_t>(c0 + x) * 2 + (x == 0 ? 1 : 0)) * kRows + r) *
+                                                  kPartialRow;
+                pm[u] = __ldcg(s + kD);
+                pl[u] = __ldcg(s + kD + 1);
+                po[u] = __ldcg(reinterpret_cast<const float4*>(s) + l16);
+              }
+            }
+            float top = mm;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) top = fmaxf(top, pm[u]);
+            if (top == -INFINITY) continue;
+            const float a = fast_exp2(mm - top);
+            ll *= a;
+            oo.x *= a;
+            oo.y *= a;
+            oo.z *= a;
+            oo.w *= a;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+              const float f = fast_exp2(pm[u] - top);
+              ll += pl[u] * f;
+              oo.x += po[u].x * f;
+              oo.y += po[u].y * f;
+              oo.z += po[u].z * f;
+              oo.w += po[u].w * f;
+            }
+            mm = top;
           }
-          finish(r, d, mm, ll, oo);
+          *reinterpret_cast<float4*>(&sm_o[share][r][4 * l16]) = oo;
+          if (l16 == 0) {
+            sm_l[share][r] = ll;
+            for (int w = share; w < kWarps; w += shares) sm_m[w][r] = w == share ? mm : -INFINITY;
+          }
         }
+        named_bar_sync(1, kConsumers);
+        finish();
         if (threadIdx.x == 0) p.tickets[c0] = 0u;   // ready for the next call
       }
     }
