@@ -77,4 +77,18 @@ cudaError_t launch_ex(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t sm
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
+// Launch the second kernel of one entry point's pair so that it may start up
+// while the first still runs, whatever the calling thread's mode: it waits for
+// the first (pdl_wait) before it reads or writes anything.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_dependent(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
+                             cudaStream_t stream, Args&&... args) {
+  const bool was = pdl_enabled();
+  set_pdl_enabled(true);
+  const cudaError_t e =
+      launch_ex(kernel, grid, block, smem, stream, 1, true, std::forward<Args>(args)...);
+  set_pdl_enabled(was);
+  return e;
+}
+
 }  // namespace nd

@@ -15,7 +15,10 @@
 // Split: the visible keys of a (sequence, kv head) are cut into tiles of 64,
 // and the tiles of all heads, laid end to end, are dealt out in equal
 // contiguous ranges to one wave of CTAs.  So a ragged batch and a single long
-// sequence both keep every SM busy, whatever the lengths.  Every CTA sums the
+// sequence both keep every SM busy, whatever the lengths; a head counts as
+// kHeadCost tiles more than it has, for the joins at its end (without that the
+// CTAs that drew the short heads finished last: 47.5 us for the ragged batch
+// below instead of 39.9).  Every CTA sums the
 // lengths itself: they live on the device, and a host-side plan would need a
 // synchronisation.  A head wholly inside one range is written at once; a head
 // cut by range borders leaves partials (max, sum, unnormalised output) in the
@@ -64,7 +67,7 @@ constexpr int kStageBytes = 2 * kTileBytes;
 constexpr int kMaxCtas = 512;                   // CTAs of one launch
 constexpr int kMaxRows = 16;                    // query heads of one pass
 constexpr int kPartialRow = kD + 4;             // acc[64], max, sum (16-byte rows)
-constexpr int kMaxSplit = 128;                  // ranges that share a head, at most (about)
+constexpr int kHeadCost = 3;                    // what a head costs beside its tiles, in tiles
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kDevErrTimeoutPaged = 6;          // a tile did not arrive in time
@@ -89,7 +92,7 @@ struct Params {
   int B, H, Hkv, G, parts;   // parts: passes of up to 16 query heads per kv head
   int n_pages, page_size, page_shift, max_pages;
   int box;             // rows of a TMA box
-  int window, sinks, min_tiles;
+  int window, sinks;
   float scale_log2;
 };
 
@@ -175,8 +178,7 @@ struct Cursor {
     return j < s.n_sink ? j : s.lo + j - s.n_sink;
   }
 };
-__device__ __forceinline__ void next_tile(const Params& p, int heads, Cursor& c) {
-  if (++c.j < c.s.n) return;
+__device__ __forceinline__ void next_head(const Params& p, int heads, Cursor& c) {
   c.j = 0;
   if (++c.hp < heads) return;
   c.hp = 0;
@@ -184,10 +186,17 @@ __device__ __forceinline__ void next_tile(const Params& p, int heads, Cursor& c)
   c.s = make_span(p, c.next_len);
   if (c.b + 1 < p.B) c.next_len = p.lens[c.b + 1];
 }
+// On to the next tile; returns how far that is in cost.
+__device__ __forceinline__ int next_tile(const Params& p, int heads, Cursor& c) {
+  if (++c.j < c.s.n) return 1;
+  next_head(p, heads, c);
+  return 1 + kHeadCost;
+}
 
-// What every warp works out for itself: the tiles of all heads, how many CTAs
-// share them, and this CTA's range of them.  (No barrier: the five warps of a
-// CTA read the same few lengths.)
+// What every warp works out for itself: the cost of all heads, how many CTAs
+// share it, and this CTA's range [lo, hi) of it.  A head of n tiles takes
+// n + kHeadCost places, its tiles the first n.  (No barrier: the five warps of
+// a CTA read the same few lengths.)
 struct Plan {
   long long total, lo, hi;
   int n_cta;
@@ -205,7 +214,7 @@ __device__ __forceinline__ Plan make_plan(const Params& p, int heads, Cursor& c)
   for (int b = b0; b < b1; ++b) {
     const Span s = make_span(p, p.lens[b]);
     if (!s.ok && p.err_word && blockIdx.x == 0) atomicCAS(p.err_word, 0, kModelErrIndex);
-    mine += s.n;
+    mine += s.n + kHeadCost;
   }
   long long upto = mine;
 #pragma unroll
@@ -215,9 +224,13 @@ __device__ __forceinline__ Plan make_plan(const Params& p, int heads, Cursor& c)
   }
   Plan r;
   r.total = __shfl_sync(0xffffffffu, upto, 31) * heads;
-  long long n_cta = (r.total + p.min_tiles - 1) / p.min_tiles;
-  n_cta = min(n_cta, static_cast<long long>(kMaxSplit) * p.B * heads);
-  r.n_cta = static_cast<int>(min(n_cta, static_cast<long long>(gridDim.x)));
+  // A range's time grows with its tiles, the join's with the ranges of a head
+  // times its rows (32 partials of one row, or 4 of each of 16, at a time):
+  // their sum is least near sqrt(T rows / 32) tiles a range for heads of T.
+  const int rows = min(p.G, kMaxRows);
+  const float mean = static_cast<float>(r.total) / (static_cast<float>(p.B) * heads);
+  const float least = fmaxf(2.f, sqrtf(mean * (rows <= 2 ? 2 : rows <= 4 ? 4 : rows) * (1.f / 32.f)));
+  r.n_cta = static_cast<int>(fminf(ceilf(static_cast<float>(r.total) / least), static_cast<float>(gridDim.x)));
   r.lo = r.hi = 0;
   if (static_cast<int>(blockIdx.x) >= r.n_cta) return r;
   r.lo = quotient(r.total * blockIdx.x, r.n_cta);
@@ -227,14 +240,19 @@ __device__ __forceinline__ Plan make_plan(const Params& p, int heads, Cursor& c)
   const bool here = at * heads <= r.lo && r.lo < upto * heads;
   int b = b0;
   if (here)
-    for (int n; r.lo >= (at + (n = make_span(p, p.lens[b]).n)) * heads; ++b) at += n;
+    for (int n; r.lo >= (at + (n = make_span(p, p.lens[b]).n + kHeadCost)) * heads; ++b) at += n;
   const int src = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
   c.b = __shfl_sync(0xffffffffu, b, src);
   const long long in = r.lo - __shfl_sync(0xffffffffu, at, src) * heads;
   c.s = make_span(p, p.lens[c.b]);
   c.next_len = c.b + 1 < p.B ? p.lens[c.b + 1] : 0;
-  c.hp = static_cast<int>(quotient(in, c.s.n));
-  c.j = static_cast<int>(in - static_cast<long long>(c.hp) * c.s.n);
+  const int places = c.s.n + kHeadCost;
+  c.hp = static_cast<int>(quotient(in, places));
+  c.j = static_cast<int>(in - static_cast<long long>(c.hp) * places);
+  if (c.j >= c.s.n) {      // the range begins behind a head's last tile
+    r.lo += places - c.j;
+    next_head(p, heads, c);
+  }
   return r;
 }
 
@@ -261,8 +279,8 @@ struct Bars {
 // there; the consumers mask them), rows of a page outside the pool are zeros.
 template <bool kTma>
 __device__ __forceinline__ void produce(const Params& p, const CUtensorMap* tm_k,
-                                        const CUtensorMap* tm_v, int heads, Cursor c, int n_tiles,
-                                        uint8_t* ring, Bars* bars) {
+                                        const CUtensorMap* tm_v, int heads, Cursor c, long long at,
+                                        long long hi, uint8_t* ring, Bars* bars) {
   const int lane = threadIdx.x & 31;
   volatile int* abort_flag = &bars->abort_flag;
   // what a lane fetches: with TMA, box `lane` of the tile; else rows lane and
@@ -284,7 +302,7 @@ __device__ __forceinline__ void produce(const Params& p, const CUtensorMap* tm_k
   look_up(c);
   bool ok = true;
   int it = 0;
-  for (; it < n_tiles; ++it) {
+  for (; at < hi; ++it) {
     const int s = it % kStages;
     if (it >= kStages && !warp_wait(&bars->empty[s], ((it / kStages) - 1) & 1, abort_flag)) {
       ok = false;
@@ -316,10 +334,8 @@ __device__ __forceinline__ void produce(const Params& p, const CUtensorMap* tm_k
       }
       cp_async_arrive(&bars->full[s]);
     }
-    if (it + 1 < n_tiles) {
-      next_tile(p, heads, c);
-      look_up(c);
-    }
+    at += next_tile(p, heads, c);
+    if (at < hi) look_up(c);
   }
   if (!ok) {
     raise_abort(abort_flag, p.err_word, kDevErrTimeoutPaged);
@@ -361,14 +377,14 @@ __global__ void __launch_bounds__(kThreads, kRows == 8 ? 3 : 2)
 
   Cursor c;
   const Plan plan = make_plan(p, heads, c);
-  const long long lo = plan.lo, hi = plan.hi;
-  if (lo == hi) return;
+  const long long lo = plan.lo, hi = plan.hi;   // lo: the range's first tile
+  if (lo >= hi) return;
   if (warp == kWarps) {
     if constexpr (kTma) {
       // rows written by earlier kernels' ordinary stores, read by bulk copies
       asm volatile("fence.proxy.async.global;" ::: "memory");
     }
-    produce<kTma>(p, &tm_k, &tm_v, heads, c, static_cast<int>(hi - lo), ring, &bars);
+    produce<kTma>(p, &tm_k, &tm_v, heads, c, lo, hi, ring, &bars);
     return;
   }
 
@@ -415,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, kRows == 8 ? 3 : 2)
     for (int r = 0; r < kR; ++r)
 #pragma unroll
       for (int s = 0; s < 8; ++s) qa[r][s] = qn[r][s];
-    if (seg_end < hi) load_q(c.hp + 1 < heads ? c.b : c.b + 1, c.hp + 1 < heads ? c.hp + 1 : 0);
+    if (head_end + kHeadCost < hi) load_q(c.hp + 1 < heads ? c.b : c.b + 1, c.hp + 1 < heads ? c.hp + 1 : 0);
     // The new token's K (lanes 0-7) and V (lanes 8-15), and its row in the
     // pool, in hand before the head's last tile is.
     const bool append = p.k_new != nullptr && c.s.ok && c.s.L > 0 && seg_end == head_end;
@@ -723,18 +739,16 @@ __global__ void __launch_bounds__(kThreads, kRows == 8 ? 3 : 2)
         if (threadIdx.x == 0) p.tickets[c0] = 0u;   // ready for the next call
       }
     }
-    if (at < hi) {
-      next_tile(p, heads, c);
-      head_start = head_end;
-    }
+    at = head_start = head_end + kHeadCost;
+    if (at < hi) next_head(p, heads, c);
   }
 }
 
 // weights[b][h][j] += sum over the group's query heads of exp(s_j - lse), for
-// every visible key, in the heads' order.  A block takes kWeightKeys keys of
-// one (sequence, kv head).
+// every visible key, in the heads' order.  A thread takes four keys of one
+// (sequence, kv head): the scores come in 16-byte pieces.
 constexpr int kWeightThreads = 256;
-constexpr int kWeightKeys = 1024;
+constexpr int kWeightKeys = 4 * kWeightThreads;
 
 __global__ void __launch_bounds__(kWeightThreads)
     paged_weights_kernel(const Params p, float* __restrict__ weights, long long weights_ld) {
@@ -742,15 +756,32 @@ __global__ void __launch_bounds__(kWeightThreads)
   pdl_trigger();
   const int b = blockIdx.y / p.Hkv, h = blockIdx.y % p.Hkv;
   const Span s = make_span(p, p.lens[b]);
-  float* w = weights + static_cast<size_t>(blockIdx.y) * weights_ld;
+  const int key0 = blockIdx.x * kWeightKeys + threadIdx.x * 4;
+  if (!any_visible(p, s, key0, 4)) return;
+  float* w = weights + static_cast<size_t>(blockIdx.y) * weights_ld + key0;
   const size_t row0 = static_cast<size_t>(b) * p.H + h * p.G;
-  for (int i = 0; i < kWeightKeys; i += kWeightThreads) {
-    const long long key = static_cast<long long>(blockIdx.x) * kWeightKeys + i + threadIdx.x;
-    if (key >= s.L || (key < s.start && key >= p.sinks)) continue;
-    float x = 0.f;
-    for (int g = 0; g < p.G; ++g)
-      x += exp2f(p.scores[(row0 + g) * p.scores_ld + key] - p.lse2[row0 + g]);
-    w[key] += x;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int g = 0; g < p.G; ++g) {
+    const float4 y = *reinterpret_cast<const float4*>(p.scores + (row0 + g) * p.scores_ld + key0);
+    const float lse2 = p.lse2[row0 + g];
+    x.x += exp2f(y.x - lse2);
+    x.y += exp2f(y.y - lse2);
+    x.z += exp2f(y.z - lse2);
+    x.w += exp2f(y.w - lse2);
+  }
+  if (all_visible(p, s, key0, 4) && (reinterpret_cast<uintptr_t>(w) & 15) == 0) {
+    float4 y = *reinterpret_cast<float4*>(w);
+    y.x += x.x;
+    y.y += x.y;
+    y.z += x.z;
+    y.w += x.w;
+    *reinterpret_cast<float4*>(w) = y;
+  } else {
+    const float v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (visible(p, s, key0 + e)) w[e] += v[e];
   }
 }
 
@@ -815,7 +846,6 @@ cudaError_t launch_paged_decode(cudaStream_t stream, const PagedDecode& a, int* 
   p.max_pages = a.pool.max_pages;
   p.window = a.window;
   p.sinks = a.window > 0 ? a.sinks : 0;
-  p.min_tiles = 2;
   p.scale_log2 = a.scale * kLog2e;
   char* ws = static_cast<char*>(a.workspace);
   p.tickets = reinterpret_cast<unsigned int*>(ws);
@@ -856,8 +886,8 @@ cudaError_t launch_paged_decode(cudaStream_t stream, const PagedDecode& a, int* 
   if (e != cudaSuccess || a.weights == nullptr || cap == 0) return e;
   const dim3 grid(static_cast<unsigned>((cap + kWeightKeys - 1) / kWeightKeys),
                   static_cast<unsigned>(a.B * p.Hkv));
-  return launch_ex(paged_weights_kernel, grid, dim3(kWeightThreads), 0, stream, 1, true, p,
-                   a.weights, a.weights_ld);
+  return launch_dependent(paged_weights_kernel, grid, dim3(kWeightThreads), 0, stream, p, a.weights,
+                          a.weights_ld);
 }
 
 }  // namespace nd

@@ -565,46 +565,88 @@ def add_layernorm(x, p, bias=None, gamma=None, beta=None, eps=1e-5, s_out=None, 
 
 
 # ---- sliding window, paged cache and logits penalties -------------------------
-def _same_device(first, name, **tensors):
-    """Every given tensor is a CUDA tensor on the device of `first`."""
-    if not isinstance(first, torch.Tensor) or not first.is_cuda:
+# A serving step makes these calls once a layer, so their checks are written to
+# cost little: plain attribute reads, one device number for all tensors.
+_BF16, _F32, _INT32 = torch.bfloat16, torch.float32, torch.int32
+_I64x3 = ctypes.c_int64 * 3
+
+
+def _device_of(t, name):
+    """The device number of a call's first tensor."""
+    dev = t.get_device() if isinstance(t, torch.Tensor) else -1
+    if dev < 0:
         raise TypeError(f"{name} must be a CUDA tensor")
-    dev = first.device
-    for n, t in tensors.items():
-        if t is None:
-            continue
-        if not isinstance(t, torch.Tensor) or not t.is_cuda:
-            raise TypeError(f"{n} must be a CUDA tensor")
-        if t.device != dev:
-            raise ValueError(f"{n} is on {t.device}, {name} on {dev}")
     return dev
 
 
-class _on:
-    """Makes the tensors' device current for a call and names its stream: the
-    caller's, which must be one of that device, or that device's current one."""
+def _tensor(t, name, dtype, dims, dev, contiguous=True):
+    """Checks one tensor (dtype None: float32 or bfloat16; dims None: any)."""
+    d = t.get_device() if isinstance(t, torch.Tensor) else -1
+    if d != dev:
+        if d < 0:
+            raise TypeError(f"{name} must be a CUDA tensor")
+        raise ValueError(f"{name} is on cuda:{d}, the call's first tensor on cuda:{dev}")
+    dt = t.dtype
+    if dtype is None:
+        if dt not in _DT:
+            raise ValueError(f"{name} must be float32 or bfloat16, got {dt}")
+    elif dt is not dtype:
+        raise TypeError(f"{name} must be {dtype}, got {dt}")
+    if dims is not None and t.dim() != dims:
+        raise ValueError(f"{name} must have {dims} dims, got shape {tuple(t.shape)}")
+    if contiguous and not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
 
-    def __init__(self, dev, stream):
-        if stream is not None and stream.device != dev:
-            raise ValueError(f"stream is on {stream.device}, the tensors on {dev}")
-        self.dev, self.stream, self.prev = dev, stream, -1
 
-    def __enter__(self):
-        cur = torch.cuda.current_device()
-        if self.dev.index != cur:
-            self.prev = cur
-            torch.cuda.set_device(self.dev)
-        s = self.stream if self.stream is not None else torch.cuda.current_stream(self.dev)
-        return s.cuda_stream
+def _vector(t, name, dtype, n, dev):
+    _tensor(t, name, dtype, None, dev)
+    if t.numel() != n:
+        raise ValueError(f"{name} must have {n} values, got {t.numel()}")
 
-    def __exit__(self, *exc):
-        if self.prev >= 0:
-            torch.cuda.set_device(self.prev)
-        return False
+
+def _matrix(t, name, dtype, rows, dev):
+    """Checks a [rows][cols] matrix with contiguous rows; returns (cols, row stride)."""
+    _tensor(t, name, dtype, 2, dev, contiguous=False)
+    r, cols = t.shape
+    if r != rows or (cols > 1 and t.stride(1) != 1):
+        raise ValueError(f"{name} must be [{rows}][cols] with contiguous rows, got {tuple(t.shape)}")
+    ld = t.stride(0) if r > 1 else cols
+    if ld < cols:
+        raise ValueError(f"{name} rows overlap")
+    return cols, ld
+
+
+def _stream_of(dev, stream):
+    """The raw stream of a call: the caller's, which must be one of the
+    tensors' device, or that device's current one."""
+    if stream is None:
+        return torch._C._cuda_getCurrentRawStream(dev)
+    if stream.device.index != dev:
+        raise ValueError(f"stream is on {stream.device}, the tensors on cuda:{dev}")
+    return stream.cuda_stream
+
+
+def _call(fn, dev, *args):
+    """fn(*args) with the tensors' device current."""
+    if torch._C._cuda_getDevice() == dev:
+        rc = fn(*args)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args)
+    if rc:
+        check(rc)
 
 
 def _addr(t):
     return None if t is None else t.data_ptr()
+
+
+def _strides4(t, name):
+    """{row, head, batch} strides of a [B][H][S][64] view, D contiguous."""
+    b, h, s, d = t.stride()
+    if d != 1:
+        raise ValueError(f"{name}: the 64 head dims of a row must be contiguous")
+    return _I64x3(s, h, b)
 
 
 def window_attn_fwd(Q, K, V, window, sinks=0, scale=None, out=None, out_dtype=torch.bfloat16,
@@ -616,58 +658,41 @@ def window_attn_fwd(Q, K, V, window, sinks=0, scale=None, out=None, out_dtype=to
 
     Returns (O, lse, row_max) like flash_attn_fwd, and like there Q, K, V and
     `out` may be strided views (a fused projection, a longer cache)."""
-    for n, t in (("Q", Q), ("K", K), ("V", V)):
-        _need(t, n, torch.bfloat16, 4, contiguous=False)
-    dev = _same_device(Q, "Q", K=K, V=V, out=out, lse=lse, row_max=row_max)
-    B, H, Sq, D = Q.shape
-    Hkv, Sk = K.shape[1], K.shape[2]
-    if K.shape != (B, Hkv, Sk, D) or V.shape != K.shape:
+    dev = _device_of(Q, "Q")
+    _tensor(Q, "Q", _BF16, 4, dev, False)
+    _tensor(K, "K", _BF16, 4, dev, False)
+    _tensor(V, "V", _BF16, 4, dev, False)
+    B, H, Sq, D = q_shape = Q.shape
+    Bk, Hkv, Sk, Dk = k_shape = K.shape
+    if Bk != B or Dk != D or V.shape != k_shape:
         raise ValueError(f"shape mismatch Q{tuple(Q.shape)} K{tuple(K.shape)} V{tuple(V.shape)}")
-    if scale is None:
-        scale = 1.0 / math.sqrt(D)
     if out is None:
-        out = torch.empty((B, H, Sq, D), dtype=out_dtype, device=dev)
-    if out.dtype not in _DT or out.shape != Q.shape:
-        raise ValueError(f"out must be float32 or bfloat16 {tuple(Q.shape)}")
-    stats = []
-    for n, t in (("lse", lse), ("row_max", row_max)):
-        if t is None:
-            t = torch.empty((B, H, Sq), dtype=torch.float32, device=dev)
-        _need(t, n, torch.float32)
-        if t.numel() != B * H * Sq:
-            raise ValueError(f"{n} must have B*H*Sq = {B * H * Sq} values")
-        stats.append(t)
-    with _on(dev, stream) as st:
-        check(_lib.load().nd_window_attn_fwd(
-            st, _addr(Q), _row_strides(Q, "Q"), _addr(K), _row_strides(K, "K"), _addr(V),
-            _row_strides(V, "V"), _addr(out), _row_strides(out, "out"), _DT[out.dtype],
-            _addr(stats[0]), _addr(stats[1]), B, H, Hkv, Sq, Sk, D, float(scale), int(window),
-            int(sinks)))
-    return out, stats[0], stats[1]
+        out = torch.empty(q_shape, dtype=out_dtype, device=Q.device)
+    _tensor(out, "out", None, 4, dev, False)
+    if out.shape != q_shape:
+        raise ValueError(f"out must be {tuple(q_shape)}, got {tuple(out.shape)}")
+    if lse is None:
+        lse = torch.empty((B, H, Sq), dtype=_F32, device=Q.device)
+    if row_max is None:
+        row_max = torch.empty((B, H, Sq), dtype=_F32, device=Q.device)
+    _vector(lse, "lse", _F32, B * H * Sq, dev)
+    _vector(row_max, "row_max", _F32, B * H * Sq, dev)
+    _call(_lib.load().nd_window_attn_fwd, dev, _stream_of(dev, stream), Q.data_ptr(),
+          _strides4(Q, "Q"), K.data_ptr(), _strides4(K, "K"), V.data_ptr(), _strides4(V, "V"),
+          out.data_ptr(), _strides4(out, "out"), _DT[out.dtype], lse.data_ptr(),
+          row_max.data_ptr(), B, H, Hkv, Sq, Sk, D, 1.0 / math.sqrt(D) if scale is None else scale,
+          window, sinks)
+    return out, lse, row_max
 
 
-def _need_pool(k_pages, v_pages, block_table, B):
-    _need(k_pages, "k_pages", torch.bfloat16, 4)
-    _need(v_pages, "v_pages", torch.bfloat16, 4)
-    if v_pages.shape != k_pages.shape:
+def _pool(k_pages, v_pages, dev):
+    """Checks a pool; returns (n_pages, Hkv, page_size, D)."""
+    _tensor(k_pages, "k_pages", _BF16, 4, dev)
+    _tensor(v_pages, "v_pages", _BF16, 4, dev)
+    shape = k_pages.shape
+    if v_pages.shape != shape:
         raise ValueError("k_pages and v_pages differ in shape")
-    _need_table(block_table, "block_table", B)
-
-
-def _need_table(table, name, B):
-    _need(table, name, torch.int32, 2, contiguous=False)
-    if table.shape[0] != B or (table.shape[1] > 1 and table.stride(1) != 1):
-        raise ValueError(f"{name} must be [{B}][pages] with contiguous rows")
-
-
-def _table_ld(table):
-    return table.stride(0) if table.shape[0] > 1 else table.shape[1]
-
-
-def _need_lens(t, name, B):
-    _need(t, name, torch.int32, 1)
-    if t.numel() != B:
-        raise ValueError(f"{name} must have {B} values")
+    return shape
 
 
 def paged_decode_workspace_size(B, H, Hkv, max_len, weights=False, D=64):
@@ -699,57 +724,48 @@ def paged_decode_attn(q, k_pages, v_pages, block_table, lens, k_new=None, v_new=
     attention weight, summed over its group's query heads.  workspace: from
     paged_decode_workspace, kept by the caller from call to call; without one
     each call makes its own.  Returns (out [B][H][64], lse [B][H] or None)."""
-    _need(q, "q", torch.bfloat16, 3)
-    B, H, D = q.shape
-    _need_pool(k_pages, v_pages, block_table, B)
-    dev = _same_device(q, "q", k_pages=k_pages, v_pages=v_pages, block_table=block_table,
-                       lens=lens, k_new=k_new, v_new=v_new, out=out, lse=lse, weights=weights,
-                       workspace=workspace)
-    n_pages, Hkv, page_size, Dk = k_pages.shape
-    max_pages = block_table.shape[1]
+    dev = _device_of(q, "q")
+    _tensor(q, "q", _BF16, 3, dev)
+    B, H, D = q_shape = q.shape
+    n_pages, Hkv, page_size, Dk = _pool(k_pages, v_pages, dev)
+    max_pages, table_ld = _matrix(block_table, "block_table", _INT32, B, dev)
     if Dk != D:
         raise ValueError(f"q has head_dim {D}, the pages {Dk}")
-    _need_lens(lens, "lens", B)
+    _vector(lens, "lens", _INT32, B, dev)
     if (k_new is None) != (v_new is None):
         raise ValueError("k_new and v_new go together")
     if k_new is not None:
-        for n, t in (("k_new", k_new), ("v_new", v_new)):
-            _need(t, n, torch.bfloat16, 3)
-            if t.shape != (B, Hkv, D):
-                raise ValueError(f"{n} must be {(B, Hkv, D)}, got {tuple(t.shape)}")
-    if scale is None:
-        scale = 1.0 / math.sqrt(D)
+        _tensor(k_new, "k_new", _BF16, 3, dev)
+        _tensor(v_new, "v_new", _BF16, 3, dev)
+        if k_new.shape != (B, Hkv, D) or v_new.shape != (B, Hkv, D):
+            raise ValueError(f"k_new and v_new must be {(B, Hkv, D)}")
     if out is None:
-        out = torch.empty((B, H, D), dtype=out_dtype, device=dev)
-    _need(out, "out")
-    if out.shape != q.shape or out.dtype not in _DT:
-        raise ValueError(f"out must be float32 or bfloat16 {tuple(q.shape)}")
+        out = torch.empty(q_shape, dtype=out_dtype, device=q.device)
+    _tensor(out, "out", None, 3, dev)
+    if out.shape != q_shape:
+        raise ValueError(f"out must be {tuple(q_shape)}, got {tuple(out.shape)}")
     if lse is None and want_lse:
-        lse = torch.empty((B, H), dtype=torch.float32, device=dev)
+        lse = torch.empty((B, H), dtype=_F32, device=q.device)
     if lse is not None:
-        _need(lse, "lse", torch.float32)
-        if lse.numel() != B * H:
-            raise ValueError(f"lse must have {B * H} values")
+        _vector(lse, "lse", _F32, B * H, dev)
     weights_ld = 0
     if weights is not None:
-        _need(weights, "weights", torch.float32, 3)
+        _tensor(weights, "weights", _F32, 3, dev)
         if weights.shape[:2] != (B, Hkv):
             raise ValueError(f"weights must be [{B}][{Hkv}][keys], got {tuple(weights.shape)}")
         weights_ld = weights.shape[2]
-    if workspace is not None:
-        _need(workspace, "workspace")
-    with _on(dev, stream) as st:
-        if workspace is None:
-            # made on the call's stream, so that its memory is reused only after the call
-            with torch.cuda.stream(stream if stream is not None else torch.cuda.current_stream(dev)):
-                workspace = paged_decode_workspace(B, H, Hkv, max_pages * page_size,
-                                                   weights is not None, device=dev)
-        check(_lib.load().nd_paged_decode_attn(
-            st, _addr(q), _addr(k_new), _addr(v_new), _addr(k_pages), _addr(v_pages), n_pages,
-            page_size, _addr(block_table), _table_ld(block_table), max_pages, _addr(lens),
-            _addr(out), _DT[out.dtype], _addr(lse), _addr(weights), weights_ld, B, H, Hkv, D,
-            int(window), int(sinks), float(scale), _addr(workspace),
-            workspace.numel() * workspace.element_size()))
+    if workspace is None:
+        # made on the call's stream, so that its memory is reused only after the call
+        with torch.cuda.stream(stream if stream is not None else torch.cuda.current_stream(dev)):
+            workspace = paged_decode_workspace(B, H, Hkv, max_pages * page_size,
+                                               weights is not None, device=q.device)
+    else:
+        _tensor(workspace, "workspace", workspace.dtype, None, dev)
+    _call(_lib.load().nd_paged_decode_attn, dev, _stream_of(dev, stream), q.data_ptr(),
+          _addr(k_new), _addr(v_new), k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page_size,
+          block_table.data_ptr(), table_ld, max_pages, lens.data_ptr(), out.data_ptr(),
+          _DT[out.dtype], _addr(lse), _addr(weights), weights_ld, B, H, Hkv, D, window, sinks,
+          1.0 / math.sqrt(D) if scale is None else scale, workspace.data_ptr(), workspace.nbytes)
     return out, lse
 
 
@@ -759,28 +775,21 @@ def paged_kv_store(src, k_col, v_col, k_pages, v_pages, block_table, B, S, pos0=
     (nd_paged_kv_store): token (b, s) goes to position pos0 + s of sequence b.
     pos0: an int, or int32 [B] on the device; lens: int32 [B] tokens of each
     sequence, the rest being padding (None: all S)."""
-    _need(src, "src", torch.bfloat16, 2, contiguous=False)
-    if src.shape[1] > 1 and src.stride(1) != 1:
-        raise ValueError("src rows must be contiguous")
-    if src.shape[0] != B * S:
-        raise ValueError(f"src must have B*S = {B * S} rows, got {src.shape[0]}")
-    _need_pool(k_pages, v_pages, block_table, B)
-    pos_dev = pos0 if isinstance(pos0, torch.Tensor) else None
-    dev = _same_device(src, "src", k_pages=k_pages, v_pages=v_pages, block_table=block_table,
-                       pos0=pos_dev, lens=lens)
-    if pos_dev is not None:
-        _need_lens(pos_dev, "pos0", B)
+    dev = _device_of(src, "src")
+    cols, ld = _matrix(src, "src", _BF16, B * S, dev)
+    n_pages, Hkv, page_size, D = _pool(k_pages, v_pages, dev)
+    max_pages, table_ld = _matrix(block_table, "block_table", _INT32, B, dev)
+    pos_dev = None
+    if isinstance(pos0, torch.Tensor):
+        _vector(pos0, "pos0", _INT32, B, dev)
+        pos_dev, pos0 = pos0.data_ptr(), 0
     if lens is not None:
-        _need_lens(lens, "lens", B)
-    n_pages, Hkv, page_size, D = k_pages.shape
-    if max(k_col, v_col) + Hkv * D > src.shape[1]:
+        _vector(lens, "lens", _INT32, B, dev)
+    if max(k_col, v_col) + Hkv * D > cols:
         raise ValueError("k_col / v_col: the heads' columns do not fit src")
-    with _on(dev, stream) as st:
-        check(_lib.load().nd_paged_kv_store(
-            st, _addr(src), src.stride(0) if src.shape[0] > 1 else src.shape[1], int(k_col),
-            int(v_col), _addr(k_pages), _addr(v_pages), n_pages, page_size, _addr(block_table),
-            _table_ld(block_table), block_table.shape[1], int(B), int(S), Hkv,
-            0 if pos_dev is not None else int(pos0), _addr(pos_dev), _addr(lens), D))
+    _call(_lib.load().nd_paged_kv_store, dev, _stream_of(dev, stream), src.data_ptr(), ld, k_col,
+          v_col, k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page_size,
+          block_table.data_ptr(), table_ld, max_pages, B, S, Hkv, pos0, pos_dev, _addr(lens), D)
 
 
 def paged_kv_evict(k_pages, v_pages, block_table, lens, weights, out_table, budget, sinks=0,
@@ -794,37 +803,29 @@ def paged_kv_evict(k_pages, v_pages, block_table, lens, weights, out_table, budg
     Returns (kept [B][Hkv][budget] int32 positions, -1 past the last;
     new_lens [B]; weights_out [B][Hkv][keys], the kept keys' weights first,
     zeros behind them)."""
-    _need(lens, "lens", torch.int32, 1)
+    dev = _device_of(k_pages, "k_pages")
+    n_pages, Hkv, page_size, D = _pool(k_pages, v_pages, dev)
+    _tensor(lens, "lens", _INT32, 1, dev)
     B = lens.numel()
-    _need_pool(k_pages, v_pages, block_table, B)
-    _need_table(out_table, "out_table", B)
-    dev = _same_device(k_pages, "k_pages", v_pages=v_pages, block_table=block_table, lens=lens,
-                       weights=weights, out_table=out_table, weights_out=weights_out, kept=kept,
-                       new_lens=new_lens)
-    n_pages, Hkv, page_size, D = k_pages.shape
-    _need(weights, "weights", torch.float32, 3)
-    if weights.shape[:2] != (B, Hkv):
-        raise ValueError(f"weights must be [{B}][{Hkv}][keys], got {tuple(weights.shape)}")
+    max_pages, table_ld = _matrix(block_table, "block_table", _INT32, B, dev)
+    out_pages, out_ld = _matrix(out_table, "out_table", _INT32, B, dev)
+    _tensor(weights, "weights", _F32, 3, dev)
     if weights_out is None:
         weights_out = torch.empty_like(weights)
-    _need(weights_out, "weights_out", torch.float32, 3)
-    if weights_out.shape[:2] != (B, Hkv):
-        raise ValueError(f"weights_out must be [{B}][{Hkv}][keys]")
+    _tensor(weights_out, "weights_out", _F32, 3, dev)
+    if weights.shape[:2] != (B, Hkv) or weights_out.shape[:2] != (B, Hkv):
+        raise ValueError(f"weights and weights_out must be [{B}][{Hkv}][keys]")
     if kept is None:
-        kept = torch.empty((B, Hkv, max(0, int(budget))), dtype=torch.int32, device=dev)
-    _need(kept, "kept", torch.int32)
-    if kept.numel() != B * Hkv * budget:
-        raise ValueError(f"kept must have B*Hkv*budget = {B * Hkv * budget} values")
+        kept = torch.empty((B, Hkv, max(0, int(budget))), dtype=_INT32, device=lens.device)
+    _vector(kept, "kept", _INT32, B * Hkv * max(0, budget), dev)
     if new_lens is None:
-        new_lens = torch.empty((B,), dtype=torch.int32, device=dev)
-    _need_lens(new_lens, "new_lens", B)
-    with _on(dev, stream) as st:
-        check(_lib.load().nd_paged_kv_evict(
-            st, _addr(k_pages), _addr(v_pages), n_pages, page_size, _addr(block_table),
-            _table_ld(block_table), block_table.shape[1], _addr(lens), _addr(weights),
-            weights.shape[2], _addr(out_table), _table_ld(out_table), out_table.shape[1],
-            _addr(weights_out), weights_out.shape[2], _addr(kept), _addr(new_lens), B, Hkv, D,
-            int(budget), int(sinks), int(recent)))
+        new_lens = torch.empty((B,), dtype=_INT32, device=lens.device)
+    _vector(new_lens, "new_lens", _INT32, B, dev)
+    _call(_lib.load().nd_paged_kv_evict, dev, _stream_of(dev, stream), k_pages.data_ptr(),
+          v_pages.data_ptr(), n_pages, page_size, block_table.data_ptr(), table_ld, max_pages,
+          lens.data_ptr(), weights.data_ptr(), weights.shape[2], out_table.data_ptr(), out_ld,
+          out_pages, weights_out.data_ptr(), weights_out.shape[2], kept.data_ptr(),
+          new_lens.data_ptr(), B, Hkv, D, budget, sinks, recent)
     return kept, new_lens, weights_out
 
 
@@ -840,66 +841,52 @@ def logits_penalty(logits, history=None, history_lens=None, repetition=None, pre
     [>= V/32] for all rows, bit v % 32 of word v / 32 allowing token v.  `out`
     may be `logits` itself.  Returns (out, idx int32 [rows], or None with
     greedy=False)."""
-    _need(logits, "logits", None, 2, contiguous=False)
-    if logits.dtype not in _DT:
-        raise TypeError(f"logits dtype {logits.dtype} not supported")
-    rows, V = logits.shape
-    dev = _same_device(logits, "logits", history=history, history_lens=history_lens,
-                       repetition=repetition, presence=presence, frequency=frequency,
-                       bias_ids=bias_ids, bias=bias, mask=mask, out=out, idx=idx)
+    dev = _device_of(logits, "logits")
+    rows = logits.shape[0]
+    V, ld = _matrix(logits, "logits", None, rows, dev)
     if out is None:
-        out = torch.empty((rows, V), dtype=out_dtype or logits.dtype, device=dev)
-    if out.dtype not in _DT or out.shape != logits.shape:
-        raise ValueError(f"out must be float32 or bfloat16 {(rows, V)}")
-    for n, t in (("logits", logits), ("out", out)):
-        if V > 1 and t.stride(1) != 1:
-            raise ValueError(f"{n} rows must be contiguous")
-        if rows > 1 and t.stride(0) < V:
-            raise ValueError(f"{n} rows overlap")
-    ld = lambda t: t.stride(0) if rows > 1 else max(V, 1)
+        out = torch.empty((rows, V), dtype=out_dtype or logits.dtype, device=logits.device)
+    out_V, out_ld = _matrix(out, "out", None, rows, dev)
+    if out_V != V:
+        raise ValueError(f"out must be {(rows, V)}, got {tuple(out.shape)}")
     n_hist = hist_ld = 0
     if history is not None:
-        _need(history, "history", torch.int32, 2, contiguous=False)
-        n_hist = history.shape[1]
-        if history.shape[0] != rows or (n_hist > 1 and history.stride(1) != 1):
-            raise ValueError(f"history must be [{rows}][tokens] with contiguous rows")
-        hist_ld = history.stride(0) if rows > 1 else n_hist
+        n_hist, hist_ld = _matrix(history, "history", _INT32, rows, dev)
     if history_lens is not None:
-        _need_lens(history_lens, "history_lens", rows)
-    for n, t in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
-        if t is not None:
-            _need(t, n, torch.float32, 1)
-            if t.numel() != rows:
-                raise ValueError(f"{n} must have {rows} values")
+        _vector(history_lens, "history_lens", _INT32, rows, dev)
+    if repetition is not None:
+        _vector(repetition, "repetition", _F32, rows, dev)
+    if presence is not None:
+        _vector(presence, "presence", _F32, rows, dev)
+    if frequency is not None:
+        _vector(frequency, "frequency", _F32, rows, dev)
     n_bias = 0
     if (bias_ids is None) != (bias is None):
         raise ValueError("bias_ids and bias go together")
-    if bias_ids is not None:
-        _need(bias_ids, "bias_ids", torch.int32, 2)
-        _need(bias, "bias", torch.float32, 2)
+    if bias is not None:
+        _tensor(bias_ids, "bias_ids", _INT32, 2, dev)
+        _tensor(bias, "bias", _F32, 2, dev)
         if bias_ids.shape != bias.shape or bias.shape[0] != rows:
             raise ValueError(f"bias_ids and bias must be [{rows}][n]")
         n_bias = bias.shape[1]
     mask_ld = 0
     if mask is not None:
-        if mask.dtype not in (torch.int32, torch.uint32):
-            raise TypeError(f"mask must be int32 or uint32 words, got {mask.dtype}")
-        if mask.dim() not in (1, 2) or (mask.shape[-1] > 1 and mask.stride(-1) != 1):
-            raise ValueError("mask must be [words] or [rows][words] with contiguous rows")
-        if mask.shape[-1] < (V + 31) // 32 or (mask.dim() == 2 and mask.shape[0] != rows):
-            raise ValueError(f"mask must have {rows} rows (or one) of at least {(V + 31) // 32} words")
+        _tensor(mask, "mask", torch.uint32 if mask.dtype is torch.uint32 else _INT32, None, dev, False)
+        words = mask.shape[-1] if mask.dim() in (1, 2) else 0
+        if words < (V + 31) // 32 or (words > 1 and mask.stride(-1) != 1) or (
+                mask.dim() == 2 and mask.shape[0] != rows):
+            raise ValueError(f"mask must be [{rows}][words] or [words] of at least "
+                             f"{(V + 31) // 32} contiguous words")
         if mask.dim() == 2:
-            mask_ld = mask.stride(0) if rows > 1 else mask.shape[1]
+            mask_ld = mask.stride(0) if rows > 1 else words
     if idx is None and greedy:
-        idx = torch.empty((rows,), dtype=torch.int32, device=dev)
+        idx = torch.empty((rows,), dtype=_INT32, device=logits.device)
     if idx is not None:
-        _need_lens(idx, "idx", rows)
-    with _on(dev, stream) as st:
-        check(_lib.load().nd_logits_penalty(
-            st, _addr(logits), _DT[logits.dtype], ld(logits), rows, V, _addr(history), hist_ld,
-            n_hist, _addr(history_lens), _addr(repetition), _addr(presence), _addr(frequency),
-            _addr(bias_ids), _addr(bias), n_bias, _addr(mask), mask_ld, _addr(out),
-            _DT[out.dtype], ld(out), _addr(idx)))
+        _vector(idx, "idx", _INT32, rows, dev)
+    _call(_lib.load().nd_logits_penalty, dev, _stream_of(dev, stream), logits.data_ptr(),
+          _DT[logits.dtype], ld, rows, V, _addr(history), hist_ld, n_hist, _addr(history_lens),
+          _addr(repetition), _addr(presence), _addr(frequency), _addr(bias_ids), _addr(bias),
+          n_bias, _addr(mask), mask_ld, out.data_ptr(), _DT[out.dtype], out_ld, _addr(idx))
     return out, idx
 
 
