@@ -15,6 +15,7 @@
 #include <cuda_bf16.h>
 #include <stdint.h>
 
+#include "argmax.cuh"
 #include "launch.cuh"
 #include "model_ops.h"
 #include "ptx.cuh"
@@ -91,15 +92,6 @@ __device__ __forceinline__ float ld_f<float>(const float* p) { return *p; }
 template <>
 __device__ __forceinline__ float ld_f<__nv_bfloat16>(const __nv_bfloat16* p) {
   return __bfloat162float(*p);
-}
-
-// (v2, i2) replaces (v, i) if larger, equal with a smaller index, or a
-// number where v is NaN.
-__device__ __forceinline__ void better(float& v, int& i, float v2, int i2) {
-  if (v2 > v || (v2 == v && i2 < i) || (v != v && v2 == v2)) {
-    v = v2;
-    i = i2;
-  }
 }
 
 constexpr int kArgmaxThreads = 512;
