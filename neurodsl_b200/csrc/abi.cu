@@ -1275,8 +1275,8 @@ __attribute__((visibility("default"))) int nd_paged_kv_store(
       k_col + static_cast<long long>(Hkv) * 64 > ld || v_col + static_cast<long long>(Hkv) * 64 > ld)
     return fail(ND_ERR_SHAPE, "%s: columns k=%d v=%d (+%d) must be multiples of 8 inside ld=%lld", fn,
                 k_col, v_col, Hkv * 64, static_cast<long long>(ld));
-  if (static_cast<long long>(B) * S * Hkv > (1LL << 36))
-    return fail(ND_ERR_SHAPE, "%s: too many rows", fn);
+  if (static_cast<long long>(B) * S > 0x7fffffffLL)
+    return fail(ND_ERR_SHAPE, "%s: B*S exceeds 2^31 - 1", fn);
   if (empty) return ok();
   if (!src) return fail(ND_ERR_INVALID_ARG, "%s: null pointer", fn);
   if (!aligned16(src)) return fail(ND_ERR_ALIGNMENT, "%s: src must be 16-byte aligned", fn);
@@ -1312,6 +1312,8 @@ __attribute__((visibility("default"))) int nd_paged_kv_evict(
     return fail(ND_ERR_SHAPE, "%s: max_out_pages * page_size must be below 2^30", fn);
   if (weights_ld < static_cast<long long>(max_pages) * page_size || weights_out_ld < budget)
     return fail(ND_ERR_SHAPE, "%s: weights rows are too short", fn);
+  if (static_cast<long long>(B) * Hkv * budget > (1LL << 36))
+    return fail(ND_ERR_SHAPE, "%s: B*Hkv*budget exceeds 2^36", fn);
   if (empty) return ok();
   if (!lens || !weights || !out_table || !weights_out || !kept || !new_lens)
     return fail(ND_ERR_INVALID_ARG, "%s: null pointer", fn);

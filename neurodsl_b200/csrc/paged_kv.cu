@@ -34,7 +34,12 @@ __device__ __forceinline__ long long pool_row(const PagedPool& pool, const int* 
 }
 
 // ------------------------------------------------------------------- store
-// Thread = 16 bytes of one (token, head) row of K and of V.
+// A warp takes 32 pieces of 16 bytes (four heads) of kTokens consecutive tokens
+// of one sequence, whose rows of a head are neighbours in a page: a lane looks
+// a token's row up, then all K and V loads go out before the first store.  Four
+// tokens a warp keep enough bytes in flight for a long prompt (65536 tokens, half of
+// them padding, 12 heads: 35.9 us; with a thread for each 16 bytes 43.4); with few tokens, one a warp spreads them over more SMs.
+template <int kTokens>
 __global__ void __launch_bounds__(256)
     paged_store_kernel(const __nv_bfloat16* __restrict__ src, long long ld, int k_col, int v_col,
                        const PagedPool pool, int B, int S, int pos0,
@@ -42,81 +47,86 @@ __global__ void __launch_bounds__(256)
                        int* __restrict__ err_word) {
   pdl_wait();
   pdl_trigger();
-  const long long n = static_cast<long long>(B) * S * pool.Hkv * kVec;
-  const long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (i >= n) return;
-  const int c = static_cast<int>(i % kVec);
-  const long long r = i / kVec;
-  const int h = static_cast<int>(r % pool.Hkv);
-  const long long bs = r / pool.Hkv;
-  const int s = static_cast<int>(bs % S);
-  const int b = static_cast<int>(bs / S);
+  const int lane = threadIdx.x & 31;
+  const long long w = static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const int per_seq = (S + kTokens - 1) / kTokens, chunks = (pool.Hkv * kVec + 31) / 32;
+  const long long group = w / chunks;
+  const int p = static_cast<int>(w - group * chunks) * 32 + lane;   // this lane's piece of a token
+  const int b = static_cast<int>(group / per_seq);
+  if (b >= B) return;
+  const int s0 = static_cast<int>(group - static_cast<long long>(b) * per_seq) * kTokens;
+  int len = S;
   if (lens != nullptr) {
-    const int len = lens[b];
-    if (len < 0 || len > S) raise(err_word);
-    if (s >= len) return;   // padding
+    len = lens[b];
+    if (len < 0 || len > S) {
+      if (s0 == 0 && p == 0) raise(err_word);
+      len = len < 0 ? 0 : S;
+    }
   }
-  const long long pos = static_cast<long long>(pos0_dev ? pos0_dev[b] : pos0) + s;
-  const long long row = pool_row(pool, pool.table, pool.table_ld, pool.max_pages, b, h, pos);
-  if (row < 0) {
-    raise(err_word);
-    return;
+  if (s0 >= len) return;   // padding
+  long long row = -1;      // of lane's token, head 0
+  if (lane < kTokens && s0 + lane < len) {
+    const long long pos = static_cast<long long>(pos0_dev ? pos0_dev[b] : pos0) + s0 + lane;
+    row = pool_row(pool, pool.table, pool.table_ld, pool.max_pages, b, 0, pos);
+    if (row < 0) raise(err_word);
   }
-  const __nv_bfloat16* x = src + bs * ld + h * 64 + c * 8;
-  const uint4 kk = *reinterpret_cast<const uint4*>(x + k_col);
-  const uint4 vv = *reinterpret_cast<const uint4*>(x + v_col);
-  *reinterpret_cast<uint4*>(pool.k + row * 64 + c * 8) = kk;
-  *reinterpret_cast<uint4*>(pool.v + row * 64 + c * 8) = vv;
+  long long rows[kTokens];
+#pragma unroll
+  for (int i = 0; i < kTokens; ++i) rows[i] = __shfl_sync(0xffffffffu, row, i);
+  const __nv_bfloat16* x = src + (static_cast<long long>(b) * S + s0) * ld;
+  const long long head = static_cast<long long>(pool.page_size) * 64;   // from head to head
+  if (p >= pool.Hkv * kVec) return;
+  uint4 kk[kTokens], vv[kTokens];
+#pragma unroll
+  for (int i = 0; i < kTokens; ++i)
+    if (rows[i] >= 0) {
+      kk[i] = *reinterpret_cast<const uint4*>(x + i * ld + k_col + p * 8);
+      vv[i] = *reinterpret_cast<const uint4*>(x + i * ld + v_col + p * 8);
+    }
+  const long long off = (p / kVec) * head + (p % kVec) * 8;
+#pragma unroll
+  for (int i = 0; i < kTokens; ++i)
+    if (rows[i] >= 0) {
+      *reinterpret_cast<uint4*>(pool.k + rows[i] * 64 + off) = kk[i];
+      *reinterpret_cast<uint4*>(pool.v + rows[i] * 64 + off) = vv[i];
+    }
 }
 
 // ---------------------------------------------------------------- eviction
-// Weights in an order of unsigned integers: NaN lowest, then -inf to +inf,
-// the two zeros equal.
+// Weights in an order of unsigned integers: 1 for NaN, the lowest, then -inf to
+// +inf, the two zeros equal; 0 is left for "no weight".
 __device__ __forceinline__ uint32_t ordered(float w) {
-  if (w != w) return 0u;
+  if (w != w) return 1u;
   const uint32_t u = w == 0.f ? 0u : __float_as_uint(w);
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-constexpr int kSelThreads = 1024;
-
-// Exclusive sum over the block of two counts packed as 32 + 32 bits; `total`
-// receives the block's sums.
-__device__ __forceinline__ unsigned long long block_scan(unsigned long long v,
-                                                         unsigned long long* sm,
-                                                         unsigned long long& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  unsigned long long x = v;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const unsigned long long y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
-  }
-  __syncthreads();   // the last call's readers are done
-  if (lane == 31) sm[warp] = x;
-  __syncthreads();
-  unsigned long long base = 0, all = 0;
-  for (int w = 0; w < kSelThreads / 32; ++w) {
-    if (w < warp) base += sm[w];
-    all += sm[w];
-  }
-  total = all;
-  return base + x - v;
-}
-
 // One block per (sequence, kv head): which positions stay.  The first `sinks`
 // and the last `recent` always do; the rest of the budget goes to the largest
-// weights between, found by their value's digits (four passes of 8 bits), the
-// lowest positions first among equals.  Writes the kept positions in order,
-// their weights, and the new length.
-__global__ void __launch_bounds__(kSelThreads)
+// weights between, the lowest positions first among equals.  The weights stay in
+// registers (kR a thread; with kR = 0, for longer caches, they are read again
+// each time, from L2): every warp owns a contiguous span of positions, lane by
+// lane, so that ballots and one sum over the warps give each kept position its
+// slot.  The smallest weight that stays is found by its digits of 11, 11 and 10
+// bits, from the top of an order-preserving integer, with a histogram in shared
+// memory each; from the second digit on only the few weights that share the
+// digits so far take part.  (Two bits at a time by counting, without
+// atomics, is 16 passes over all weights: 36 us for 256 heads of up to 8192
+// keys, against 16.5.)
+template <int kThreads, int kR>
+__global__ void __launch_bounds__(kThreads, kThreads < 1024 ? 2 : 1)
     paged_select_kernel(const PagedEvict a, int* __restrict__ err_word) {
-  __shared__ unsigned int hist[256];
-  __shared__ unsigned long long scan_sm[kSelThreads / 32];
-  __shared__ uint32_t s_prefix;
-  __shared__ int s_need;
+  constexpr int kW = kThreads / 32;
+  constexpr int kBins = 2048, kPer = kBins / kThreads;   // bins a thread
+  constexpr int kAll = 1 << 30;
+  __shared__ uint32_t hist[kBins];
+  __shared__ uint32_t warp_sum[kW];
+  __shared__ uint32_t found_digit;
+  __shared__ int found_above;
+  __shared__ int sure_sm[kW], tie_sm[kW];
   pdl_wait();
   pdl_trigger();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int b = blockIdx.x / a.pool.Hkv, h = blockIdx.x % a.pool.Hkv;
   const long long cap = static_cast<long long>(a.pool.max_pages) * a.pool.page_size;
   int L = a.lens[b];
@@ -132,96 +142,195 @@ __global__ void __launch_bounds__(kSelThreads)
   const int lo = a.sinks, hi = L - a.recent;         // the positions that compete
   const int need = a.budget - a.sinks - a.recent;    // how many of them stay
 
-  uint32_t threshold = 0;
-  int ties = 0;            // of those equal to the threshold
-  if (!all && need > 0) {
-    uint32_t prefix = 0, mask = 0;
-    int left = need;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = threadIdx.x; i < 256; i += kSelThreads) hist[i] = 0;
-      __syncthreads();
-      for (int i = lo + threadIdx.x; i < hi; i += kSelThreads) {
-        const uint32_t u = ordered(w[i]);
-        if ((u & mask) == prefix) atomicAdd(&hist[(u >> shift) & 255u], 1u);
-      }
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        int rest = left, d = 255;
-        while (static_cast<int>(hist[d]) < rest) rest -= static_cast<int>(hist[d--]);
-        s_prefix = prefix | (static_cast<uint32_t>(d) << shift);
-        s_need = rest;
-      }
-      __syncthreads();
-      prefix = s_prefix;
-      left = s_need;
-      mask |= 255u << shift;
-      __syncthreads();
-    }
-    threshold = prefix;
-    ties = left;
+  // rows of 32 positions a warp takes, and its first position
+  const int rows = kR > 0 ? kR : (L + kThreads - 1) / kThreads;
+  const int p0 = warp * rows * 32 + lane;
+  // a position's ordered weight, 0 where it does not compete
+  auto read = [&](int r) -> uint32_t {
+    const int p = p0 + 32 * r;
+    return p >= lo && p < hi ? ordered(w[p]) : 0u;
+  };
+  constexpr bool kKeep = kR > 0 && kR <= 16;   // the weights themselves in registers too
+  uint32_t x[kR > 0 ? kR : 1];
+  float v[kR > 0 ? kR : 1];
+  if constexpr (kR > 0) {
+#pragma unroll
+    for (int r = 0; r < kR; ++r) v[r] = p0 + 32 * r < L ? w[p0 + 32 * r] : 0.f;
+#pragma unroll
+    for (int r = 0; r < kR; ++r) x[r] = p0 + 32 * r >= lo && p0 + 32 * r < hi ? ordered(v[r]) : 0u;
   }
+  auto weight = [&](int r) -> uint32_t {
+    if constexpr (kR > 0) return x[r];
+    else return read(r);
+  };
 
-  int slot0 = 0, tie0 = 0;
-  for (int base = 0; base < L; base += kSelThreads) {
-    const int i = base + threadIdx.x;
-    bool sure = false, tie = false;
-    float x = 0.f;
-    if (i < L) {
-      x = w[i];
-      if (all || i < lo || i >= hi) {
-        sure = true;
-      } else if (need > 0) {
-        const uint32_t u = ordered(x);
-        sure = u > threshold;
-        tie = u == threshold;
+  // threshold: the largest value with at least `need` weights at or above it
+  uint32_t threshold = 0;
+  int above = 0;           // weights above the threshold
+  if (!all && need > 0) {
+#pragma unroll
+    for (int digit = 0; digit < 3; ++digit) {
+      const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0;
+      const uint32_t bins = digit == 2 ? 1023u : 2047u;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) hist[i * kThreads + threadIdx.x] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int r = 0; r < (kR > 0 ? kR : kAll); ++r) {
+        if (kR == 0 && r >= rows) break;
+        const uint32_t u = weight(r);
+        const uint32_t known = digit == 0 ? 0u : (u ^ threshold) >> (digit == 1 ? 21 : 10);
+        if (u != 0 && known == 0) atomicAdd(&hist[u >> shift & bins], 1u);
       }
+      __syncthreads();
+      // bins from the highest down: thread i takes the kPer below its neighbour's
+      const int first = kBins - 1 - static_cast<int>(threadIdx.x) * kPer;
+      uint32_t mine = 0;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) mine += hist[first - i];
+      uint32_t upto = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
+      }
+      if (lane == 31) warp_sum[warp] = upto;
+      __syncthreads();
+      upto += __reduce_add_sync(0xffffffffu, lane < warp && lane < kW ? warp_sum[lane] : 0u);
+      const uint32_t left = static_cast<uint32_t>(need - above);
+      if (upto >= left && upto - mine < left) {      // one thread's bins reach it
+        uint32_t c = upto - mine;
+        int i = 0;
+        while (c + hist[first - i] < left) c += hist[first - i++];
+        found_digit = static_cast<uint32_t>(first - i);
+        found_above = above + static_cast<int>(c);
+      }
+      __syncthreads();
+      threshold |= found_digit << shift;
+      above = found_above;
     }
-    unsigned long long sums;
-    const unsigned long long at =
-        block_scan((static_cast<unsigned long long>(tie) << 32) | sure, scan_sm, sums);
-    const int tie_at = tie0 + static_cast<int>(at >> 32);
-    const int ties_before = min(tie_at, ties) - min(tie0, ties);
-    if (sure || (tie && tie_at < ties)) {
-      const int slot = slot0 + static_cast<int>(at & 0xffffffffu) + ties_before;
-      kept[slot] = i;
-      w_out[slot] = x;
-    }
-    const int tie1 = tie0 + static_cast<int>(sums >> 32);
-    slot0 += static_cast<int>(sums & 0xffffffffu) + min(tie1, ties) - min(tie0, ties);
-    tie0 = tie1;
   }
-  for (int i = n + threadIdx.x; i < a.budget; i += kSelThreads) kept[i] = -1;
-  for (long long i = n + threadIdx.x; i < a.weights_out_ld; i += kSelThreads) w_out[i] = 0.f;
+  const int ties = need - above;   // of the weights equal to the threshold
+
+  // how many each warp keeps for certain, and how many equal the threshold
+  // (with the weights in registers, a bit a position)
+  auto is_sure = [&](int r) {
+    const int p = p0 + 32 * r;
+    return p < L && (all || p < lo || p >= hi || (need > 0 && weight(r) > threshold));
+  };
+  auto is_tie = [&](int r) { return !all && need > 0 && weight(r) == threshold; };   // threshold > 0
+  uint32_t sure_bits = 0, tie_bits = 0;
+  if constexpr (kR > 0) {
+    const uint32_t t_up = !all && need > 0 ? threshold : ~0u;   // nothing lies above, or ties, ~0
+#pragma unroll
+    for (int r = 0; r < kR; ++r) {
+      sure_bits |= static_cast<uint32_t>(x[r] > t_up) << r;
+      tie_bits |= static_cast<uint32_t>(x[r] == t_up) << r;
+    }
+    // the positions that do not compete
+#pragma unroll
+    for (int r = 0; r < kR; ++r) {
+      const int p = p0 + 32 * r;
+      sure_bits |= static_cast<uint32_t>(p < L && (all || p < lo || p >= hi)) << r;
+    }
+  }
+  int n_sure = 0, n_tie = 0;
+#pragma unroll
+  for (int r = 0; r < (kR > 0 ? kR : kAll); ++r) {
+    if (kR == 0 && r >= rows) break;
+    n_sure += __popc(__ballot_sync(0xffffffffu, kR > 0 ? sure_bits >> r & 1u : is_sure(r)));
+    n_tie += __popc(__ballot_sync(0xffffffffu, kR > 0 ? tie_bits >> r & 1u : is_tie(r)));
+  }
+  if (lane == 0) {
+    sure_sm[warp] = n_sure;
+    tie_sm[warp] = n_tie;
+  }
+  __syncthreads();
+  const bool before = lane < warp && lane < kW;
+  int slot = __reduce_add_sync(0xffffffffu, before ? static_cast<unsigned>(sure_sm[lane]) : 0u);
+  int tie_at = __reduce_add_sync(0xffffffffu, before ? static_cast<unsigned>(tie_sm[lane]) : 0u);
+  slot += min(tie_at, ties);
+  const uint32_t below = (1u << lane) - 1u;
+#pragma unroll
+  for (int r = 0; r < (kR > 0 ? kR : kAll); ++r) {
+    if (kR == 0 && r >= rows) break;
+    const bool tie = kR > 0 ? tie_bits >> r & 1u : is_tie(r);
+    const uint32_t m_tie = __ballot_sync(0xffffffffu, tie);
+    const bool keep = (kR > 0 ? sure_bits >> r & 1u : is_sure(r)) || (tie && tie_at + __popc(m_tie & below) < ties);
+    const uint32_t m = __ballot_sync(0xffffffffu, keep);
+    if (keep) {
+      const int at = slot + __popc(m & below);
+      kept[at] = p0 + 32 * r;
+      w_out[at] = kKeep ? v[kKeep ? r : 0] : w[p0 + 32 * r];
+    }
+    slot += __popc(m);
+    tie_at += __popc(m_tie);
+  }
+  for (int i = n + threadIdx.x; i < a.budget; i += kThreads) kept[i] = -1;
+  // zeros behind the kept weights, 16 bytes at a time where the rows allow
+  long long z = n;
+  if (a.weights_out_ld % 4 == 0 && (reinterpret_cast<uintptr_t>(w_out) & 15) == 0) {
+    const long long z4 = (z + 3) / 4, e4 = a.weights_out_ld / 4;
+    if (z + threadIdx.x < 4 * z4) w_out[z + threadIdx.x] = 0.f;
+#pragma unroll 4
+    for (long long i = z4 + threadIdx.x; i < e4; i += kThreads)
+      reinterpret_cast<float4*>(w_out)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  } else {
+    for (long long i = z + threadIdx.x; i < a.weights_out_ld; i += kThreads) w_out[i] = 0.f;
+  }
   if (h == 0 && threadIdx.x == 0) a.new_lens[b] = n;
 }
 
-// Thread = 16 bytes of one kept (slot, head) row of K and of V.
+// A warp moves 32 kept rows of one (sequence, kv head): a lane looks one up,
+// then eight lanes move a row, 4 rows of K and V an instruction and 16 in flight.
 __global__ void __launch_bounds__(256)
     paged_gather_kernel(const PagedEvict a, int* __restrict__ err_word) {
   pdl_wait();
   pdl_trigger();
-  const long long n = static_cast<long long>(a.B) * a.pool.Hkv * a.budget * kVec;
-  const long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (i >= n) return;
-  const int c = static_cast<int>(i % kVec);
-  const long long r = i / kVec;
-  const int slot = static_cast<int>(r % a.budget);
-  const int bh = static_cast<int>(r / a.budget);
-  const int b = bh / a.pool.Hkv, h = bh % a.pool.Hkv;
-  const int pos = a.kept[r];
-  if (pos < 0) return;
-  const long long src =
-      pool_row(a.pool, a.pool.table, a.pool.table_ld, a.pool.max_pages, b, h, pos);
-  const long long dst = pool_row(a.pool, a.out_table, a.out_table_ld, a.out_pages, b, h, slot);
-  if (src < 0 || dst < 0) raise(err_word);
-  if (dst < 0) return;
-  uint4 kk = make_uint4(0, 0, 0, 0), vv = kk;   // a row without a page reads as zeros
-  if (src >= 0) {
-    kk = *reinterpret_cast<const uint4*>(a.pool.k + src * 64 + c * 8);
-    vv = *reinterpret_cast<const uint4*>(a.pool.v + src * 64 + c * 8);
+  const int lane = threadIdx.x & 31;
+  const int per_head = (a.budget + 31) / 32;
+  const long long w = static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const long long bh = w / per_head;
+  if (bh >= static_cast<long long>(a.B) * a.pool.Hkv) return;
+  const int b = static_cast<int>(bh / a.pool.Hkv), h = static_cast<int>(bh % a.pool.Hkv);
+  const int slot = static_cast<int>(w - bh * per_head) * 32 + lane;
+  const int pos = slot < a.budget ? a.kept[bh * a.budget + slot] : -1;
+  long long src = -1, dst = -1;
+  if (pos >= 0) {
+    src = pool_row(a.pool, a.pool.table, a.pool.table_ld, a.pool.max_pages, b, h, pos);
+    dst = pool_row(a.pool, a.out_table, a.out_table_ld, a.out_pages, b, h, slot);
+    if (src < 0 || dst < 0) raise(err_word);
   }
-  *reinterpret_cast<uint4*>(a.pool.k + dst * 64 + c * 8) = kk;
-  *reinterpret_cast<uint4*>(a.pool.v + dst * 64 + c * 8) = vv;
+  if (!__any_sync(0xffffffffu, dst >= 0)) return;
+  const int c = (lane & 7) * 8;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    uint4 kk[4], vv[4];
+    long long to[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = half * 16 + i * 4 + (lane >> 3);
+      const long long from = __shfl_sync(0xffffffffu, src, r);
+      to[i] = __shfl_sync(0xffffffffu, dst, r);
+      kk[i] = vv[i] = make_uint4(0, 0, 0, 0);   // a row without a page reads as zeros
+      if (from >= 0 && to[i] >= 0) {
+        kk[i] = *reinterpret_cast<const uint4*>(a.pool.k + from * 64 + c);
+        vv[i] = *reinterpret_cast<const uint4*>(a.pool.v + from * 64 + c);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (to[i] >= 0) {
+        *reinterpret_cast<uint4*>(a.pool.k + to[i] * 64 + c) = kk[i];
+        *reinterpret_cast<uint4*>(a.pool.v + to[i] * 64 + c) = vv[i];
+      }
+  }
+}
+
+template <int kThreads, int kR>
+cudaError_t launch_select(cudaStream_t stream, const PagedEvict& a, unsigned heads, int* err_word) {
+  return launch_ex(paged_select_kernel<kThreads, kR>, dim3(heads), dim3(kThreads), 0, stream, 1, true,
+                   a, err_word);
 }
 
 }  // namespace
@@ -229,22 +338,33 @@ __global__ void __launch_bounds__(256)
 cudaError_t launch_paged_store(cudaStream_t stream, const __nv_bfloat16* src, long long ld,
                                int k_col, int v_col, const PagedPool& pool, int B, int S, int pos0,
                                const int* pos0_dev, const int* lens, int* err_word) {
-  const long long n = static_cast<long long>(B) * S * pool.Hkv * kVec;
-  if (n == 0) return cudaSuccess;
-  return launch_ex(paged_store_kernel, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0,
-                   stream, 1, true, src, ld, k_col, v_col, pool, B, S, pos0, pos0_dev, lens,
-                   err_word);
+  if (B == 0 || S == 0 || pool.Hkv == 0) return cudaSuccess;
+  const long long chunks = (static_cast<long long>(pool.Hkv) * kVec + 31) / 32;
+  const bool few = B * static_cast<long long>(S) * chunks < 32 * current_sm_count();
+  const long long warps = chunks * B * (few ? S : (S + 3) / 4);
+  return launch_ex(few ? paged_store_kernel<1> : paged_store_kernel<4>,
+                   dim3(static_cast<unsigned>((warps + 7) / 8)), dim3(256), 0, stream, 1, true, src,
+                   ld, k_col, v_col, pool, B, S, pos0, pos0_dev, lens, err_word);
 }
 
 cudaError_t launch_paged_evict(cudaStream_t stream, const PagedEvict& a, int* err_word) {
   const unsigned heads = static_cast<unsigned>(a.B * a.pool.Hkv);
   if (heads == 0) return cudaSuccess;
-  cudaError_t e = launch_ex(paged_select_kernel, dim3(heads), dim3(kSelThreads), 0, stream, 1, true,
-                            a, err_word);
+  // weights in registers as far as they go
+  const long long cap = static_cast<long long>(a.pool.max_pages) * a.pool.page_size;
+  cudaError_t e;
+  if (cap <= 1024)
+    e = launch_select<256, 4>(stream, a, heads, err_word);
+  else if (cap <= 8192)
+    e = launch_select<512, 16>(stream, a, heads, err_word);
+  else if (cap <= 32768)
+    e = launch_select<1024, 32>(stream, a, heads, err_word);
+  else
+    e = launch_select<1024, 0>(stream, a, heads, err_word);
   if (e != cudaSuccess) return e;
-  const long long n = static_cast<long long>(heads) * a.budget * kVec;
-  return launch_ex(paged_gather_kernel, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0,
-                   stream, 1, true, a, err_word);
+  const long long warps = static_cast<long long>(heads) * ((a.budget + 31) / 32);
+  return launch_dependent(paged_gather_kernel, dim3(static_cast<unsigned>((warps + 7) / 8)), dim3(256),
+                          0, stream, a, err_word);
 }
 
 }  // namespace nd
