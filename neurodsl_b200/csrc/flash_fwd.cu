@@ -47,7 +47,13 @@
 // later than the first's, so each query tile leaves out one tile of the stream
 // it shares with the other.  Only tiles cut by a border of the visible range
 // are masked, by a bit mask per 32 columns (two instructions a score; the
-// comparisons it replaces would be four).
+// comparisons it replaces would be four).  (Leaving out a half in which none of
+// a warp's rows sees a key, one exponential in ten, measured slower: 141 against
+// 137 us at B=2, H=16, S=8192, window 1024, 4 sinks; a step's time is its chain
+// from scores to weights, not the exponentials alone.)  With fewer items of 256
+// rows than SMs an item is one query tile: a step takes less time, and twice as
+// many SMs work (27.1 -> 20.2 us for 509 queries against 4099 keys, B=2, H=16,
+// window 1024).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <limits.h>
@@ -263,6 +269,8 @@ struct WorkItem {
 // a K/V head and the position of query 0.
 struct FlashWindow {
   int window, sinks, group, off;
+  int solo;       // items of one query tile (the second tile's warps are idle)
+  __host__ __device__ int item_rows() const { return solo ? kBM : kRowsPerCta; }
 };
 
 template <bool kCausal, bool kWindow>
@@ -272,15 +280,20 @@ __device__ __forceinline__ WorkItem decode_item(int k, int BH, int n_blk, int n_
   if constexpr (kWindow) {
     w.blk = n_blk - 1 - k / BH;
     w.bh = k % BH;
-    const int p0 = win.off + w.blk * kRowsPerCta;        // position of the first row
+    const int p0 = win.off + w.blk * win.item_rows();    // position of the first row
     const int lo0 = max(0, p0 - win.window + 1) / kBN;
     const int hi0 = min((p0 + kBM - 1) / kBN, n_k - 1);
-    const int hi1 = min((p0 + 2 * kBM - 1) / kBN, n_k - 1);
-    // rows past Sq may have their whole window past Sk
-    const int lo1 = min(max(0, p0 + kBM - win.window + 1) / kBN, hi1);
     const int sink_tiles = ceil_div(win.sinks, kBN);
     w.lo = lo0;
     w.n_sink = min(sink_tiles, lo0);
+    if (win.solo) {
+      w.skip = 0;
+      w.n_total = w.n_kv[0] = w.n_kv[1] = w.n_sink + hi0 - lo0 + 1;
+      return w;
+    }
+    const int hi1 = min((p0 + 2 * kBM - 1) / kBN, n_k - 1);
+    // rows past Sq may have their whole window past Sk
+    const int lo1 = min(max(0, p0 + kBM - win.window + 1) / kBN, hi1);
     w.skip = sink_tiles > lo0 ? 0 : lo1 - lo0;
     w.n_total = w.n_sink + hi1 - lo0 + 1;
     w.n_kv[0] = w.n_total - (hi1 - hi0);
@@ -360,7 +373,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const int n_blk = ceil_div(Sq, kRowsPerCta);
+  const int item_rows = kWindow ? win.item_rows() : kRowsPerCta;
+  const int n_tiles = kWindow && win.solo ? 1 : kTiles;   // query tiles of an item
+  const int n_blk = ceil_div(Sq, item_rows);
   const int n_k = ceil_div(Sk, kBN);
   const int n_items = n_blk * BH;
   const int cta = static_cast<int>(blockIdx.x);
@@ -369,11 +384,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int b = 0; b < 2; ++b) {
       mbar_init(&bars->q_full[b], 1);
-      mbar_init(&bars->q_empty[b], kTiles);
+      mbar_init(&bars->q_empty[b], n_tiles);
     }
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&bars->kv_full[s], 1);
-      mbar_init(&bars->kv_empty[s], kTiles);
+      mbar_init(&bars->kv_empty[s], n_tiles);
     }
     for (int i = 0; i < kTiles; ++i) {
       mbar_init(&bars->s_full[i], 1);
@@ -420,10 +435,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const WorkItem w = decode_item<kCausal, kWindow>(k, BH, n_blk, n_k, win);
         const int h = kStrided ? w.bh % lay.H : 0, b = kStrided ? w.bh / lay.H : 0;
-        mbar_arrive_expect_tx(&bars->q_full[qb], kTiles * kTileBytes);
-        for (int i = 0; i < kTiles; ++i) {
+        mbar_arrive_expect_tx(&bars->q_full[qb], n_tiles * kTileBytes);
+        for (int i = 0; i < n_tiles; ++i) {
           void* dst = smem + kOffQ + (qb * kTiles + i) * kTileBytes;
-          const int row = w.blk * kRowsPerCta + i * kBM;
+          const int row = w.blk * item_rows + i * kBM;
           if constexpr (kStrided)
             load_rows(&tm_q, &bars->q_full[qb], dst, row, h, b, lay.q_token_major);
           else
@@ -471,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int j = (kv_it > kStages ? kv_it - kStages : 0); j < kv_it; ++j)
         (void)mbar_wait(&bars->kv_full[j % kStages], (j / kStages) & 1, abort_flag);
     }
-  } else if (warp == kWarpMma || warp == kWarpMma + 1) {
+  } else if (warp == kWarpMma || (warp == kWarpMma + 1 && (!kWindow || n_tiles > 1))) {
     // --------------------------------------------- UMMA issuers, one per tile
     regs_decrease<kRegsControl>();
     if (elect_one()) {
@@ -584,8 +599,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       umma_commit(&bars->drained[i]);
       (void)mbar_wait(&bars->drained[i], 0, abort_flag);
     }
-  } else if (warp > kWarpMma + 1) {
-    regs_decrease<kRegsControl>();  // idle warp of the control warpgroup
+  } else if (warp > kWarpMma) {
+    regs_decrease<kRegsControl>();  // idle warps of the control warpgroup
   } else {
     // -------------------------------------------------------------- softmax
     // warp -> (tile, TMEM lane quarter); thread = one score row.
@@ -664,9 +679,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     PendingRow pend;
     pend.valid = false;
-    for (int n = 0, k; ok && (k = item_of(n, cta, grid)) < n_items; ++n) {
+    for (int n = 0, k; ok && (!kWindow || tile < n_tiles) && (k = item_of(n, cta, grid)) < n_items; ++n) {
       const WorkItem w = decode_item<kCausal, kWindow>(k, BH, n_blk, n_k, win);
-      const int q_idx = w.blk * kRowsPerCta + tile * kBM + row;
+      const int q_idx = w.blk * item_rows + tile * kBM + row;
       const int nkv = tile == 0 ? w.n_kv[0] : w.n_kv[1];
       float m_used = -INFINITY;  // offset of the exponentials (log2 units)
       float m_true = -INFINITY;  // true running row max (log2 units)
@@ -674,44 +689,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int j = 0; j < nkv; ++j, ++it) {
         if (!warp_wait(&bars->s_full[tile], it & 1, abort_flag)) { ok = false; break; }
         tc_fence_after();
-        uint32_t sr[kBN];
-#pragma unroll
-        for (int c = 0; c < kBN / 32; ++c)
-          tmem_ld32(s_addr + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&sr[c * 32]));
-        tmem_ld_wait();
-        // S_i now lives in registers: let the tensor core write the next one.
-        tc_fence_before();
-        mbar_arrive(&bars->s_free[tile]);
-        float* sv = reinterpret_cast<float*>(sr);
+        // whether the tile is masked; window form: whether a border of the visible
+        // range cuts it
         bool last = (j == nkv - 1);
+        [[maybe_unused]] int k0 = 0;
         if constexpr (kWindow) {
-          // `last`: whether a border of the visible range cuts this tile
-          const int k0 = w.key_tile(w.stream_pos(tile, j)) * kBN;
-          const int p_min = win.off + w.blk * kRowsPerCta + tile * kBM, p_max = p_min + kBM - 1;
+          k0 = w.key_tile(w.stream_pos(tile, j)) * kBN;
+          const int p_min = win.off + w.blk * item_rows + tile * kBM, p_max = p_min + kBM - 1;
           last = k0 + kBN - 1 > p_min || (k0 <= p_max - win.window && k0 + kBN > win.sinks);
-          if (last) {
-            const int hi = p_min + row - k0;          // columns up to hi are not in the future,
-            const int lo = hi - win.window + 1;       // from lo on in the window,
-            const int sk = win.sinks - k0;            // below sk sinks
-#pragma unroll
-            for (int q = 0; q < kBN / 32; ++q) {
-              const int h32 = hi - 32 * q, l32 = lo - 32 * q, s32 = sk - 32 * q;
-              const uint32_t past = h32 < 0 ? 0u : h32 >= 31 ? ~0u : (2u << h32) - 1u;
-              const uint32_t near = l32 <= 0 ? ~0u : l32 > 31 ? 0u : ~0u << l32;
-              const uint32_t sink = s32 <= 0 ? 0u : s32 > 31 ? ~0u : (1u << s32) - 1u;
-              const uint32_t seen = past & (near | sink);
-#pragma unroll
-              for (int c = 0; c < 32; ++c)
-                if (!(seen & (1u << c))) sv[32 * q + c] = -INFINITY;
-            }
-          }
-        } else if (last) {
-          const int k0 = j * kBN;
-#pragma unroll
-          for (int c = 0; c < kBN; ++c) {
-            const int k_idx = k0 + c;
-            if ((k_idx >= Sk) || (kCausal && k_idx > q_idx)) sv[c] = -INFINITY;
-          }
         }
         // P_i may be overwritten, and O_i rescaled, once the previous
         // O_i += P_i·V has completed (for j == 0, the previous item's last).
@@ -774,6 +759,43 @@ __global__ void __launch_bounds__(kThreads, 1)
           if constexpr (kWindow) nm = m_used == -INFINITY ? 0.f : nm;
           return f2_pack(nm, nm);
         };
+        // Bits of the columns [k, k + 32) that this row sees.
+        [[maybe_unused]] auto seen_bits = [&](int k) -> uint32_t {
+          const int hi = win.off + q_idx - k;       // columns up to hi are not in the future,
+          const int lo = hi - win.window + 1;       // from lo on in the window,
+          const int sk = win.sinks - k;             // below sk sinks
+          const uint32_t past = hi < 0 ? 0u : hi >= 31 ? ~0u : (2u << hi) - 1u;
+          const uint32_t near = lo <= 0 ? ~0u : lo > 31 ? 0u : ~0u << lo;
+          const uint32_t sink = sk <= 0 ? 0u : sk > 31 ? ~0u : (1u << sk) - 1u;
+          return past & (near | sink);
+        };
+        uint32_t sr[kBN];
+#pragma unroll
+        for (int c = 0; c < kBN / 32; ++c)
+          tmem_ld32(s_addr + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&sr[c * 32]));
+        tmem_ld_wait();
+        // S_i now lives in registers: let the tensor core write the next one.
+        tc_fence_before();
+        mbar_arrive(&bars->s_free[tile]);
+        float* sv = reinterpret_cast<float*>(sr);
+        if (last) {
+          if constexpr (kWindow) {
+#pragma unroll
+            for (int q = 0; q < kBN / 32; ++q) {
+              const uint32_t seen = seen_bits(k0 + 32 * q);
+#pragma unroll
+              for (int c = 0; c < 32; ++c)
+                if (!(seen & (1u << c))) sv[32 * q + c] = -INFINITY;
+            }
+          } else {
+            const int k0 = j * kBN;
+#pragma unroll
+            for (int c = 0; c < kBN; ++c) {
+              const int k_idx = k0 + c;
+              if ((k_idx >= Sk) || (kCausal && k_idx > q_idx)) sv[c] = -INFINITY;
+            }
+          }
+        }
         uint32_t pk[kBN / 4];   // half a row of packed probabilities
         // ---- first half of the keys: its max, then its exponentials
         const float t_a = half_max<0>(sv) * scale_log2;
@@ -851,7 +873,7 @@ cudaError_t launch_typed(cudaStream_t stream, const CUtensorMap& tq, const CUten
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e != cudaSuccess) return e;
   sms = limited_sms(sms);
-  const int n_items = ceil_div(Sq, kRowsPerCta) * BH;
+  const int n_items = ceil_div(Sq, kWindow ? win.item_rows() : kRowsPerCta) * BH;
   dim3 grid(n_items < sms ? n_items : sms);
   kern<<<grid, kThreads, kSmemBytes, stream>>>(tq, tk, tv, to, lay, lse, mx, BH, Sq, Sk, scale_log2,
                                                device_error_word(), win);
@@ -991,6 +1013,8 @@ cudaError_t launch_window_fwd(cudaStream_t stream, const __nv_bfloat16* Q, const
   win.sinks = sinks < Sk ? sinks : Sk;
   win.group = H / Hkv;
   win.off = Sk - Sq;
+  // fewer items of two query tiles than SMs: items of one
+  win.solo = static_cast<long long>(ceil_div(Sq, kRowsPerCta)) * BH < limited_sms(current_sm_count());
   const float sl2 = scale * kLog2e;
 #define ND_WINDOW_LAUNCH(F, S_)                                                                   \
   launch_typed<true, F, S_, true>(stream, tq, tk, tv, to, lay, lse, row_max, BH, Sq, Sk, sl2, win)

@@ -21,6 +21,7 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <utility>
 
 namespace nd {
@@ -77,17 +78,38 @@ cudaError_t launch_ex(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t sm
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
-// Launch the second kernel of one entry point's pair so that it may start up
-// while the first still runs, whatever the calling thread's mode: it waits for
-// the first (pdl_wait) before it reads or writes anything.
+// Launch a kernel that reads and writes nothing before pdl_wait(), whatever the
+// calling thread's mode: its blocks may be placed while the kernel before it
+// still runs, and it sees that kernel's work as after an ordinary launch.
 template <typename... KArgs, typename... Args>
 cudaError_t launch_dependent(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
-                             cudaStream_t stream, Args&&... args) {
+                             cudaStream_t stream, int cluster_x, Args&&... args) {
   const bool was = pdl_enabled();
   set_pdl_enabled(true);
   const cudaError_t e =
-      launch_ex(kernel, grid, block, smem, stream, 1, true, std::forward<Args>(args)...);
+      launch_ex(kernel, grid, block, smem, stream, cluster_x, true, std::forward<Args>(args)...);
   set_pdl_enabled(was);
+  return e;
+}
+
+// Allow `kernel` up to `bytes` of dynamic shared memory, once per device and
+// growth: `state` (static in the caller, zero at first) holds what each device
+// has been told.
+struct SmemOptIn {
+  std::atomic<int> bytes[64];
+};
+template <typename... KArgs>
+cudaError_t allow_smem(void (*kernel)(KArgs...), int bytes, SmemOptIn& state) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (state.bytes[dev].load(std::memory_order_acquire) >= bytes) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) {
+    int had = state.bytes[dev].load(std::memory_order_relaxed);
+    while (had < bytes && !state.bytes[dev].compare_exchange_weak(had, bytes, std::memory_order_release)) {}
+  }
   return e;
 }
 

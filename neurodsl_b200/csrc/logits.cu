@@ -457,11 +457,11 @@ cudaError_t launch_typed(cudaStream_t stream, const LogitsPenalty& a, int* err_w
   }
   part = part < kMaxPart ? part : kMaxPart;
   const size_t smem = static_cast<size_t>(table) * 12 + (n > 0 || a.mask ? static_cast<size_t>(part) / 4 + 8 : 0);
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             static_cast<int>(smem));
+  static SmemOptIn opt_in[2];
+  const cudaError_t e = allow_smem(kern, static_cast<int>(smem), opt_in[vec]);
   if (e != cudaSuccess) return e;
-  return launch_ex(kern, dim3(static_cast<unsigned>(a.rows) * nc), dim3(kThreads), smem, stream, nc,
-                   true, a, table, part, err_word);
+  return launch_dependent(kern, dim3(static_cast<unsigned>(a.rows) * nc), dim3(kThreads), smem, stream,
+                          nc, a, table, part, err_word);
 }
 
 }  // namespace

@@ -329,8 +329,8 @@ __global__ void __launch_bounds__(256)
 
 template <int kThreads, int kR>
 cudaError_t launch_select(cudaStream_t stream, const PagedEvict& a, unsigned heads, int* err_word) {
-  return launch_ex(paged_select_kernel<kThreads, kR>, dim3(heads), dim3(kThreads), 0, stream, 1, true,
-                   a, err_word);
+  return launch_dependent(paged_select_kernel<kThreads, kR>, dim3(heads), dim3(kThreads), 0, stream, 1,
+                          a, err_word);
 }
 
 }  // namespace
@@ -342,9 +342,9 @@ cudaError_t launch_paged_store(cudaStream_t stream, const __nv_bfloat16* src, lo
   const long long chunks = (static_cast<long long>(pool.Hkv) * kVec + 31) / 32;
   const bool few = B * static_cast<long long>(S) * chunks < 32 * current_sm_count();
   const long long warps = chunks * B * (few ? S : (S + 3) / 4);
-  return launch_ex(few ? paged_store_kernel<1> : paged_store_kernel<4>,
-                   dim3(static_cast<unsigned>((warps + 7) / 8)), dim3(256), 0, stream, 1, true, src,
-                   ld, k_col, v_col, pool, B, S, pos0, pos0_dev, lens, err_word);
+  return launch_dependent(few ? paged_store_kernel<1> : paged_store_kernel<4>,
+                          dim3(static_cast<unsigned>((warps + 7) / 8)), dim3(256), 0, stream, 1, src,
+                          ld, k_col, v_col, pool, B, S, pos0, pos0_dev, lens, err_word);
 }
 
 cudaError_t launch_paged_evict(cudaStream_t stream, const PagedEvict& a, int* err_word) {
@@ -364,7 +364,7 @@ cudaError_t launch_paged_evict(cudaStream_t stream, const PagedEvict& a, int* er
   if (e != cudaSuccess) return e;
   const long long warps = static_cast<long long>(heads) * ((a.budget + 31) / 32);
   return launch_dependent(paged_gather_kernel, dim3(static_cast<unsigned>((warps + 7) / 8)), dim3(256),
-                          0, stream, a, err_word);
+                          0, stream, 1, a, err_word);
 }
 
 }  // namespace nd

@@ -581,17 +581,19 @@ def _device_of(t, name):
 
 def _tensor(t, name, dtype, dims, dev, contiguous=True):
     """Checks one tensor (dtype None: float32 or bfloat16; dims None: any)."""
+    if (isinstance(t, torch.Tensor) and t.get_device() == dev and t.dtype is dtype
+            and (dims is None or t.dim() == dims) and (not contiguous or t.is_contiguous())):
+        return
     d = t.get_device() if isinstance(t, torch.Tensor) else -1
+    if d < 0:
+        raise TypeError(f"{name} must be a CUDA tensor")
     if d != dev:
-        if d < 0:
-            raise TypeError(f"{name} must be a CUDA tensor")
         raise ValueError(f"{name} is on cuda:{d}, the call's first tensor on cuda:{dev}")
-    dt = t.dtype
     if dtype is None:
-        if dt not in _DT:
-            raise ValueError(f"{name} must be float32 or bfloat16, got {dt}")
-    elif dt is not dtype:
-        raise TypeError(f"{name} must be {dtype}, got {dt}")
+        if t.dtype not in _DT:
+            raise ValueError(f"{name} must be float32 or bfloat16, got {t.dtype}")
+    elif t.dtype is not dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
     if dims is not None and t.dim() != dims:
         raise ValueError(f"{name} must have {dims} dims, got shape {tuple(t.shape)}")
     if contiguous and not t.is_contiguous():
