@@ -105,6 +105,16 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool t
 __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+// A box of K or V rows whose lines L2 may give up first: they are read once a
+// step, and would push out what is read again (the scores, the partials).
+__device__ __forceinline__ void tma_load_rows(const CUtensorMap* map, uint64_t* bar, void* dst, int row,
+                                              uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%3, %4}], [%2], %5;" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(0), "r"(row), "l"(policy)
+      : "memory");
+}
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -300,6 +310,8 @@ __device__ __forceinline__ void produce(const Params& p, const CUtensorMap* tm_k
     }
   };
   look_up(c);
+  uint64_t policy = 0;
+  if constexpr (kTma) asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
   bool ok = true;
   int it = 0;
   for (; at < hi; ++it) {
@@ -317,8 +329,8 @@ __device__ __forceinline__ void produce(const Params& p, const CUtensorMap* tm_k
         // a box that starts past the pool's last row reads as zeros
         const int r = static_cast<int>(row[0] < 0 ? static_cast<long long>(p.n_pages) * p.Hkv * p.page_size
                                                   : row[0]);
-        tma_load_2d(tm_k, &bars->full[s], dst + lane * p.box * kRowBytes, 0, r);
-        tma_load_2d(tm_v, &bars->full[s], dst + kTileBytes + lane * p.box * kRowBytes, 0, r);
+        tma_load_rows(tm_k, &bars->full[s], dst + lane * p.box * kRowBytes, r, policy);
+        tma_load_rows(tm_v, &bars->full[s], dst + kTileBytes + lane * p.box * kRowBytes, r, policy);
       }
     } else {
       const int piece = lane & 7;
