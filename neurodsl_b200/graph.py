@@ -318,7 +318,7 @@ def _infer_output_shape(op: str, inputs, attrs):
     if op in ("identity", "flash_attn", "flash_attention", "layernorm", "gelu",
               "scale_mask", "softmax"):
         return tuple(inputs[0].shape)
-    if op == "kv_decode_attn":
+    if op in ("kv_decode_attn", "window_attention", "paged_decode_attn", "logits_penalty"):
         return tuple(inputs[0].shape)
     if op == "embedding":                                    # [E, idx]
         return (inputs[1].numel(), inputs[0].shape[1])
@@ -661,6 +661,93 @@ def _dispatch_kv_decode_attn(dev, output_buffer, inputs, attrs, out_sym, out_nod
     return output_buffer
 
 
+def _dispatch_window_attention(dev, output_buffer, inputs, attrs, out_sym, out_node, ctx_store):
+    """:window_attention — :flash_attention with a sliding window and sinks:
+    inputs q (S, H·D), k and v (Sk, Hkv·D), the queries being the last S of the
+    Sk positions; attrs :n_heads, :window, optional :n_kv_heads, :sinks, :d_head."""
+    q, k, v = inputs[0], inputs[1], inputs[2]
+    S, d = q.shape
+    H = attrs["n_heads"]
+    Hkv = attrs.get("n_kv_heads", H)
+    D = attrs.get("d_head", d // H)
+    if H * D != d or Hkv * D != k.shape[1]:
+        raise NeuroDSLError(2, f"heads {H} / {Hkv} x d_head {D} != widths {d} / {k.shape[1]}")
+    Sk = k.shape[0]
+    lse = out_node.aux_data.get("flash_l")
+    if lse is None or tuple(lse.shape) != (H, S):
+        lse = torch.empty((H, S), dtype=torch.float32, device=dev.torch_device)
+        out_node.aux_data["flash_l"] = lse
+        out_node.aux_data["flash_m"] = torch.empty_like(lse)
+    m = out_node.aux_data["flash_m"]
+    buf, aliased = _alias_safe(output_buffer, out_node, inputs)
+    ops.window_attn_fwd(_token_major_view(_bf16_rows(q), S, H, D),
+                        _token_major_view(_bf16_rows(k), Sk, Hkv, D),
+                        _token_major_view(_bf16_rows(v), Sk, Hkv, D), int(attrs["window"]),
+                        sinks=int(attrs.get("sinks", 0)), scale=1.0 / math.sqrt(D),
+                        out=_token_major_view(buf, S, H, D), lse=lse, row_max=m)
+    if aliased:
+        _copy_back(buf, output_buffer)
+    _store_ctx(ctx_store, out_sym, {"Q": q, "K": k, "V": v, "out": output_buffer, "l": lse, "m": m,
+                                    "d_head": D, "causal": True, "n_heads": H,
+                                    "window": attrs["window"], "sinks": attrs.get("sinks", 0)})
+    return output_buffer
+
+
+def _dispatch_paged_decode_attn(dev, output_buffer, inputs, attrs, out_sym, out_node, ctx_store):
+    """:paged_decode_attn — inputs [q (B, H·D), k_pages, v_pages
+    ([n_pages][Hkv][page][D] bf16), block_table, lens (int32)] (+ optional [k_new,
+    v_new] (B, Hkv·D) appended at lens - 1), attrs :n_heads, optional :window,
+    :sinks.  Output (B, H·D)."""
+    q, kp, vp, table, lens = inputs[:5]
+    B, d = q.shape
+    H = attrs["n_heads"]
+    Hkv, page, D = kp.shape[1], kp.shape[2], kp.shape[3]
+    if H * D != d:
+        raise NeuroDSLError(2, f"n_heads {H} x d_head {D} != dim {d}")
+    kn = vn = None
+    if len(inputs) == 7:
+        kn = _bf16_rows(inputs[5]).view(B, Hkv, D)
+        vn = _bf16_rows(inputs[6]).view(B, Hkv, D)
+    need = ops.paged_decode_workspace_size(B, H, Hkv, table.shape[1] * page)
+    ws = out_node.aux_data.get("decode_workspace")
+    if ws is None or ws.numel() < need:
+        ws = torch.zeros(need, dtype=torch.uint8, device=dev.torch_device)
+        out_node.aux_data["decode_workspace"] = ws
+    out, lse = ops.paged_decode_attn(_bf16_rows(q).view(B, H, D), kp, vp, table, lens, k_new=kn,
+                                     v_new=vn, window=int(attrs.get("window", 0)),
+                                     sinks=int(attrs.get("sinks", 0)), scale=1.0 / math.sqrt(D),
+                                     out=output_buffer.view(B, H, D), workspace=ws)
+    out_node.aux_data["decode_lse"] = lse
+    _store_ctx(ctx_store, out_sym, {"q": q, "lens": lens, "l": lse, "n_heads": H, "d_head": D})
+    return output_buffer
+
+
+def _dispatch_logits_penalty(dev, output_buffer, inputs, attrs, out_sym, out_node, ctx_store):
+    """:logits_penalty — inputs [logits (B, V)] (+ optional [history (B, n) int32]),
+    attrs :repetition, :presence, :frequency (numbers or (B,) tensors),
+    :bias_ids, :bias, :mask.  The greedy tokens are aux_data "token"."""
+    logits = inputs[0]
+    B = logits.shape[0]
+    history = inputs[1] if len(inputs) > 1 else None
+
+    def per_row(name):
+        x = attrs.get(name)
+        if x is None or isinstance(x, torch.Tensor):
+            return x
+        return torch.full((B,), float(x), dtype=torch.float32, device=dev.torch_device)
+
+    buf, aliased = _alias_safe(output_buffer, out_node, inputs)
+    _, idx = ops.logits_penalty(logits, history=history, repetition=per_row("repetition"),
+                                presence=per_row("presence"), frequency=per_row("frequency"),
+                                bias_ids=attrs.get("bias_ids"), bias=attrs.get("bias"),
+                                mask=attrs.get("mask"), out=buf)
+    if aliased:
+        _copy_back(buf, output_buffer)
+    out_node.aux_data["token"] = idx
+    _store_ctx(ctx_store, out_sym, {"logits": logits, "token": idx})
+    return output_buffer
+
+
 _GELU_APPROX = {"sigmoid": "sigmoid", "tanh": "tanh", "erf": "erf"}
 
 
@@ -793,6 +880,9 @@ def register_b200_ops():
     register_op("flash_attn", _dispatch_flash_attn)
     register_op("flash_attention", _dispatch_flash_attention)
     register_op("kv_decode_attn", _dispatch_kv_decode_attn)
+    register_op("window_attention", _dispatch_window_attention)
+    register_op("paged_decode_attn", _dispatch_paged_decode_attn)
+    register_op("logits_penalty", _dispatch_logits_penalty)
     register_op("fused_linear_gelu", _dispatch_fused_linear_gelu)
     register_op("fused_linear_residual", _dispatch_fused_linear_residual)
     register_op("layernorm", _dispatch_layernorm)
