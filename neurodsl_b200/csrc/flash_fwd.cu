@@ -51,9 +51,13 @@
 // a warp's rows sees a key, one exponential in ten, measured slower: 141 against
 // 137 us at B=2, H=16, S=8192, window 1024, 4 sinks; a step's time is its chain
 // from scores to weights, not the exponentials alone.)  With fewer items of 256
-// rows than SMs an item is one query tile: a step takes less time, and twice as
-// many SMs work (27.1 -> 20.2 us for 509 queries against 4099 keys, B=2, H=16,
-// window 1024).
+// rows than SMs an item is one query tile (solo), which the two softmax groups
+// share: group i takes every second K/V tile of the stream, from the i-th on,
+// with its own scores, weights and accumulator, and at the item's end group 1
+// hands its row sums and accumulator over through shared memory.  So twice as
+// many SMs work, and each takes two K/V tiles in little more than the time of
+// one (509 queries against 4099 keys, B=2, H=16, window 1024: 27.1 us in items of
+// 256 rows, 20.4 with one group a tile, 18.3 so).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <limits.h>
@@ -136,6 +140,7 @@ struct Bars {
   uint64_t p_full[kTiles];   // P_i(k) written, O_i rescaled and read out (128 threads)
   uint64_t o_done[kTiles];   // O_i += P_i(k)·V_k complete (UMMA commit)
   uint64_t drained[kTiles];
+  uint64_t x_full, x_empty;  // solo items: group 1's share handed over / read
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -258,9 +263,20 @@ struct WorkItem {
   // window form: the stream is K/V tiles [0, n_sink), then lo, lo + 1, ...;
   // query tile 1 leaves out the first `skip` (0 or 1) of the latter
   int n_sink, lo, skip;
-  // K/V tile at stream position s, and stream position of query tile i's j-th
-  __device__ __forceinline__ int key_tile(int s) const { return s < n_sink ? s : lo + s - n_sink; }
+  // solo items: group i takes the stream positions i, i + 2, ...  A stream of an
+  // odd number of tiles ends with a copy of its last (positions past `copies`),
+  // of which group 1 sees nothing: the groups so keep to every second position
+  // across items too, and neither waits for a ring stage that it holds itself
+  // (its scores run one tile ahead of its weights).
+  int solo, copies;
+  // K/V tile at stream position s, and stream position of query tile (solo:
+  // group) i's j-th
+  __device__ __forceinline__ int key_tile(int s) const {
+    if (s > copies) s = copies;
+    return s < n_sink ? s : lo + s - n_sink;
+  }
   __device__ __forceinline__ int stream_pos(int i, int j) const {
+    if (solo) return 2 * j + i;
     return (i == 1 && j >= n_sink) ? j + skip : j;
   }
 };
@@ -269,7 +285,7 @@ struct WorkItem {
 // a K/V head and the position of query 0.
 struct FlashWindow {
   int window, sinks, group, off;
-  int solo;       // items of one query tile (the second tile's warps are idle)
+  int solo;       // items of one query tile, which both groups share
   __host__ __device__ int item_rows() const { return solo ? kBM : kRowsPerCta; }
 };
 
@@ -286,11 +302,16 @@ __device__ __forceinline__ WorkItem decode_item(int k, int BH, int n_blk, int n_
     const int sink_tiles = ceil_div(win.sinks, kBN);
     w.lo = lo0;
     w.n_sink = min(sink_tiles, lo0);
+    w.solo = win.solo;
     if (win.solo) {
       w.skip = 0;
-      w.n_total = w.n_kv[0] = w.n_kv[1] = w.n_sink + hi0 - lo0 + 1;
+      const int n = w.n_sink + hi0 - lo0 + 1;
+      w.copies = n - 1;
+      w.n_kv[0] = w.n_kv[1] = (n + 1) / 2;
+      w.n_total = 2 * w.n_kv[0];
       return w;
     }
+    w.copies = 0x7fffffff;
     const int hi1 = min((p0 + 2 * kBM - 1) / kBN, n_k - 1);
     // rows past Sq may have their whole window past Sk
     const int lo1 = min(max(0, p0 + kBM - win.window + 1) / kBN, hi1);
@@ -300,7 +321,8 @@ __device__ __forceinline__ WorkItem decode_item(int k, int BH, int n_blk, int n_
     w.n_kv[1] = w.n_total - w.skip;
     return w;
   }
-  w.n_sink = w.lo = w.skip = 0;
+  w.n_sink = w.lo = w.skip = w.solo = 0;
+  w.copies = 0x7fffffff;
   // Heavy items first: with a causal mask the last query rows see the most keys.
   w.blk = kCausal ? (n_blk - 1 - k / BH) : k / BH;
   w.bh = k % BH;
@@ -348,6 +370,7 @@ struct Cursor {
   int n_sink, skip;   // window form: as in WorkItem
 };
 
+
 // A row whose output is still to be written (the previous item's).
 struct PendingRow {
   float l, m_used, m_true;
@@ -374,7 +397,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int item_rows = kWindow ? win.item_rows() : kRowsPerCta;
-  const int n_tiles = kWindow && win.solo ? 1 : kTiles;   // query tiles of an item
+  const bool solo = kWindow && win.solo != 0;
+  const int n_tiles = solo ? 1 : kTiles;   // query tiles of an item
   const int n_blk = ceil_div(Sq, item_rows);
   const int n_k = ceil_div(Sk, kBN);
   const int n_items = n_blk * BH;
@@ -384,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int b = 0; b < 2; ++b) {
       mbar_init(&bars->q_full[b], 1);
-      mbar_init(&bars->q_empty[b], n_tiles);
+      mbar_init(&bars->q_empty[b], kTiles);
     }
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&bars->kv_full[s], 1);
@@ -397,6 +421,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&bars->o_done[i], 1);
     }
     for (int i = 0; i < kTiles; ++i) mbar_init(&bars->drained[i], 1);
+    if constexpr (kWindow) {
+      mbar_init(&bars->x_full, 128);
+      mbar_init(&bars->x_empty, 128);
+    }
     bars->abort_flag = 0;
     fence_barrier_init();
   }
@@ -486,7 +514,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int j = (kv_it > kStages ? kv_it - kStages : 0); j < kv_it; ++j)
         (void)mbar_wait(&bars->kv_full[j % kStages], (j / kStages) & 1, abort_flag);
     }
-  } else if (warp == kWarpMma || (warp == kWarpMma + 1 && (!kWindow || n_tiles > 1))) {
+  } else if (warp == kWarpMma || warp == kWarpMma + 1) {
     // --------------------------------------------- UMMA issuers, one per tile
     regs_decrease<kRegsControl>();
     if (elect_one()) {
@@ -514,7 +542,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       // ring position of the cursor's tile
       auto ring_pos = [&](const Cursor& c) {
-        if constexpr (kWindow) return c.base + c.j + (c.j >= c.n_sink ? c.skip : 0);
+        if constexpr (kWindow) return c.base + (solo ? 2 * c.j + i : c.j + (c.j >= c.n_sink ? c.skip : 0));
         return c.base + c.j;
       };
       auto advance = [&](Cursor& c) {
@@ -562,7 +590,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int s = pos % kStages, qb = c.n & 1;
 #pragma unroll
           for (int kk = 0; kk < kD / 16; ++kk) {
-            const uint64_t a = sdesc_sw128(sQ + (qb * kTiles + i) * kTileBytes + kk * 32, 16, 1024);
+            const uint64_t a = sdesc_sw128(sQ + (qb * kTiles + (solo ? 0 : i)) * kTileBytes + kk * 32, 16, 1024);
             const uint64_t b = sdesc_sw128(sK + s * kTileBytes + kk * 32, 16, 1024);
             umma_ss(tmem + col_s(i), a, b, kIdescS, kk > 0 ? 1u : 0u);
           }
@@ -587,7 +615,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           umma_commit(&bars->o_done[i]);
           ++pv_cnt;
           umma_commit(&bars->kv_empty[s]);
-          if (p.j + 1 == p.nkv && p.nkv + (kWindow ? p.skip : 0) < p.total) {
+          if (!solo && p.j + 1 == p.nkv && p.nkv + (kWindow ? p.skip : 0) < p.total) {
             skipped = p.base + p.nkv;
             release_skipped();
           }
@@ -599,8 +627,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       umma_commit(&bars->drained[i]);
       (void)mbar_wait(&bars->drained[i], 0, abort_flag);
     }
-  } else if (warp > kWarpMma) {
-    regs_decrease<kRegsControl>();  // idle warps of the control warpgroup
+  } else if (warp > kWarpMma + 1) {
+    regs_decrease<kRegsControl>();  // idle warp of the control warpgroup
   } else {
     // -------------------------------------------------------------- softmax
     // warp -> (tile, TMEM lane quarter); thread = one score row.
@@ -620,12 +648,37 @@ __global__ void __launch_bounds__(kThreads, 1)
     // box and written by one tensor store (rows past Sq are clipped by it).
     uint8_t* stage = smem + kOffStage + warp * kStageBytesWarp;
     const uint32_t r7 = static_cast<uint32_t>(lane & 7);
-    auto write_row = [&](const PendingRow& pr) {
+    // Solo items: group 1's rows pass through the staging area of its own warps,
+    // 16 pieces of 16 bytes a row, swizzled; its offsets, sums and maxima through
+    // the Q tile that solo items leave unused.
+    const uint32_t x_row = smem_u32(smem + kOffStage) + (kSoftmaxThreads / 64) * kStageBytesWarp +
+                           static_cast<uint32_t>(row) * (kD * 4);
+    float* x_stat = reinterpret_cast<float*>(smem + kOffQ + kTileBytes) + row;
+    auto write_row = [&](PendingRow pr) {
       uint32_t orr[kD];
 #pragma unroll
       for (int c = 0; c < kD / 32; ++c)
         tmem_ld32(o_addr + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&orr[c * 32]));
       tmem_ld_wait();
+      if constexpr (kWindow) {
+        if (solo) {
+          // group 1's share of the row, on the larger of the two offsets
+          const float m1 = x_stat[0], l1 = x_stat[128];
+          const float m = fmaxf(pr.m_used, m1);
+          const float a0 = fast_exp2(pr.m_used - m), a1 = fast_exp2(m1 - m);
+          pr.l = pr.l * a0 + l1 * a1;
+          pr.m_used = m;
+          pr.m_true = fmaxf(pr.m_true, x_stat[256]);
+#pragma unroll
+          for (int c = 0; c < kD / 4; ++c) {
+            uint32_t v[4];
+            ld_shared_v4(x_row + ((c ^ (row & 15)) << 4), v);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              orr[4 * c + e] = __float_as_uint(__uint_as_float(orr[4 * c + e]) * a0 + __uint_as_float(v[e]) * a1);
+          }
+        }
+      }
       const float inv_l = 1.f / pr.l;
       // the previous store from this buffer has finished reading it
       if (lane == 0) bulk_wait_read_all();
@@ -679,9 +732,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     PendingRow pend;
     pend.valid = false;
-    for (int n = 0, k; ok && (!kWindow || tile < n_tiles) && (k = item_of(n, cta, grid)) < n_items; ++n) {
+    for (int n = 0, k; ok && (k = item_of(n, cta, grid)) < n_items; ++n) {
       const WorkItem w = decode_item<kCausal, kWindow>(k, BH, n_blk, n_k, win);
-      const int q_idx = w.blk * item_rows + tile * kBM + row;
+      const int q_idx = w.blk * item_rows + (solo ? 0 : tile * kBM) + row;
       const int nkv = tile == 0 ? w.n_kv[0] : w.n_kv[1];
       float m_used = -INFINITY;  // offset of the exponentials (log2 units)
       float m_true = -INFINITY;  // true running row max (log2 units)
@@ -695,8 +748,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         [[maybe_unused]] int k0 = 0;
         if constexpr (kWindow) {
           k0 = w.key_tile(w.stream_pos(tile, j)) * kBN;
-          const int p_min = win.off + w.blk * item_rows + tile * kBM, p_max = p_min + kBM - 1;
+          const int p_min = win.off + w.blk * item_rows + (solo ? 0 : tile * kBM), p_max = p_min + kBM - 1;
           last = k0 + kBN - 1 > p_min || (k0 <= p_max - win.window && k0 + kBN > win.sinks);
+          if (w.stream_pos(tile, j) > w.copies) {   // the copy: nothing of it is seen
+            k0 = 0x40000000;
+            last = true;
+          }
         }
         // P_i may be overwritten, and O_i rescaled, once the previous
         // O_i += P_i·V has completed (for j == 0, the previous item's last).
@@ -834,6 +891,36 @@ __global__ void __launch_bounds__(kThreads, 1)
       pend.q_idx = q_idx;
       pend.bh = w.bh;
       pend.valid = true;
+      if constexpr (kWindow) {
+        if (solo) {
+          // the item ends here: group 1 hands its share over, group 0 writes
+          pend.valid = false;
+          if (!warp_wait(&bars->o_done[tile], (it - 1) & 1, abort_flag)) { ok = false; break; }
+          tc_fence_after();
+          if (tile == 1) {
+            if (n > 0 && !warp_wait(&bars->x_empty, (n - 1) & 1, abort_flag)) { ok = false; break; }
+#pragma unroll
+            for (int h = 0; h < kD / 32; ++h) {
+              uint32_t orr[32];
+              tmem_ld32(o_addr + h * 32, orr);
+              tmem_ld_wait();
+#pragma unroll
+              for (int c = 0; c < 8; ++c)
+                st_shared_v4(x_row + (((8 * h + c) ^ (row & 15)) << 4), orr[4 * c], orr[4 * c + 1], orr[4 * c + 2],
+                             orr[4 * c + 3]);
+            }
+            x_stat[0] = m_used;
+            x_stat[128] = l;
+            x_stat[256] = m_true;
+            mbar_arrive(&bars->x_full);
+          } else {
+            if (!warp_wait(&bars->x_full, n & 1, abort_flag)) { ok = false; break; }
+            write_row(pend);
+            mbar_arrive(&bars->x_empty);
+          }
+          tc_fence_before();
+        }
+      }
     }
     // the last item's rows, once its last P·V has completed
     if (ok && pend.valid) {
@@ -864,15 +951,11 @@ cudaError_t launch_typed(cudaStream_t stream, const CUtensorMap& tq, const CUten
                          float* lse, float* mx, int BH, int Sq, int Sk, float scale_log2,
                          const FlashWindow& win = {}) {
   auto kern = flash_fwd_kernel<kCausal, kOutF32, kStrided, kWindow>;
-  cudaError_t e =
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+  static SmemOptIn opt_in;
+  const cudaError_t e = allow_smem(kern, kSmemBytes, opt_in);
   if (e != cudaSuccess) return e;
   // Persistent CTAs: one per SM (at most one fits, by shared memory and TMEM).
-  int dev = 0, sms = 0;
-  e = cudaGetDevice(&dev);
-  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  if (e != cudaSuccess) return e;
-  sms = limited_sms(sms);
+  const int sms = limited_sms(current_sm_count());
   const int n_items = ceil_div(Sq, kWindow ? win.item_rows() : kRowsPerCta) * BH;
   dim3 grid(n_items < sms ? n_items : sms);
   kern<<<grid, kThreads, kSmemBytes, stream>>>(tq, tk, tv, to, lay, lse, mx, BH, Sq, Sk, scale_log2,

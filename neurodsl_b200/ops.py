@@ -569,6 +569,8 @@ def add_layernorm(x, p, bias=None, gamma=None, beta=None, eps=1e-5, s_out=None, 
 # cost little: plain attribute reads, one device number for all tensors.
 _BF16, _F32, _INT32 = torch.bfloat16, torch.float32, torch.int32
 _I64x3 = ctypes.c_int64 * 3
+_cuda_device = torch._C._cuda_getDevice          # the current device's number
+_raw_stream = torch._C._cuda_getCurrentRawStream  # a device's current stream as an int
 
 
 def _device_of(t, name):
@@ -622,7 +624,7 @@ def _stream_of(dev, stream):
     """The raw stream of a call: the caller's, which must be one of the
     tensors' device, or that device's current one."""
     if stream is None:
-        return torch._C._cuda_getCurrentRawStream(dev)
+        return _raw_stream(dev)
     if stream.device.index != dev:
         raise ValueError(f"stream is on {stream.device}, the tensors on cuda:{dev}")
     return stream.cuda_stream
@@ -630,7 +632,7 @@ def _stream_of(dev, stream):
 
 def _call(fn, dev, *args):
     """fn(*args) with the tensors' device current."""
-    if torch._C._cuda_getDevice() == dev:
+    if _cuda_device() == dev:
         rc = fn(*args)
     else:
         with torch.cuda.device(dev):

@@ -134,12 +134,19 @@ def test_writes_only_its_rows():
 
 
 def test_full_window_is_causal_attention():
+    """Small problems sum a row's keys in two groups, nd_flash_attn_fwd in one, so
+    the two agree to rounding: each lies within the bounds above of the same
+    exact result, hence within twice those of the other (bits: 2 * (2 * 2^-8 A +
+    2^-8 |O|), and the fp32 terms of lse and the maxima, which no grouping
+    changes for the maxima)."""
     ops = _ops()
     Q, K, V, out = make("token", 2, 4, 4, 333, 333, seed=2)
     a = ops.window_attn_fwd(Q, K, V, 333)
     b = ops.flash_attn_fwd(Q, K, V, causal=True)
-    for x, y in zip(a, b):
-        assert torch.equal(x, y)
+    want = reference(Q, K, V, 333, 0, 0.125)
+    compare(a, want, torch.bfloat16, 333)
+    compare(b, want, torch.bfloat16, 333)
+    assert torch.equal(a[2], b[2])
 
 
 def test_same_bits_every_time_and_in_a_graph():
