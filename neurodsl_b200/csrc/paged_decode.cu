@@ -29,9 +29,13 @@
 // the range whatever heads its tiles belong to, and four warps take 16 keys
 // of a tile each, with their own running max and sum; they join through shared
 // memory at a head's end while the next head's tiles are already arriving.
-// Two producers, by the page size: where a page holds whole groups of 16 rows,
-// one TMA box per group (or per tile, from 64 rows on) with the 128-byte
-// swizzle; else 16-byte cp.async pieces into the same layout.
+// Two producers, by the page size: where a page holds whole boxes of 8 rows or
+// more (the largest power of two that divides it, up to the tile), one TMA box
+// each with the 128-byte swizzle; else 16-byte cp.async pieces into the same
+// layout, by four warps (two beside 16 query heads, whose consumers need the
+// registers).  64 sequences of 2048 keys, 12 heads: 68.6 us at pages of 64 rows,
+// 71.0 at 16, 75.6 at 24 (by pieces 119.8 with one warp); by pieces 86.4 at 100
+// (98.3 in boxes of 4), 94.7 at 7, 119.4 at 1.
 //
 // S = Q K^T takes Q as the 16-row operand of mma.m16n8k16 (query head = row)
 // and K's rows as they lie (ldmatrix).  The scores' fragment is then, packed to
@@ -57,10 +61,19 @@ namespace {
 constexpr int kD = 64;
 constexpr int kWarps = 4;                       // consumer warps
 constexpr int kConsumers = kWarps * 32;
-constexpr int kThreads = kConsumers + 32;       // + the producer warp
+constexpr int kMinBox = 8;                      // rows of a TMA box, at least
 constexpr int kKeysPerWarp = 16;
 constexpr int kTile = kWarps * kKeysPerWarp;    // keys per tile
-constexpr int kStages = 4;                      // ring depth, in tiles
+// The producer's warps, the ring's depth in tiles and the CTAs of an SM: more
+// warps where they copy piece by piece, and so fewer CTAs, with deeper rings.
+template <int kRows, bool kTma>
+struct Shape {
+  static constexpr int kProducers = kTma ? 1 : kRows == 8 ? 4 : 2;
+  static constexpr int kThreads = kConsumers + 32 * kProducers;
+  static constexpr int kStages = kTma ? 4 : kRows == 8 ? 6 : 5;
+  static constexpr int kCtas = kTma && kRows == 8 ? 3 : 2;
+};
+constexpr int kMaxStages = 6;
 constexpr int kRowBytes = kD * 2;
 constexpr int kTileBytes = kTile * kRowBytes;   // K or V of a tile
 constexpr int kStageBytes = 2 * kTileBytes;
@@ -279,34 +292,34 @@ __device__ __forceinline__ long long pool_row(const Params& p, int b, int h, int
 }
 
 struct Bars {
-  uint64_t full[kStages];    // a tile has landed
-  uint64_t empty[kStages];   // the four consumer warps have read it
+  uint64_t full[kMaxStages];    // a tile has landed
+  uint64_t empty[kMaxStages];   // the four consumer warps have read it
   int abort_flag;
 };
 
 // ---- the producer warp: every tile of the range into the ring, in order.
 // Rows without a visible key are not copied (their stage bytes are whatever was
 // there; the consumers mask them), rows of a page outside the pool are zeros.
-template <bool kTma>
+template <bool kTma, int kStages, int kProducers>
 __device__ __forceinline__ void produce(const Params& p, const CUtensorMap* tm_k,
                                         const CUtensorMap* tm_v, int heads, Cursor c, long long at,
                                         long long hi, uint8_t* ring, Bars* bars) {
   const int lane = threadIdx.x & 31;
   volatile int* abort_flag = &bars->abort_flag;
-  // what a lane fetches: with TMA, box `lane` of the tile; else rows lane and
-  // lane + 32.  Looked up one tile ahead.
-  long long row[2] = {-2, -2};     // -2: nothing to copy, -1: zeros
+  // what a lane looks up, one tile ahead: with TMA, box `lane` of the tile; else
+  // the row `lane` of its warp's share of the tile
+  constexpr int kShare = kTile / kProducers;
+  static_assert(kTma ? kProducers == 1 : kShare <= 32, "a row a lane");
+  const int row0 = kTma ? 0 : (static_cast<int>(threadIdx.x) - kConsumers) / 32 * kShare;
+  long long row = -2;     // -2: nothing to copy, -1: zeros
   auto look_up = [&](const Cursor& x) {
     const int key0 = x.key_tile() * kTile, h = x.hp / p.parts;
     if constexpr (kTma) {
       const int key = key0 + lane * p.box;
-      row[0] = lane * p.box < kTile && any_visible(p, x.s, key, p.box) ? pool_row(p, x.b, h, key) : -2;
+      row = lane * p.box < kTile && any_visible(p, x.s, key, p.box) ? pool_row(p, x.b, h, key) : -2;
     } else {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int key = key0 + lane + 32 * i;
-        row[i] = visible(p, x.s, key) ? pool_row(p, x.b, h, key) : -2;
-      }
+      const int key = key0 + row0 + lane;
+      row = lane < kShare && visible(p, x.s, key) ? pool_row(p, x.b, h, key) : -2;
     }
   };
   look_up(c);
@@ -322,27 +335,27 @@ __device__ __forceinline__ void produce(const Params& p, const CUtensorMap* tm_k
     }
     uint8_t* dst = ring + s * kStageBytes;
     if constexpr (kTma) {
-      const bool go = row[0] != -2;
+      const bool go = row != -2;
       const unsigned n = __popc(__ballot_sync(0xffffffffu, go));
       if (lane == 0) mbar_arrive_expect_tx(&bars->full[s], n * p.box * 2 * kRowBytes);
       if (go) {
         // a box that starts past the pool's last row reads as zeros
-        const int r = static_cast<int>(row[0] < 0 ? static_cast<long long>(p.n_pages) * p.Hkv * p.page_size
-                                                  : row[0]);
+        const int r = static_cast<int>(row < 0 ? static_cast<long long>(p.n_pages) * p.Hkv * p.page_size : row);
         tma_load_rows(tm_k, &bars->full[s], dst + lane * p.box * kRowBytes, r, policy);
         tma_load_rows(tm_v, &bars->full[s], dst + kTileBytes + lane * p.box * kRowBytes, r, policy);
       }
     } else {
       const int piece = lane & 7;
-#pragma unroll 4
-      for (int i = 0; i < kTile / 4; ++i) {
-        const int r = 4 * i + (lane >> 3);
-        const long long src = __shfl_sync(0xffffffffu, i < kTile / 8 ? row[0] : row[1], r & 31);
-        if (src == -2) continue;
+#pragma unroll
+      for (int i = 0; i < kShare / 4; ++i) {
+        const long long src = __shfl_sync(0xffffffffu, row, 4 * i + (lane >> 3));
+        const int r = row0 + 4 * i + (lane >> 3);
         const size_t off = static_cast<size_t>(src < 0 ? 0 : src) * kD + piece * 8;
         const uint32_t to = smem_u32(dst) + r * kRowBytes + ((piece ^ (r & 7)) << 4);
-        cp_async16(to, p.k + off, src >= 0);
-        cp_async16(to + kTileBytes, p.v + off, src >= 0);
+        if (src != -2) {
+          cp_async16(to, p.k + off, src >= 0);
+          cp_async16(to + kTileBytes, p.v + off, src >= 0);
+        }
       }
       cp_async_arrive(&bars->full[s]);
     }
@@ -358,9 +371,10 @@ __device__ __forceinline__ void produce(const Params& p, const CUtensorMap* tm_k
 }
 
 template <int kRows, bool kOutF32, bool kTma>
-__global__ void __launch_bounds__(kThreads, kRows == 8 ? 3 : 2)
+__global__ void __launch_bounds__(Shape<kRows, kTma>::kThreads, Shape<kRows, kTma>::kCtas)
     paged_decode_kernel(const Params p, const __grid_constant__ CUtensorMap tm_k,
                         const __grid_constant__ CUtensorMap tm_v) {
+  constexpr int kStages = Shape<kRows, kTma>::kStages, kProducers = Shape<kRows, kTma>::kProducers;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Bars bars;
   __shared__ float sm_m[kWarps][kRows], sm_l[kWarps][kRows];
@@ -373,7 +387,7 @@ __global__ void __launch_bounds__(kThreads, kRows == 8 ? 3 : 2)
   const int heads = p.Hkv * p.parts;
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(&bars.full[s], kTma ? 1 : 32);
+      mbar_init(&bars.full[s], kTma ? 1 : 32 * kProducers);
       mbar_init(&bars.empty[s], kWarps);
     }
     bars.abort_flag = 0;
@@ -391,12 +405,12 @@ __global__ void __launch_bounds__(kThreads, kRows == 8 ? 3 : 2)
   const Plan plan = make_plan(p, heads, c);
   const long long lo = plan.lo, hi = plan.hi;   // lo: the range's first tile
   if (lo >= hi) return;
-  if (warp == kWarps) {
+  if (warp >= kWarps) {
     if constexpr (kTma) {
       // rows written by earlier kernels' ordinary stores, read by bulk copies
       asm volatile("fence.proxy.async.global;" ::: "memory");
     }
-    produce<kTma>(p, &tm_k, &tm_v, heads, c, lo, hi, ring, &bars);
+    produce<kTma, kStages, kProducers>(p, &tm_k, &tm_v, heads, c, lo, hi, ring, &bars);
     return;
   }
 
@@ -808,11 +822,12 @@ template <int kRows, bool kOutF32, bool kTma>
 cudaError_t launch_typed(cudaStream_t stream, const Params& p, long long max_tiles,
                          const CUtensorMap& tk, const CUtensorMap& tv) {
   auto kern = paged_decode_kernel<kRows, kOutF32, kTma>;
-  constexpr int smem = kStages * kStageBytes + 1024;   // + alignment
+  using S = Shape<kRows, kTma>;
+  constexpr int smem = S::kStages * kStageBytes + 1024;   // + alignment
   static SmemOptIn opt_in;
   const cudaError_t e = allow_smem(kern, smem, opt_in);
   if (e != cudaSuccess) return e;
-  long long grid = static_cast<long long>(current_sm_count()) * (kRows == 8 ? 3 : 2);
+  long long grid = static_cast<long long>(current_sm_count()) * S::kCtas;
   if (grid > kMaxCtas) grid = kMaxCtas;
   if (grid > max_tiles) grid = max_tiles;
   // Placed early, before the kernel before it has ended, a call starts 0.3 us
@@ -820,9 +835,9 @@ cudaError_t launch_typed(cudaStream_t stream, const Params& p, long long max_til
   // early blocks of the next call stand in the way of this call's second kernel
   // (62.0 -> 67.0 us a call for 8 sequences of 32768 keys).
   if (p.scores == nullptr)
-    return launch_dependent(kern, dim3(static_cast<unsigned>(grid)), dim3(kThreads), smem, stream, 1, p,
+    return launch_dependent(kern, dim3(static_cast<unsigned>(grid)), dim3(S::kThreads), smem, stream, 1, p,
                             tk, tv);
-  return launch_ex(kern, dim3(static_cast<unsigned>(grid)), dim3(kThreads), smem, stream, 1, true, p,
+  return launch_ex(kern, dim3(static_cast<unsigned>(grid)), dim3(S::kThreads), smem, stream, 1, true, p,
                    tk, tv);
 }
 
@@ -880,10 +895,11 @@ cudaError_t launch_paged_decode(cudaStream_t stream, const PagedDecode& a, int* 
   p.scores_ld = scores_ld(cap);
   const long long per_head = cap > 0 ? (cap + kTile - 1) / kTile : 1;
   const long long max_tiles = static_cast<long long>(a.B) * p.Hkv * p.parts * per_head;
-  // TMA boxes need whole groups of 16 rows in a page and row numbers in 31 bits
+  // TMA boxes: a page holds whole boxes, row numbers fit 31 bits
   const long long pool_rows = static_cast<long long>(p.n_pages) * p.Hkv * p.page_size;
-  const bool tma = p.page_size % kKeysPerWarp == 0 && pool_rows < (1LL << 31);
-  p.box = p.page_size % 64 == 0 ? 64 : p.page_size % 32 == 0 ? 32 : 16;
+  const bool tma = p.page_size % kMinBox == 0 && pool_rows < (1LL << 31);
+  p.box = kTile;
+  while (p.page_size % p.box != 0) p.box /= 2;
   CUtensorMap tk = {}, tv = {};
   cudaError_t e = cudaSuccess;
   if (tma) {
