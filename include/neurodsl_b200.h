@@ -499,7 +499,10 @@ int nd_window_attn_fwd(void *stream, const void *Q, const int64_t *q_strides, co
  * takes no write; it, and a length that is negative or past the table (cut to
  * fit, and nothing appended), set the device error word to 16
  * (nd_device_error).  D must be 64; H a multiple of Hkv; page_size >= 1,
- * max_pages * page_size < 2^30.
+ * max_pages * page_size < 2^30; at most 65535 (sequence, head) pairs a call.
+ * These kernels and nd_logits_penalty may be placed while the kernel before
+ * them still runs, whatever nd_set_pdl says; they read nothing before it has
+ * ended.
  */
 
 /* Scratch bytes of nd_paged_decode_attn for at most max_len = max_pages *
@@ -576,7 +579,8 @@ int nd_paged_kv_evict(void *stream, void *k_pages, void *v_pages, int n_pages, i
  *   x = -inf where the mask's bit is 0
  * each operation rounded to fp32, out [rows][V] in out_dtype.
  *   logits [rows][V] in dtype, row stride ld; out may be logits (same dtype
- *   and stride), and may otherwise not overlap it.
+ *   and stride), or other columns of the same rows, and may not overlap it
+ *   otherwise.
  *   history [rows][history_ld] int32 or NULL: n_history entries a row, the
  *   first history_lens[row] of them used (NULL: all), negative ones skipped.
  *   repetition (> 0), presence, frequency [rows] fp32 or NULL (left out).

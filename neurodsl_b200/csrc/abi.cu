@@ -308,6 +308,12 @@ int flash_attn_common(const char* fn, void* stream, const void* Q, const void* K
                       void* O, int o_dtype, float* lse, float* row_max, int B, int H, int Sq,
                       int Sk, int D, float scale, int causal, nd::FlashStrides st, int Hkv,
                       const FlashMask* mask = nullptr) {
+  if (mask != nullptr) {   // a single row's stride is never applied either
+    if (Sq == 1) st.q[0] = H > 1 ? st.q[1] : 64;
+    if (Sq == 1) st.o[0] = H > 1 ? st.o[1] : 64;
+    if (Sk == 1) st.k[0] = Hkv > 1 ? st.k[1] : 64;
+    if (Sk == 1) st.v[0] = Hkv > 1 ? st.v[1] : 64;
+  }
   normalize_unit_strides(st.q, Sq, H, B);
   normalize_unit_strides(st.o, Sq, H, B);
   normalize_unit_strides(st.k, Sk, Hkv, B);
@@ -1268,7 +1274,7 @@ __attribute__((visibility("default"))) int nd_paged_kv_store(
   int rc = check_pool(fn, k_pages, v_pages, n_pages, page_size, table, table_ld, max_pages, B, Hkv,
                       D, empty);
   if (rc) return rc;
-  if (pos0_dev == nullptr && lens == nullptr &&
+  if (!empty && pos0_dev == nullptr && lens == nullptr &&
       static_cast<long long>(pos0) + S > static_cast<long long>(max_pages) * page_size)
     return fail(ND_ERR_SHAPE, "%s: pos0 %d + S %d exceeds max_pages * page_size", fn, pos0, S);
   if (ld % 8 || k_col % 8 || v_col % 8 || k_col < 0 || v_col < 0 ||
@@ -1378,9 +1384,16 @@ __attribute__((visibility("default"))) int nd_logits_penalty(
   } else {
     const char* x = static_cast<const char*>(logits);
     const char* y = static_cast<const char*>(out);
-    const long long xn = ((rows - 1) * static_cast<long long>(ld) + V) * (dtype == ND_F32 ? 4 : 2);
-    const long long yn = ((rows - 1) * static_cast<long long>(out_ld) + V) * (out_dtype == ND_F32 ? 4 : 2);
-    if (x < y + yn && y < x + xn) return fail(ND_ERR_INVALID_ARG, "%s: out overlaps logits", fn);
+    const long long xs = dtype == ND_F32 ? 4 : 2, ys = out_dtype == ND_F32 ? 4 : 2;
+    const long long xn = ((rows - 1) * static_cast<long long>(ld) + V) * xs;
+    const long long yn = ((rows - 1) * static_cast<long long>(out_ld) + V) * ys;
+    if (x < y + yn && y < x + xn) {
+      // rows side by side in rows of one buffer do not meet
+      const long long pitch = ld * xs;
+      const long long d = ((y - x) % pitch + pitch) % pitch;   // out's first byte in a row of logits
+      if (pitch != out_ld * ys || d < V * xs || d + V * ys > pitch)
+        return fail(ND_ERR_INVALID_ARG, "%s: out overlaps logits", fn);
+    }
   }
   const uintptr_t in_size = dtype == ND_F32 ? 4 : 2, out_size = out_dtype == ND_F32 ? 4 : 2;
   if (reinterpret_cast<uintptr_t>(logits) % in_size || reinterpret_cast<uintptr_t>(out) % out_size)

@@ -1096,8 +1096,9 @@ cudaError_t launch_window_fwd(cudaStream_t stream, const __nv_bfloat16* Q, const
   win.sinks = sinks < Sk ? sinks : Sk;
   win.group = H / Hkv;
   win.off = Sk - Sq;
-  // fewer items of two query tiles than SMs: items of one
-  win.solo = static_cast<long long>(ceil_div(Sq, kRowsPerCta)) * BH < limited_sms(current_sm_count());
+  // fewer items of two query tiles than the device has SMs: items of one (the
+  // thread's SM limit does not enter, so that results do not depend on it)
+  win.solo = static_cast<long long>(ceil_div(Sq, kRowsPerCta)) * BH < current_sm_count();
   const float sl2 = scale * kLog2e;
 #define ND_WINDOW_LAUNCH(F, S_)                                                                   \
   launch_typed<true, F, S_, true>(stream, tq, tk, tv, to, lay, lse, row_max, BH, Sq, Sk, sl2, win)

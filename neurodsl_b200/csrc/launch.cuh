@@ -21,7 +21,7 @@
 
 #include <cuda_runtime.h>
 
-#include <atomic>
+#include <mutex>
 #include <utility>
 
 namespace nd {
@@ -92,11 +92,13 @@ cudaError_t launch_dependent(void (*kernel)(KArgs...), dim3 grid, dim3 block, si
   return e;
 }
 
-// Allow `kernel` up to `bytes` of dynamic shared memory, once per device and
-// growth: `state` (static in the caller, zero at first) holds what each device
-// has been told.
+// Allow `kernel` up to `bytes` of dynamic shared memory: told to the runtime once
+// per device, context and growth.  `state` is static in the caller.
+unsigned long long current_context_id();
 struct SmemOptIn {
-  std::atomic<int> bytes[64];
+  std::mutex mu;
+  int bytes[64] = {};
+  unsigned long long context[64] = {};
 };
 template <typename... KArgs>
 cudaError_t allow_smem(void (*kernel)(KArgs...), int bytes, SmemOptIn& state) {
@@ -104,11 +106,13 @@ cudaError_t allow_smem(void (*kernel)(KArgs...), int bytes, SmemOptIn& state) {
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  if (state.bytes[dev].load(std::memory_order_acquire) >= bytes) return cudaSuccess;
+  const unsigned long long ctx = current_context_id();
+  std::lock_guard<std::mutex> lk(state.mu);
+  if (state.context[dev] == ctx && state.bytes[dev] >= bytes) return cudaSuccess;
   e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e == cudaSuccess) {
-    int had = state.bytes[dev].load(std::memory_order_relaxed);
-    while (had < bytes && !state.bytes[dev].compare_exchange_weak(had, bytes, std::memory_order_release)) {}
+    state.context[dev] = ctx;
+    state.bytes[dev] = bytes;
   }
   return e;
 }

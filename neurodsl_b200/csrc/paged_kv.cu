@@ -4,6 +4,10 @@
 // Both move rows of 128 bytes (64 bf16) and are bound by HBM: the store reads
 // and writes every token's K and V row once, the eviction reads 4 bytes of
 // weight per position and moves the kept rows once.
+//
+// The kernels that write the cache do not let the next kernel start early: the
+// contiguous decode attention, with programmatic launch on, reads cached rows
+// before it waits.
 #include <cuda_bf16.h>
 #include <stdint.h>
 
@@ -46,7 +50,6 @@ __global__ void __launch_bounds__(256)
                        const int* __restrict__ pos0_dev, const int* __restrict__ lens,
                        int* __restrict__ err_word) {
   pdl_wait();
-  pdl_trigger();
   const int lane = threadIdx.x & 31;
   const long long w = static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
   const int per_seq = (S + kTokens - 1) / kTokens, chunks = (pool.Hkv * kVec + 31) / 32;
@@ -286,7 +289,6 @@ __global__ void __launch_bounds__(kThreads, kThreads < 1024 ? 2 : 1)
 __global__ void __launch_bounds__(256)
     paged_gather_kernel(const PagedEvict a, int* __restrict__ err_word) {
   pdl_wait();
-  pdl_trigger();
   const int lane = threadIdx.x & 31;
   const int per_head = (a.budget + 31) / 32;
   const long long w = static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);

@@ -569,6 +569,7 @@ def add_layernorm(x, p, bias=None, gamma=None, beta=None, eps=1e-5, s_out=None, 
 # cost little: plain attribute reads, one device number for all tensors.
 _BF16, _F32, _INT32 = torch.bfloat16, torch.float32, torch.int32
 _I64x3 = ctypes.c_int64 * 3
+_INT_MAX = 2**31 - 1
 _cuda_device = torch._C._cuda_getDevice          # the current device's number
 _raw_stream = torch._C._cuda_getCurrentRawStream  # a device's current stream as an int
 
@@ -685,7 +686,7 @@ def window_attn_fwd(Q, K, V, window, sinks=0, scale=None, out=None, out_dtype=to
           _strides4(Q, "Q"), K.data_ptr(), _strides4(K, "K"), V.data_ptr(), _strides4(V, "V"),
           out.data_ptr(), _strides4(out, "out"), _DT[out.dtype], lse.data_ptr(),
           row_max.data_ptr(), B, H, Hkv, Sq, Sk, D, 1.0 / math.sqrt(D) if scale is None else scale,
-          window, sinks)
+          min(window, _INT_MAX), min(sinks, _INT_MAX))
     return out, lse, row_max
 
 
@@ -768,7 +769,8 @@ def paged_decode_attn(q, k_pages, v_pages, block_table, lens, k_new=None, v_new=
     _call(_lib.load().nd_paged_decode_attn, dev, _stream_of(dev, stream), q.data_ptr(),
           _addr(k_new), _addr(v_new), k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page_size,
           block_table.data_ptr(), table_ld, max_pages, lens.data_ptr(), out.data_ptr(),
-          _DT[out.dtype], _addr(lse), _addr(weights), weights_ld, B, H, Hkv, D, window, sinks,
+          _DT[out.dtype], _addr(lse), _addr(weights), weights_ld, B, H, Hkv, D,
+          min(window, _INT_MAX), min(sinks, _INT_MAX),
           1.0 / math.sqrt(D) if scale is None else scale, workspace.data_ptr(), workspace.nbytes)
     return out, lse
 

@@ -239,3 +239,19 @@ def test_refusals():
     with pytest.raises(RuntimeError):
         big = torch.zeros(200, device=DEV)
         ops.logits_penalty(big[:100].view(2, 50), out=big[50:150].view(2, 50))
+
+
+def test_out_beside_logits_in_one_buffer():
+    ops = _ops()
+    buf = torch.randn(4, 2000, device=DEV)
+    x = buf[:, :1000].clone()
+    out, idx = ops.logits_penalty(buf[:, :1000], out=buf[:, 1000:])
+    assert torch.equal(out, x) and torch.equal(buf[:, :1000], x) and torch.equal(idx.long(), x.argmax(1))
+    with pytest.raises(RuntimeError):
+        ops.logits_penalty(buf[:, :1000], out=buf[:, 999:1999])
+
+
+@pytest.mark.parametrize("n_hist, n_bias, V", [(9000, 0, 30000), (20000, 300, 9001), (7000, 7000, 70000), (1, 0, 300000)])
+def test_long_lists(n_hist, n_bias, V):
+    """Lists longer than the largest table, vocabularies longer than a bit map."""
+    run(2, V, n_hist, n_bias, True, seed=n_hist, lens=True)

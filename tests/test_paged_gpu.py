@@ -560,3 +560,62 @@ def test_evict_refusals():
                dict(new_lens=torch.zeros(3, dtype=torch.int32, device=DEV)), dict(w=w.view(1, 2, -1))):
         with pytest.raises(ValueError):
             call(**kw)
+
+
+def test_empty_tables_and_batches():
+    """No pages at all: every sequence is empty; no sequences: nothing to do."""
+    ops = _ops()
+    kp = torch.zeros((1, 2, 16, D), dtype=torch.bfloat16, device=DEV)
+    q = _randn(_gen(1), 3, 4, D)
+    table = torch.empty((3, 0), dtype=torch.int32, device=DEV)
+    lens = torch.zeros(3, dtype=torch.int32, device=DEV)
+    w = torch.ones((3, 2, 5), device=DEV)
+    out, lse = ops.paged_decode_attn(q, kp, kp, table, lens, weights=w)
+    assert (out == 0).all() and (lse == -math.inf).all() and (w == 1).all()
+    out, lse = ops.paged_decode_attn(q[:0], kp, kp, table[:0], lens[:0])
+    assert out.shape == (0, 4, D)
+    ops.paged_kv_store(_randn(_gen(1), 0, 4 * D), 0, 2 * D, kp, kp, table[:0], 0, 7)
+    assert ops.device_error() == 0
+
+
+def test_window_past_31_bits_is_no_window():
+    c = Cache([300, 20], 2, 16)
+    run_decode(c, 4, window=2**40, sinks=2**40)
+
+
+@pytest.mark.parametrize("page", [4, 8, 12, 20, 32, 48, 256])
+def test_more_page_sizes(page):
+    run_decode(Cache([1, 700, 64, 333], 2, page), 24, append=True, window=200, sinks=9, with_weights=True)
+
+
+def test_tables_wider_than_used():
+    """Tables and weights in longer rows, as views."""
+    c = Cache([100, 40, 77], 2, 16)
+    wide = torch.full((3, 20), 10**6, dtype=torch.int32, device=DEV)
+    wide[:, 2:2 + c.max_pages] = c.table
+    c.table = wide[:, 2:2 + c.max_pages]
+    run_decode(c, 4, append=True, with_weights=True)
+
+
+def test_store_then_contiguous_decode_with_programmatic_launch():
+    """The contiguous decode attention reads cached rows before it waits for the
+    kernel before it; a store right in front of it has to have ended by then."""
+    ops = _ops()
+    g = _gen(5)
+    B, H, L_max, S = 8, 12, 2048, 2000
+    kc = torch.zeros((B, H, L_max, D), dtype=torch.bfloat16, device=DEV)
+    vc = torch.zeros_like(kc)
+    table = torch.arange(B, dtype=torch.int32, device=DEV)[:, None].contiguous()
+    src = _randn(g, B * S, 2 * H * D)
+    q = _randn(g, B, H, D)
+    want = None
+    for _ in range(5):
+        kc.zero_()
+        vc.zero_()
+        with ops.pdl(True):
+            ops.paged_kv_store(src, 0, H * D, kc, vc, table, B, S)
+            out, lse = ops.kv_decode_attn(q, kc, vc, S)
+        if want is None:
+            torch.cuda.synchronize()
+            want = ops.kv_decode_attn(q, kc, vc, S)
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1])

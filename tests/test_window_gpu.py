@@ -188,3 +188,41 @@ def test_refusals():
             ops.window_attn_fwd(Q, K, V, **kw)
     with pytest.raises(RuntimeError):
         ops.window_attn_fwd(K, Q[:, :2], Q[:, :2], 4)       # more queries than keys
+
+
+@pytest.mark.parametrize("B, H, Hkv, Sq, Sk, window, sinks", [
+    (2, 70, 35, 256, 300, 33, 2),      # two one-tile items for some SMs, streams of 1 to 3 tiles
+    (1, 146, 73, 250, 640, 250, 1),
+    (1, 3, 1, 384, 384, 384, 0),
+    (4, 8, 8, 128, 128, 128, 0),       # a stream of one tile, shared by two groups
+    (1, 2, 2, 1, 128, 128, 0),         # its last position alone: nothing to mask but the copy
+    (1, 2, 2, 1, 129, 1, 0),
+])
+def test_one_tile_items(B, H, Hkv, Sq, Sk, window, sinks):
+    Q, K, V, out = make("cache", B, H, Hkv, Sq, Sk, seed=Sk)
+    got = _ops().window_attn_fwd(Q, K, V, window, sinks=sinks, out=out)
+    compare(got, reference(Q, K, V, window, sinks, 0.125), torch.bfloat16, Sk)
+
+
+def test_results_do_not_depend_on_the_sm_limit():
+    ops = _ops()
+    for shape in ((1, 8, 4, 300, 500), (2, 100, 50, 300, 300)):
+        Q, K, V, _ = make("head", *shape, seed=7)
+        want = ops.window_attn_fwd(Q, K, V, 70, sinks=4)
+        with ops.sm_limit(5):
+            got = ops.window_attn_fwd(Q, K, V, 70, sinks=4)
+        for x, y in zip(got, want):
+            assert torch.equal(x, y)
+
+
+def test_single_rows_of_any_stride():
+    """The stride of a dimension of one row is never applied."""
+    ops = _ops()
+    Q, K, V, _ = make("head", 2, 4, 2, 1, 90, seed=8)
+    want = ops.window_attn_fwd(Q, K, V, 40, sinks=1)
+    odd = Q.as_strided(Q.shape, (4 * D, D, 3, 1))
+    got = ops.window_attn_fwd(odd, K, V, 40, sinks=1)
+    assert torch.equal(got[0], want[0])
+    q, k, v, _ = make("head", 1, 2, 2, 1, 1, seed=9)
+    got = ops.window_attn_fwd(q, k.as_strided(k.shape, (2 * D, D, 1, 1)), v, 2**40, sinks=2**40)
+    compare(got, reference(q, k, v, 1, 0, 0.125), torch.bfloat16, 1)
