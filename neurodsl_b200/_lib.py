@@ -115,6 +115,7 @@ class NeuroDSLError(RuntimeError):
 
 
 _lib = None
+calls = None  # the extension that load_calls() found; False: none
 _lock = threading.Lock()
 
 
@@ -136,6 +137,25 @@ def load(path: str = LIB_PATH):
                 fn.argtypes = args
             _lib = lib
     return _lib
+
+
+def load_calls():
+    """The extension that makes the serving operators' calls (csrc/py_calls.cpp)
+    bound to the library's entry points.  False where it was not built or this
+    interpreter's torch cannot load it: the same entry points are then called
+    through ctypes."""
+    global calls
+    lib = load()
+    try:
+        from . import _calls
+    except ImportError:
+        calls = False
+    else:
+        _calls.bind(*(ctypes.cast(fn, _vp).value for fn in (
+            lib.nd_window_attn_fwd, lib.nd_paged_decode_attn, lib.nd_paged_kv_store,
+            lib.nd_paged_kv_evict, lib.nd_logits_penalty)))
+        calls = _calls
+    return calls
 
 
 def check(status: int):

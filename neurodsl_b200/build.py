@@ -21,6 +21,7 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libneurodsl_b200.so")
+CALLS = os.path.join(PKG, "_calls.so")
 SOURCES = ["abi.cu", "tma.cu", "flash_fwd.cu", "kv_decode.cu", "gemm.cu", "layernorm.cu", "model_ops.cu",
            "tp_comm.cu", "elementwise.cu", "paged_decode.cu", "paged_kv.cu", "logits.cu"]
 
@@ -86,12 +87,38 @@ def build(force: bool = False, verbose: bool = False, extra_flags=None) -> str:
     return LIB
 
 
+def build_calls(force: bool = False) -> str:
+    """neurodsl_b200/_calls.so: the CPython extension that makes the serving
+    operators' calls (csrc/py_calls.cpp), against this interpreter and its torch."""
+    src = os.path.join(CSRC, "py_calls.cpp")
+    if not force and not _stale(CALLS, [src, os.path.join(ROOT, "include", "neurodsl_b200.h")]):
+        return CALLS
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths
+    cuda = os.path.dirname(os.path.dirname(nvcc()))
+    libs = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I", os.path.join(ROOT, "include"), "-isystem", sysconfig.get_paths()["include"],
+           "-isystem", os.path.join(cuda, "include")]
+    for d in include_paths():
+        cmd += ["-isystem", d]
+    cmd += [src, "-o", CALLS, "-L", libs, "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("building _calls.so failed:\n" + r.stdout + r.stderr)
+    return CALLS
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--force", action="store_true")
     ap.add_argument("--verbose", action="store_true")
     a = ap.parse_args()
     print(build(force=a.force, verbose=a.verbose))
+    print(build_calls(force=a.force))
 
 
 if __name__ == "__main__":

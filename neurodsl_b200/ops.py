@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import operator
 
 import torch
 
@@ -642,6 +643,26 @@ def _call(fn, dev, *args):
         check(rc)
 
 
+def _quick(name, *args):
+    """The call as the extension makes it (csrc/py_calls.cpp), where its
+    arguments are the common kind; whether it was made.  Otherwise the caller's
+    own checks follow, which refuse the call or carry it out."""
+    calls = _lib.calls
+    if calls is None:
+        calls = _lib.load_calls()
+    rc = getattr(calls, name)(*args) if calls else None
+    if rc:
+        check(rc)
+    return rc is not None
+
+
+def _int(v):
+    """v as a C int that is refused, or unlimited, just as v would be (the
+    foreign-function call would drop the high bits)."""
+    v = operator.index(v)
+    return v if -_INT_MAX <= v <= _INT_MAX else (_INT_MAX if v > 0 else -1)
+
+
 def _addr(t):
     return None if t is None else t.data_ptr()
 
@@ -663,6 +684,9 @@ def window_attn_fwd(Q, K, V, window, sinks=0, scale=None, out=None, out_dtype=to
 
     Returns (O, lse, row_max) like flash_attn_fwd, and like there Q, K, V and
     `out` may be strided views (a fused projection, a longer cache)."""
+    if out is not None and stream is None and _quick(
+            "window_attn_fwd", Q, K, V, window, sinks, scale, out, lse, row_max):
+        return out, lse, row_max
     dev = _device_of(Q, "Q")
     _tensor(Q, "Q", _BF16, 4, dev, False)
     _tensor(K, "K", _BF16, 4, dev, False)
@@ -686,7 +710,7 @@ def window_attn_fwd(Q, K, V, window, sinks=0, scale=None, out=None, out_dtype=to
           _strides4(Q, "Q"), K.data_ptr(), _strides4(K, "K"), V.data_ptr(), _strides4(V, "V"),
           out.data_ptr(), _strides4(out, "out"), _DT[out.dtype], lse.data_ptr(),
           row_max.data_ptr(), B, H, Hkv, Sq, Sk, D, 1.0 / math.sqrt(D) if scale is None else scale,
-          min(window, _INT_MAX), min(sinks, _INT_MAX))
+          _int(window), _int(sinks))
     return out, lse, row_max
 
 
@@ -729,6 +753,10 @@ def paged_decode_attn(q, k_pages, v_pages, block_table, lens, k_new=None, v_new=
     attention weight, summed over its group's query heads.  workspace: from
     paged_decode_workspace, kept by the caller from call to call; without one
     each call makes its own.  Returns (out [B][H][64], lse [B][H] or None)."""
+    if (out is not None and stream is None and (lse is not None or not want_lse) and _quick(
+            "paged_decode_attn", q, k_pages, v_pages, block_table, lens, k_new, v_new, window, sinks,
+            scale, out, lse, weights, workspace)):
+        return out, lse
     dev = _device_of(q, "q")
     _tensor(q, "q", _BF16, 3, dev)
     B, H, D = q_shape = q.shape
@@ -770,7 +798,7 @@ def paged_decode_attn(q, k_pages, v_pages, block_table, lens, k_new=None, v_new=
           _addr(k_new), _addr(v_new), k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page_size,
           block_table.data_ptr(), table_ld, max_pages, lens.data_ptr(), out.data_ptr(),
           _DT[out.dtype], _addr(lse), _addr(weights), weights_ld, B, H, Hkv, D,
-          min(window, _INT_MAX), min(sinks, _INT_MAX),
+          _int(window), _int(sinks),
           1.0 / math.sqrt(D) if scale is None else scale, workspace.data_ptr(), workspace.nbytes)
     return out, lse
 
@@ -781,6 +809,9 @@ def paged_kv_store(src, k_col, v_col, k_pages, v_pages, block_table, B, S, pos0=
     (nd_paged_kv_store): token (b, s) goes to position pos0 + s of sequence b.
     pos0: an int, or int32 [B] on the device; lens: int32 [B] tokens of each
     sequence, the rest being padding (None: all S)."""
+    if stream is None and _quick("paged_kv_store", src, k_col, v_col, k_pages, v_pages, block_table,
+                                 B, S, pos0, lens):
+        return
     dev = _device_of(src, "src")
     cols, ld = _matrix(src, "src", _BF16, B * S, dev)
     n_pages, Hkv, page_size, D = _pool(k_pages, v_pages, dev)
@@ -793,9 +824,10 @@ def paged_kv_store(src, k_col, v_col, k_pages, v_pages, block_table, B, S, pos0=
         _vector(lens, "lens", _INT32, B, dev)
     if max(k_col, v_col) + Hkv * D > cols:
         raise ValueError("k_col / v_col: the heads' columns do not fit src")
-    _call(_lib.load().nd_paged_kv_store, dev, _stream_of(dev, stream), src.data_ptr(), ld, k_col,
-          v_col, k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page_size,
-          block_table.data_ptr(), table_ld, max_pages, B, S, Hkv, pos0, pos_dev, _addr(lens), D)
+    _call(_lib.load().nd_paged_kv_store, dev, _stream_of(dev, stream), src.data_ptr(), ld,
+          _int(k_col), _int(v_col), k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page_size,
+          block_table.data_ptr(), table_ld, max_pages, B, S, Hkv, _int(pos0), pos_dev,
+          _addr(lens), D)
 
 
 def paged_kv_evict(k_pages, v_pages, block_table, lens, weights, out_table, budget, sinks=0,
@@ -809,6 +841,10 @@ def paged_kv_evict(k_pages, v_pages, block_table, lens, weights, out_table, budg
     Returns (kept [B][Hkv][budget] int32 positions, -1 past the last;
     new_lens [B]; weights_out [B][Hkv][keys], the kept keys' weights first,
     zeros behind them)."""
+    if kept is not None and stream is None and _quick(
+            "paged_kv_evict", k_pages, v_pages, block_table, lens, weights, out_table, budget, sinks,
+            recent, weights_out, kept, new_lens):
+        return kept, new_lens, weights_out
     dev = _device_of(k_pages, "k_pages")
     n_pages, Hkv, page_size, D = _pool(k_pages, v_pages, dev)
     _tensor(lens, "lens", _INT32, 1, dev)
@@ -831,7 +867,7 @@ def paged_kv_evict(k_pages, v_pages, block_table, lens, weights, out_table, budg
           v_pages.data_ptr(), n_pages, page_size, block_table.data_ptr(), table_ld, max_pages,
           lens.data_ptr(), weights.data_ptr(), weights.shape[2], out_table.data_ptr(), out_ld,
           out_pages, weights_out.data_ptr(), weights_out.shape[2], kept.data_ptr(),
-          new_lens.data_ptr(), B, Hkv, D, budget, sinks, recent)
+          new_lens.data_ptr(), B, Hkv, D, _int(budget), _int(sinks), _int(recent))
     return kept, new_lens, weights_out
 
 
@@ -847,6 +883,10 @@ def logits_penalty(logits, history=None, history_lens=None, repetition=None, pre
     [>= V/32] for all rows, bit v % 32 of word v / 32 allowing token v.  `out`
     may be `logits` itself.  Returns (out, idx int32 [rows], or None with
     greedy=False)."""
+    if out is not None and stream is None and (idx is not None or not greedy) and _quick(
+            "logits_penalty", logits, history, history_lens, repetition, presence, frequency,
+            bias_ids, bias, mask, out, idx):
+        return out, idx
     dev = _device_of(logits, "logits")
     rows = logits.shape[0]
     V, ld = _matrix(logits, "logits", None, rows, dev)

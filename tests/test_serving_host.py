@@ -175,3 +175,22 @@ def test_python_front_end_refuses_host_tensors():
         ops.paged_kv_evict(bf, bf, i32, i32[:, 0], torch.zeros(1, 1, 8), i32, 4)
     with pytest.raises(TypeError):
         ops.logits_penalty(torch.zeros(1, 10))
+
+
+def test_the_calls_extension_leaves_everything_uncommon_to_the_checks():
+    """It is built and loads; it answers None, never a status, to tensors that
+    are not on a GPU, to things that are no tensors and to a wrong count."""
+    torch = pytest.importorskip("torch")
+    lib, _ = _lib()
+    calls = lib.load_calls()
+    assert calls, "python -m neurodsl_b200.build makes it"
+    host = torch.zeros(2, 3)
+    for name, n in [("window_attn_fwd", 9), ("paged_decode_attn", 14), ("paged_kv_store", 10),
+                    ("paged_kv_evict", 12), ("logits_penalty", 11)]:
+        fn = getattr(calls, name)
+        for value in (None, host, "x", 3, 2**70, 1.5, object()):
+            assert fn(*[value] * n) is None
+            assert fn(host, *[value] * (n - 1)) is None
+        assert fn() is None and fn(*[host] * (n + 1)) is None
+    with pytest.raises(TypeError):
+        calls.bind(1, 2)
