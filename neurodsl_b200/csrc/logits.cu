@@ -14,18 +14,21 @@
 // Bound: HBM, one read and one write of the logits.  A row is one CTA's, or a
 // cluster's when there are few rows, each CTA taking a contiguous part of the
 // vocabulary.  A CTA first enters the listed tokens of its part (history and
-// biases) into a hash table in shared memory, with their counts, and marks them
-// in a bit map; then it streams its part without a barrier, some thousand tokens
-// a round, with the mask alone, and after each round every thread computes the
-// listed tokens it passed anew, while their lines are in the cache.  The rare
-// tokens so cost a few steps a round and not a divergent path a value, nor
-// scattered traffic to memory (all of them at the end: 46.8 us for 512 rows of
-// 50257 tokens with histories of 1024; with the penalties inside the stream and
-// a count for every token of a slice, the lists read once a slice: 161 us; now
-// 45.1).  Counts are integers, so the order of the atomics does not matter; biases
-// are summed by one warp in list order, their tokens computed last.  The CTAs'
-// best tokens meet in distributed shared memory, so the logits are not read
-// again for the argmax.
+// biases) into a hash table in shared memory, with their counts; the first to
+// enter a token takes it off the part's bit map of allowed tokens and sends for
+// its logit (an asynchronous copy that no one waits for).  Then the CTA streams its
+// part without a barrier, -inf for what the map lacks, and at the end computes and
+// writes the listed tokens.  So the stream, which runs at the copy rate (23 us for
+// 512 rows of 50257, bf16 to fp32), does not branch, and what precedes it is two
+// trips to memory.  Earlier forms: every penalty inside the stream and a count for
+// each token of a slice, the lists read once a slice, 161 us for those rows with
+// histories of 1024; listed tokens looked up and read again after each round of the
+// stream, 45.9; the logits of the listed tokens read at the end, 45.5; now 37.8 (44.0
+// where a history's tokens are all different, 46.6 before).  The rest over the
+// stream's time: the lists 6 us, the listed tokens' writing 4, four rows on some SMs
+// and three on others.  Counts are integers, so the order of the atomics does not
+// matter; biases are summed by one warp in list order.  The CTAs' best tokens meet
+// in distributed shared memory, so the logits are not read again for the argmax.
 #include <cuda_bf16.h>
 #include <stdint.h>
 
@@ -41,10 +44,11 @@ namespace nd {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxPart = 1 << 18;               // tokens of a bit map
+constexpr int kMaxPart = 1 << 18;               // tokens of the bit map
 constexpr int kCluster = 8;                     // CTAs of a row, at most
-constexpr int kMaxTable = 8192;                 // table entries, a power of two
-constexpr int kBiased = 1 << 31;                // flag beside a token's count
+constexpr int kMaxTable = 8192;                 // table entries
+constexpr int kBiased = 1 << 31;                // flag beside a token in the table
+constexpr int kForbidden = -0x7fffffff - 1;     // taken off a forbidden token's count
 constexpr int kNone = 0x7fffffff;
 
 template <typename T>
@@ -55,6 +59,15 @@ template <typename T>
 __device__ __forceinline__ T rounded(float x) {
   if constexpr (sizeof(T) == 4) return x;
   else return __float2bfloat16_rn(x);
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+__device__ __forceinline__ float warp_max(float x) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+  return x;
 }
 // kN values as they lie in memory (8 or 16 bytes).
 template <typename T, int kN>
@@ -95,19 +108,22 @@ struct Piece {
 // loads and stores each cover contiguous bytes.  kVec: a row's input and output
 // have the same place within a group, so that groups aligned in one are aligned
 // in the other (the launcher checks); else token by token.
-// `table` entries of shared memory, a power of two, for the listed tokens, and
-// bit maps of `part` tokens (a multiple of 32), which a CTA takes at a time.
+// In shared memory `table` entries (a multiple of four) for the listed tokens,
+// n_sums for those with a bias, and a bit map of `part` tokens (a multiple of 32),
+// which a CTA takes at a time.
 template <typename TI, typename TO, bool kVec>
 __global__ void __launch_bounds__(kThreads, 4)
-    logits_penalty_kernel(const LogitsPenalty a, int table, int part, int* __restrict__ err_word) {
+    logits_penalty_kernel(const LogitsPenalty a, int table, int n_sums, int part, int* __restrict__ err_word) {
   constexpr int kN = sizeof(TI) + sizeof(TO) == 4 ? 8 : 4;   // 8: both bf16
-  constexpr int kUnroll = sizeof(TI) == 4 || kN == 8 ? 4 : 8;   // groups in flight a thread
-  constexpr uint32_t kMaskN = (1u << kN) - 1u;
+  // groups in flight a thread: four of fp32 in and out would spill
+  constexpr int kUnroll = sizeof(TI) + sizeof(TO) == 8 ? 3 : 4;
   extern __shared__ __align__(16) uint8_t smem_raw[];
-  int* key = reinterpret_cast<int*>(smem_raw);                  // token, -1: free
-  int* count = key + table;                                     // and the flag kBiased
-  float* bias = reinterpret_cast<float*>(count + table);
-  uint2* bits = reinterpret_cast<uint2*>(bias + table);         // x: allowed, y: listed
+  int* key = reinterpret_cast<int*>(smem_raw);                  // token and the flag kBiased, -1: free
+  int* count = key + table;                                     // below zero: the mask forbids it
+  uint32_t* value = reinterpret_cast<uint32_t*>(count + table); // the word of the token's logit
+  int* bias_key = reinterpret_cast<int*>(value + table);        // the biased tokens once more, with
+  float* bias = reinterpret_cast<float*>(bias_key + n_sums);    // the sums of their biases
+  uint32_t* bits = reinterpret_cast<uint32_t*>(bias + n_sums);  // tokens that the stream keeps
   __shared__ float best_v[kThreads / 32], cta_v;
   __shared__ int best_i[kThreads / 32], cta_i;
   const int nc = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
@@ -121,281 +137,274 @@ __global__ void __launch_bounds__(kThreads, 4)
   const int first = head > 0 ? -1 : 0;
   const int n_groups = (a.V - head + kN - 1) / kN - first;
   const int per = (n_groups + nc - 1) / nc;
-  const int g_end = first + min(n_groups, (rank + 1) * per);
-  const bool lists = a.history != nullptr || a.bias_ids != nullptr;
+  const int g_begin = first + rank * per, g_end = first + min(n_groups, (rank + 1) * per);
+  const bool lists = table > 0;
+  const int* hist = a.history ? a.history + row * a.history_ld : nullptr;
+  const int* ids = a.bias_ids ? a.bias_ids + static_cast<long long>(row) * a.n_bias : nullptr;
+  const int n_bias = ids ? a.n_bias : 0;
+  const uint32_t* words = a.mask ? a.mask + row * a.mask_ld : nullptr;
+  const int n_words = (a.V + 31) >> 5;
+  auto clear_tables = [&]() {
+    for (int i = threadIdx.x; i < table / 4; i += kThreads) {
+      reinterpret_cast<int4*>(key)[i] = make_int4(-1, -1, -1, -1);
+      reinterpret_cast<int4*>(count)[i] = make_int4(0, 0, 0, 0);
+    }
+    for (int i = threadIdx.x; i < n_sums; i += kThreads) {
+      bias_key[i] = -1;
+      bias[i] = 0.f;
+    }
+  };
+  clear_tables();
   pdl_wait();
   pdl_trigger();
 
-  const int* hist = nullptr;
-  const int* ids = nullptr;
+  // The lists' first entries and the mask before everything else: they are what
+  // the stream waits for.  The rows of the history are read whole; its length
+  // says which entries count.
+  auto read = [&](const int* list, int n, int i, int (&t)[4]) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) t[u] = i + u * kThreads < n ? list[i + u * kThreads] : -1;
+  };
+  int th[4], tb[4];
+  read(hist, hist ? a.n_history : 0, threadIdx.x, th);
+  read(ids, n_bias, threadIdx.x, tb);
+  int n_hist = hist ? a.n_history : 0;
+  if (hist && a.history_lens) n_hist = a.history_lens[row];
   float rep = 1.f, pres = 0.f, freq = 0.f;
-  int n_hist = 0, n_bias = 0;
-  if (a.history != nullptr) {
-    hist = a.history + row * a.history_ld;
-    if (a.repetition) rep = a.repetition[row];
-    if (a.presence) pres = a.presence[row];
-    if (a.frequency) freq = a.frequency[row];
-    n_hist = a.history_lens ? a.history_lens[row] : a.n_history;
-    if (n_hist < 0 || n_hist > a.n_history) {
-      if (threadIdx.x == 0 && err_word) atomicCAS(err_word, 0, kModelErrIndex);
-      n_hist = n_hist < 0 ? 0 : a.n_history;
-    }
-  }
-  if (a.bias_ids != nullptr) {
-    ids = a.bias_ids + static_cast<long long>(row) * a.n_bias;
-    n_bias = a.n_bias;
-  }
-  const uint32_t* words = a.mask ? a.mask + row * a.mask_ld : nullptr;
-  const int n_words = (a.V + 31) >> 5;
+  if (a.repetition) rep = a.repetition[row];
+  if (a.presence) pres = a.presence[row];
+  if (a.frequency) freq = a.frequency[row];
 
   float bv = -INFINITY;
   int bi = kNone;
-  auto slot_of = [&](int t) { return (static_cast<uint32_t>(t) * 2654435761u) >> 19 & (table - 1); };
-  // Token t, entry s of the table, anew from its logit.  (In place: the stream
-  // left that as it was, unless the mask forbids the token.)
-  auto finish = [&](int t, uint32_t s, int v0) {
-    if (!(bits[(t - v0) >> 5].x >> ((t - v0) & 31) & 1u)) return;   // streamed as -inf
-    float x = load_f(in + t);
-    const int c = count[s] & ~kBiased;
-    if (c > 0) {
-      if (a.repetition) x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
-      if (a.presence) x = __fsub_rn(x, pres);
-      if (a.frequency) x = __fsub_rn(x, __fmul_rn(freq, static_cast<float>(c)));
-    }
-    if (count[s] < 0) x = __fadd_rn(x, bias[s]);
+  // open addressing in a table of n entries
+  auto slot_of = [](int t, int n) { return static_cast<int>(__umulhi(static_cast<uint32_t>(t) * 2654435761u, n)); };
+  auto after = [](int s, int n) { return s + 1 < n ? s + 1 : 0; };
+  auto finish = [&](int t, float x) {
     out[t] = rounded<TO>(x);
     x = static_cast<float>(rounded<TO>(x));
     if (x == x) better(bv, bi, x, t);
   };
-  // the same for a token the stream passed; one with a bias waits for its sum
-  auto finish_listed = [&](int t, int v0) {
-    uint32_t s = slot_of(t);
-    while (key[s] != t) s = (s + 1) & (table - 1);
-    if (count[s] >= 0) finish(t, s, v0);
-  };
-  const bool maps = lists || words != nullptr;
-  for (int g0 = first + rank * per; g0 < g_end; g0 += part / kN) {
+  for (int g0 = g_begin; g0 < g_end; g0 += part / kN) {
     const int g1 = min(g_end, g0 + part / kN);
-    const int v0 = head + kN * g0;                      // token of the bit maps' bit 0
-    const int t0 = max(v0, 0), t1 = min(a.V, head + kN * g1);   // the part's tokens
+    const int t0 = max(0, head + kN * g0), t1 = min(a.V, head + kN * g1);   // the part's tokens
     // whole groups [ga, gz); their loads run one round ahead, the first round's
     // while the lists are worked through
     const int ga = kVec ? max(g0, 0) : g1, gz = kVec ? max(ga, min(g1, (a.V - head) / kN)) : g1;
     constexpr int kRound = kUnroll * kThreads;
+    if (g0 != g_begin) {
+      __syncthreads();   // the last part's map and tables have been read
+      read(hist, n_hist, threadIdx.x, th);
+      read(ids, n_bias, threadIdx.x, tb);
+      clear_tables();
+    }
+    // the map: words w0 ... of the mask, and one behind the last for the shifts
+    const int w0 = t0 >> 5, n_map = ((t1 - 1) >> 5) - w0 + 2;
+    for (int i = threadIdx.x; i < n_map; i += kThreads) {
+      if (words != nullptr && w0 + i < n_words)
+        cp_async4(smem_u32(bits + i), words + w0 + i);
+      else
+        bits[i] = ~0u;
+    }
+    // the tokens around the whole groups, few but without alignment
+    const int n0 = max(0, min(t1, head + kN * ga) - t0), z = max(t0 + n0, head + kN * gz);
+    const int n1 = max(0, t1 - z);
+    auto around = [&](int i) { return i < n0 ? t0 + i : z + i - n0; };
+    const float x_around = threadIdx.x < n0 + n1 ? load_f(in + around(threadIdx.x)) : 0.f;
     Piece<TI, kN> next[kUnroll];
     const TI* src = in + head + static_cast<size_t>(ga + threadIdx.x) * kN;   // of the next round
-    auto load_round = [&](int left) {    // left: groups from this thread's next on
 #pragma unroll
-      for (int i = 0; i < kUnroll; ++i)
-        if (i * kThreads < left) next[i].load(src + i * kThreads * kN);
-      src += kRound * kN;
-    };
-    // the lists' first entries too
-    auto read = [&](const int* list, int n, int i, int (&t)[4]) {
-#pragma unroll
-      for (int u = 0; u < 4; ++u) t[u] = i + u * kThreads < n ? list[i + u * kThreads] : -1;
-    };
-    int th[4], tb[4];
-    read(hist, n_hist, threadIdx.x, th);
-    read(ids, n_bias, threadIdx.x, tb);
-    load_round(gz - ga - threadIdx.x);
-    if (maps) {
-      __syncthreads();   // the last part's maps and table have been read
-      const int n_map = ((t1 - v0) >> 5) + 1, w0 = v0 >> 5;     // w0: -1 before token 0
-      for (int i = threadIdx.x; i < n_map; i += 4 * kThreads) {
-        uint32_t lo[4], hi[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int w = w0 + i + u * kThreads;
-          lo[u] = hi[u] = ~0u;
-          if (words != nullptr) {
-            lo[u] = w >= 0 && w < n_words ? words[w] : 0u;
-            hi[u] = (v0 & 31) != 0 && w + 1 < n_words ? words[w + 1] : 0u;
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (i + u * kThreads < n_map)
-            bits[i + u * kThreads] = make_uint2(__funnelshift_r(lo[u], hi[u], v0 & 31), 0u);
-      }
-    }
+    for (int i = 0; i < kUnroll; ++i)
+      if (i * kThreads < gz - ga - static_cast<int>(threadIdx.x)) next[i].load(src + i * kThreads * kN);
+    cp_async_wait_all();
+    __syncthreads();
     if (lists) {
-      // ---- the listed tokens of the part.  At most `table` * 3/4 of them: the
-      // lists, or else the part, are no longer than that.
+      // ---- the listed tokens of the part.  The tables hold more entries than that:
+      // the launcher sizes them by the lists, or else by the part.
+      if (n_hist < 0 || n_hist > a.n_history) {
+        if (threadIdx.x == 0 && err_word) atomicCAS(err_word, 0, kModelErrIndex);
+        n_hist = n_hist < 0 ? 0 : a.n_history;
+      }
+      // The first to enter a token sends for the word that holds its logit and
+      // takes it off the map.
       auto enter = [&](int t, bool biased) {
-        uint32_t s = slot_of(t);
-        for (;; s = (s + 1) & (table - 1)) {
-          const int k = atomicCAS(&key[s], -1, t);
-          if (k == -1 || k == t) break;
+        int s = slot_of(t, table), k;
+        while ((k = atomicCAS(&key[s], -1, t)) != -1 && (k & ~kBiased) != t) s = after(s, table);
+        if (k == -1) {
+          cp_async4(smem_u32(value + s), reinterpret_cast<const void*>(reinterpret_cast<uintptr_t>(in + t) & ~uintptr_t{3}));
+          const uint32_t bit = 1u << (t & 31);
+          if (!(atomicAnd(&bits[(t >> 5) - w0], ~bit) & bit)) atomicAdd(&count[s], kForbidden);
         }
-        if (biased)
-          atomicOr(&count[s], kBiased);
-        else
+        if (!biased) {
           atomicAdd(&count[s], 1);
-        atomicOr(&bits[(t - v0) >> 5].y, 1u << ((t - v0) & 31));
+          return;
+        }
+        atomicOr(&key[s], kBiased);
+        s = slot_of(t, n_sums);
+        while ((k = atomicCAS(&bias_key[s], -1, t)) != -1 && k != t) s = after(s, n_sums);
       };
-      auto enter_all = [&](const int (&t)[4], bool biased) {
+      auto enter_all = [&](const int (&t)[4], int i, int n, bool biased) {
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
+          if (i + u * kThreads >= n) break;
           if (t[u] >= t0 && t[u] < t1) enter(t[u], biased);
           if (t[u] >= a.V && err_word) atomicCAS(err_word, 0, kModelErrIndex);
         }
       };
-      for (int i = threadIdx.x; i < table; i += kThreads) {
-        key[i] = -1;
-        count[i] = 0;
-        bias[i] = 0.f;
-      }
-      __syncthreads();
-      enter_all(th, false);
-      enter_all(tb, true);
+      enter_all(th, threadIdx.x, n_hist, false);
+      enter_all(tb, threadIdx.x, n_bias, true);
       for (int i = threadIdx.x + 4 * kThreads; i < n_hist; i += 4 * kThreads) {
         read(hist, n_hist, i, th);
-        enter_all(th, false);
+        enter_all(th, i, n_hist, false);
       }
       for (int i = threadIdx.x + 4 * kThreads; i < n_bias; i += 4 * kThreads) {
         read(ids, n_bias, i, tb);
-        enter_all(tb, true);
+        enter_all(tb, i, n_bias, true);
       }
+      // in place the stream writes where they come from
+      if (static_cast<const void*>(in) == out) cp_async_wait_all();
     }
-    if (maps) __syncthreads();
-    if (lists) {
-      // The biases' sums: the last warp, in list order, while the others stream.
-      // Entries of a warp's 32 that name one token are summed alike by every
-      // lane that names it.
-      if (n_bias > 0 && warp == kThreads / 32 - 1) {
-        const float* val = a.bias + static_cast<long long>(row) * a.n_bias;
-        for (int i0 = 0; i0 < n_bias; i0 += 32) {
-          const int i = i0 + lane;
-          const int t = i < n_bias ? ids[i] : -1;
-          const bool here = t >= t0 && t < t1;
-          if (!__any_sync(0xffffffffu, here)) continue;
-          const float x = here ? val[i] : 0.f;
-          uint32_t s = 0;
-          if (here)
-            for (s = slot_of(t); key[s] != t;) s = (s + 1) & (table - 1);
-          float sum = here ? bias[s] : 0.f;
-          const unsigned same = __match_any_sync(0xffffffffu, here ? t : -1 - lane);
-          if (__all_sync(0xffffffffu, same == 1u << lane)) {
-            sum += x;
-          } else {
-            for (int l = 0; l < 32; ++l) {
-              const float y = __shfl_sync(0xffffffffu, x, l);
-              if (same >> l & 1u) sum += y;
-            }
+    __syncthreads();
+    // The biases' sums: the last warp, in list order, while the others stream.
+    // Entries of a warp's 32 that name one token are summed alike by every lane
+    // that names it.
+    if (n_bias > 0 && warp == kThreads / 32 - 1) {
+      const float* val = a.bias + static_cast<long long>(row) * a.n_bias;
+      for (int i0 = 0; i0 < n_bias; i0 += 32) {
+        const int i = i0 + lane;
+        const int t = i < n_bias ? ids[i] : -1;
+        const bool here = t >= t0 && t < t1;
+        if (!__any_sync(0xffffffffu, here)) continue;
+        const float x = here ? val[i] : 0.f;
+        int s = 0;
+        if (here)
+          for (s = slot_of(t, n_sums); bias_key[s] != t;) s = after(s, n_sums);
+        float sum = here ? bias[s] : 0.f;
+        const unsigned same = __match_any_sync(0xffffffffu, here ? t : -1 - lane);
+        if (__all_sync(0xffffffffu, same == 1u << lane)) {
+          sum += x;
+        } else {
+          for (int l = 0; l < 32; ++l) {
+            const float y = __shfl_sync(0xffffffffu, x, l);
+            if (same >> l & 1u) sum += y;
           }
-          __syncwarp();
-          if (here) bias[s] = sum;
-          __syncwarp();
         }
+        __syncwarp();
+        if (here) bias[s] = sum;
+        __syncwarp();
       }
     }
 
-    // ---- stream the part: whole groups, then the tokens around them
+    // The value of listed token t, entry s, but for the biases.  (The mask's -inf
+    // was streamed: count[s] >= 0 here.)
+    auto penalised = [&](int t, int s) {
+      float x;
+      if constexpr (sizeof(TI) == 4)
+        x = __uint_as_float(value[s]);
+      else
+        x = __uint_as_float(reinterpret_cast<uintptr_t>(in + t) & 2 ? value[s] & 0xffff0000u : value[s] << 16);
+      const int c = count[s];
+      if (c > 0) {
+        if (a.repetition) x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
+        if (a.presence) x = __fsub_rn(x, pres);
+        if (a.frequency) x = __fsub_rn(x, __fmul_rn(freq, static_cast<float>(c)));
+      }
+      return x;
+    };
+    auto stray = [&](int v, float x) {
+      if (!(bits[(v >> 5) - w0] >> (v & 31) & 1u)) x = -INFINITY;
+      out[v] = rounded<TO>(x);
+      x = static_cast<float>(rounded<TO>(x));
+      if (x > -INFINITY) better(bv, bi, x, v);
+    };
+    if (threadIdx.x < n0 + n1) stray(around(threadIdx.x), x_around);
+    for (int i = threadIdx.x + kThreads; i < n0 + n1; i += kThreads) stray(around(i), load_f(in + around(i)));
+
+    // ---- stream the part's whole groups; listed tokens as -inf, so that they
+    // take no part in the maximum
+    float pv = -INFINITY;        // the largest value of the thread's groups, and
+    int pg = -1;                 // the first group with it
     {
       TO* dst = out + head + static_cast<size_t>(ga + threadIdx.x) * kN;
-      // a round moves whole words of the maps on: one place in a word a thread
-      const uint2* map = bits + (ga - g0 + threadIdx.x) * kN / 32;
-      const int place = (ga - g0 + threadIdx.x) * kN & 31;
-      float pv = -INFINITY;   // the largest value of the thread's groups, and
-      int pg = -1;            // the first group with it
-      auto round = [&](int g, int left, auto all) {
+      // a round moves whole words of the map on: one place in a word a thread
+      const int v = head + (ga + static_cast<int>(threadIdx.x)) * kN, place = v & 31;
+      const uint32_t* map = bits + (v >> 5) - w0;
+      auto round = [&](int g, int left, auto all) {   // all: this round and the next are whole
         Piece<TI, kN> raw[kUnroll];
 #pragma unroll
         for (int i = 0; i < kUnroll; ++i) raw[i] = next[i];
-        load_round(left - kRound);
-        uint32_t found = 0;      // the round's listed tokens, kN bits a group
+        src += kRound * kN;
+#pragma unroll
+        for (int i = 0; i < kUnroll; ++i)
+          if (all || i * kThreads < left - kRound) next[i].load(src + i * kThreads * kN);
 #pragma unroll
         for (int i = 0; i < kUnroll; ++i) {
           if (!all && i * kThreads >= left) break;
           float x[kN];
           raw[i].unpack(x);
-          uint32_t listed = 0;
-          if (maps) {
-            const uint2 m = map[i * kThreads * kN / 32];
-            listed = m.y >> place & kMaskN;
-            found |= listed << (i * kN);
-            const uint32_t allowed = m.x >> place;
+          const uint32_t* m = map + i * kThreads * kN / 32;
+          const uint32_t keep = __funnelshift_r(m[0], m[1], place);
 #pragma unroll
-            for (int e = 0; e < kN; ++e)
-              if (!(allowed & (1u << e))) x[e] = -INFINITY;
-          }
+          for (int e = 0; e < kN; ++e)
+            if (!(keep & (1u << e))) x[e] = -INFINITY;
           Piece<TO, kN> y;
           y.pack(x);
           y.store(dst + i * kThreads * kN);
-          if (a.idx != nullptr) {
-            y.unpack(x);         // as they were stored
-            if (listed != 0) {   // listed tokens take part below; fmaxf passes over NaN
+          float top = x[0];        // fmaxf passes over NaN
 #pragma unroll
-              for (int e = 0; e < kN; ++e)
-                if (listed & (1u << e)) x[e] = __int_as_float(0x7fffffff);
-            }
-            float top = x[0];
-#pragma unroll
-            for (int e = 1; e < kN; ++e) top = fmaxf(top, x[e]);
-            const bool more = top > pv;
-            pv = more ? top : pv;
-            pg = more ? g + i * kThreads : pg;
-          }
-        }
-        // while their lines are at hand
-        for (; found != 0; found &= found - 1) {
-          const int b = __ffs(found) - 1;
-          finish_listed(head + (g + b / kN * kThreads) * kN + b % kN, v0);
+          for (int e = 1; e < kN; ++e) top = fmaxf(top, x[e]);
+          top = static_cast<float>(rounded<TO>(top));
+          const bool more = top > pv;
+          pv = more ? top : pv;
+          pg = more ? g + i * kThreads : pg;
         }
         dst += kRound * kN;
         map += kRound * kN / 32;
       };
       int gb = ga;
-      for (; gb + kRound <= gz; gb += kRound) round(gb + threadIdx.x, gz - gb - threadIdx.x, std::true_type{});
-      if (gb < gz) round(gb + threadIdx.x, gz - gb - threadIdx.x, std::false_type{});
-      // which of the group's tokens it was: this thread wrote them
-      if (pg >= 0) {
-        const uint32_t listed = maps ? bits[(pg - g0) * kN >> 5].y >> ((pg - g0) * kN & 31) : 0u;
-        const TO* y = out + head + static_cast<size_t>(pg) * kN;
-        int e = 0;
-        while (e < kN - 1 && (load_f(y + e) != pv || (listed >> e & 1u))) ++e;
-        better(bv, bi, pv, head + kN * pg + e);
-      }
+      for (; gb + 2 * kRound <= gz; gb += kRound) round(gb + threadIdx.x, 0, std::true_type{});
+      for (; gb < gz; gb += kRound) round(gb + threadIdx.x, gz - gb - static_cast<int>(threadIdx.x), std::false_type{});
     }
-    {
-      const int n0 = max(0, min(t1, head + kN * ga) - t0), z = max(t0 + n0, head + kN * gz);
-      const int n1 = max(0, t1 - z);
-      for (int i = threadIdx.x; i < n0 + n1; i += kThreads) {
-        const int v = i < n0 ? t0 + i : z + i - n0;
-        const uint2 m = maps ? bits[(v - v0) >> 5] : make_uint2(~0u, 0u);
-        float x = load_f(in + v);
-        if (!(m.x >> ((v - v0) & 31) & 1u)) x = -INFINITY;
-        out[v] = rounded<TO>(x);
-        x = static_cast<float>(rounded<TO>(x));
-        if (m.y >> ((v - v0) & 31) & 1u)
-          finish_listed(v, v0);
-        else if (x == x)
-          better(bv, bi, x, v);
-      }
-    }
+    // Which token it was, for the warp's largest, from what the thread wrote; the
+    // loads pass while the listed tokens are finished.  (A listed one of that value
+    // may have come to lie before it, and is as good.)
+    const float top = warp_max(pv);
+    const bool mine = pg >= 0 && pv == top;
+    Piece<TO, kN> wrote;
+    if (mine) wrote.load(out + head + static_cast<size_t>(pg) * kN);
 
-    // ---- the tokens with a bias
-    if (n_bias > 0) {
-      __syncthreads();   // streamed, biases summed
-      for (int s = threadIdx.x; s < table; s += kThreads)
-        if (count[s] < 0) finish(key[s], s, v0);
+    // ---- the listed tokens
+    if (lists) {
+      cp_async_wait_all();
+      __syncthreads();   // streamed, values here, biases summed
+      for (int s = threadIdx.x; s < table / 4; s += kThreads) {
+        const int4 k = reinterpret_cast<const int4*>(key)[s];
+        const int ks[4] = {k.x, k.y, k.z, k.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)   // free and flagged ones are below zero
+          if (ks[e] >= 0 && count[4 * s + e] >= 0) finish(ks[e], penalised(ks[e], 4 * s + e));
+      }
+      if (n_bias > 0) {
+        for (int i = threadIdx.x; i < n_sums; i += kThreads) {
+          const int t = bias_key[i];
+          if (t < 0) continue;
+          int s = slot_of(t, table);
+          while ((key[s] & ~kBiased) != t) s = after(s, table);
+          if (count[s] >= 0) finish(t, __fadd_rn(penalised(t, s), bias[i]));
+        }
+      }
+    }
+    if (mine) {
+      float x[kN];
+      wrote.unpack(x);
+      int e = kN - 1;
+#pragma unroll
+      for (int i = kN - 2; i >= 0; --i)
+        if (x[i] == pv) e = i;
+      better(bv, bi, pv, head + kN * pg + e);
     }
   }
   if (a.idx == nullptr) return;
-
-  // A part without a value above -inf: its first token that is a number.  (The
-  // stream looks for values above -inf alone.)
-  if (__syncthreads_and(bi == kNone || bv == -INFINITY)) {
-    const int v0 = max(0, head + kN * (first + rank * per)), v1 = min(a.V, head + kN * g_end);
-    for (int v = v0 + threadIdx.x; v < v1; v += kThreads) {
-      const float x = load_f(out + v);
-      if (x == x) {
-        better(bv, bi, x, v);
-        break;
-      }
-    }
-  }
 
   // ---- the greedy token: warp, CTA, cluster
   auto reduce = [&]() {
@@ -406,20 +415,35 @@ __global__ void __launch_bounds__(kThreads, 4)
       better(bv, bi, v2, i2);
     }
   };
-  reduce();
-  if (lane == 0) {
-    best_v[warp] = bv;
-    best_i[warp] = bi;
-  }
-  __syncthreads();
-  if (warp == 0) {
-    bv = lane < kThreads / 32 ? best_v[lane] : -INFINITY;
-    bi = lane < kThreads / 32 ? best_i[lane] : kNone;
+  auto reduce_cta = [&]() {   // the same in every thread
     reduce();
     if (lane == 0) {
-      cta_v = bv;
-      cta_i = bi;
+      best_v[warp] = bv;
+      best_i[warp] = bi;
     }
+    __syncthreads();
+    bv = best_v[lane % (kThreads / 32)];
+    bi = best_i[lane % (kThreads / 32)];
+    reduce();
+  };
+  reduce_cta();
+  // No value above -inf: the first token that is a number.  (The stream looks for
+  // values above -inf alone.)
+  if (bi == kNone || bv == -INFINITY) {
+    const int v0 = max(0, head + kN * g_begin), v1 = min(a.V, head + kN * g_end);
+    for (int v = v0 + threadIdx.x; v < v1; v += kThreads) {
+      const float x = load_f(out + v);
+      if (x == x) {
+        better(bv, bi, x, v);
+        break;
+      }
+    }
+    __syncthreads();   // every warp has read the first round's
+    reduce_cta();
+  }
+  if (threadIdx.x == 0) {
+    cta_v = bv;
+    cta_i = bi;
   }
   if (nc > 1) cluster_sync();   // every CTA of the cluster reaches both barriers
   if (rank == 0 && threadIdx.x == 0) {
@@ -444,24 +468,27 @@ cudaError_t launch_typed(cudaStream_t stream, const LogitsPenalty& a, int* err_w
   int nc = 1;
   while (nc < kCluster && static_cast<long long>(a.rows) * nc < 3 * current_sm_count() && a.V / (2 * nc) >= 1024)
     nc *= 2;
-  // The table holds the lists, filled to three quarters at most; lists longer
-  // than the largest table are worked through part by part, a part no longer
-  // than what the table holds.
-  const long long n = (a.history ? a.n_history : 0) + static_cast<long long>(a.bias_ids ? a.n_bias : 0);
-  int table = 0;
+  // The tables hold twice the lists (at four thirds a search is so long that 512
+  // rows with 1024 different tokens each took 62 us for 4x); lists longer than
+  // three quarters of the largest table are worked through part by part, a part no
+  // longer than that.  (Small tables leave the L1 cache to the loads in flight:
+  // with 26 KB more a row the stream took 27 us for 23.)
+  constexpr int kMost = kMaxTable / 4 * 3;
+  const long long n_bias = a.bias_ids ? a.n_bias : 0, n = (a.history ? a.n_history : 0) + n_bias;
+  auto entries = [](long long m) {
+    return 2 * m < kMaxTable ? (2 * static_cast<int>(m) + 3) / 4 * 4 : kMaxTable;
+  };
+  const int table = entries(n), n_sums = entries(n_bias);
   // a CTA's share of the row, at most
   int part = ((a.V + nc - 1) / nc + 24 + 31) / 32 * 32;
-  if (n > 0) {
-    for (table = 64; table < kMaxTable && table * 3LL / 4 < n; table *= 2) {}
-    if (table * 3LL / 4 < n && part > table * 3 / 4) part = table * 3 / 4;
-  }
+  if (n > kMost && part > kMost) part = kMost;
   part = part < kMaxPart ? part : kMaxPart;
-  const size_t smem = static_cast<size_t>(table) * 12 + (n > 0 || a.mask ? static_cast<size_t>(part) / 4 + 8 : 0);
+  const size_t smem = static_cast<size_t>(table) * 12 + static_cast<size_t>(n_sums) * 8 + static_cast<size_t>(part) / 8 + 16;
   static SmemOptIn opt_in[2];
   const cudaError_t e = allow_smem(kern, static_cast<int>(smem), opt_in[vec]);
   if (e != cudaSuccess) return e;
   return launch_dependent(kern, dim3(static_cast<unsigned>(a.rows) * nc), dim3(kThreads), smem, stream,
-                          nc, a, table, part, err_word);
+                          nc, a, table, n_sums, part, err_word);
 }
 
 }  // namespace

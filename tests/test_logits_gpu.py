@@ -255,3 +255,25 @@ def test_out_beside_logits_in_one_buffer():
 def test_long_lists(n_hist, n_bias, V):
     """Lists longer than the largest table, vocabularies longer than a bit map."""
     run(2, V, n_hist, n_bias, True, seed=n_hist, lens=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows, V, n_hist, n_bias, pad", [
+    (5, 4097, 700, 40, 0), (3, 4099, 64, 3, 7), (6, 33, 300, 20, 1), (2, 20011, 9000, 300, 2)])
+def test_in_place_with_lists(dtype, rows, V, n_hist, n_bias, pad):
+    """Listed tokens are computed from the logits that the stream overwrites."""
+    run(rows, V, n_hist, n_bias, True, dtype, dtype, seed=V + pad, pad=pad, in_place=True, lens=True)
+
+
+@pytest.mark.parametrize("V, n_hist", [(50257, 1024), (6000, 6000), (130001, 6144)])
+def test_histories_of_different_tokens(V, n_hist):
+    """Every entry another token: the fullest table."""
+    rng = np.random.default_rng(V)
+    rows = 3
+    hist = np.stack([rng.permutation(V)[:n_hist] for _ in range(rows)]).astype(np.int32)
+    x = torch.from_numpy(rng.standard_normal((rows, V)).astype(np.float32) * 4).to(DEV).to(torch.bfloat16)
+    rep, freq = np.full(rows, 1.3, np.float32), np.full(rows, 0.2, np.float32)
+    want, tol = reference(x.float().cpu().numpy(), hist, None, rep, None, freq, None, None, None)
+    d = lambda a: torch.from_numpy(a).to(DEV)
+    y, idx = _ops().logits_penalty(x, history=d(hist), repetition=d(rep), frequency=d(freq), out_dtype=torch.float32)
+    check(y, idx, want, tol)
