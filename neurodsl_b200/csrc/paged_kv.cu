@@ -104,6 +104,43 @@ __device__ __forceinline__ uint32_t ordered(float w) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
+// A warp moves 32 kept rows of one (sequence, kv head), a lane's from position
+// `pos` (-1: none) to `slot`: a lane looks its row up, then eight lanes move a row,
+// 4 rows of K and V an instruction and 16 in flight.
+__device__ __forceinline__ void gather_rows(const PagedEvict& a, int b, int h, int slot, int pos, int* err_word) {
+  const int lane = threadIdx.x & 31;
+  long long src = -1, dst = -1;
+  if (pos >= 0) {
+    src = pool_row(a.pool, a.pool.table, a.pool.table_ld, a.pool.max_pages, b, h, pos);
+    dst = pool_row(a.pool, a.out_table, a.out_table_ld, a.out_pages, b, h, slot);
+    if (src < 0 || dst < 0) raise(err_word);
+  }
+  if (!__any_sync(0xffffffffu, dst >= 0)) return;
+  const int c = (lane & 7) * 8;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    uint4 kk[4], vv[4];
+    long long to[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = half * 16 + i * 4 + (lane >> 3);
+      const long long from = __shfl_sync(0xffffffffu, src, r);
+      to[i] = __shfl_sync(0xffffffffu, dst, r);
+      kk[i] = vv[i] = make_uint4(0, 0, 0, 0);   // a row without a page reads as zeros
+      if (from >= 0 && to[i] >= 0) {
+        kk[i] = *reinterpret_cast<const uint4*>(a.pool.k + from * 64 + c);
+        vv[i] = *reinterpret_cast<const uint4*>(a.pool.v + from * 64 + c);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (to[i] >= 0) {
+        *reinterpret_cast<uint4*>(a.pool.k + to[i] * 64 + c) = kk[i];
+        *reinterpret_cast<uint4*>(a.pool.v + to[i] * 64 + c) = vv[i];
+      }
+  }
+}
+
 // One block per (sequence, kv head): which positions stay.  The first `sinks`
 // and the last `recent` always do; the rest of the budget goes to the largest
 // weights between, the lowest positions first among equals.  The weights stay in
@@ -115,8 +152,11 @@ __device__ __forceinline__ uint32_t ordered(float w) {
 // memory each; from the second digit on only the few weights that share the
 // digits so far take part.  (Two bits at a time by counting, without
 // atomics, is 16 passes over all weights: 36 us for 256 heads of up to 8192
-// keys, against 16.5.)
-template <int kThreads, int kR>
+// keys, against 16.5 with these.)
+//
+// kGather: the block then moves its rows itself (the launcher's rule), from the
+// positions left in the histogram's memory.
+template <int kThreads, int kR, bool kGather>
 __global__ void __launch_bounds__(kThreads, kThreads < 1024 ? 2 : 1)
     paged_select_kernel(const PagedEvict a, int* __restrict__ err_word) {
   constexpr int kW = kThreads / 32;
@@ -128,7 +168,7 @@ __global__ void __launch_bounds__(kThreads, kThreads < 1024 ? 2 : 1)
   __shared__ int found_above;
   __shared__ int sure_sm[kW], tie_sm[kW];
   pdl_wait();
-  pdl_trigger();
+  if (!kGather) pdl_trigger();   // what follows a writing of the cache starts when that is done
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int b = blockIdx.x / a.pool.Hkv, h = blockIdx.x % a.pool.Hkv;
   const long long cap = static_cast<long long>(a.pool.max_pages) * a.pool.page_size;
@@ -264,10 +304,18 @@ __global__ void __launch_bounds__(kThreads, kThreads < 1024 ? 2 : 1)
     if (keep) {
       const int at = slot + __popc(m & below);
       kept[at] = p0 + 32 * r;
+      if (kGather) hist[at] = static_cast<uint32_t>(p0 + 32 * r);
       w_out[at] = kKeep ? v[kKeep ? r : 0] : w[p0 + 32 * r];
     }
     slot += __popc(m);
     tie_at += __popc(m_tie);
+  }
+  if constexpr (kGather) {
+    __syncthreads();
+    for (int i = warp * 32; i < n; i += kThreads) {
+      const int slot = i + lane;
+      gather_rows(a, b, h, slot, slot < n ? static_cast<int>(hist[slot]) : -1, err_word);
+    }
   }
   for (int i = n + threadIdx.x; i < a.budget; i += kThreads) kept[i] = -1;
   // zeros behind the kept weights, 16 bytes at a time where the rows allow
@@ -284,54 +332,21 @@ __global__ void __launch_bounds__(kThreads, kThreads < 1024 ? 2 : 1)
   if (h == 0 && threadIdx.x == 0) a.new_lens[b] = n;
 }
 
-// A warp moves 32 kept rows of one (sequence, kv head): a lane looks one up,
-// then eight lanes move a row, 4 rows of K and V an instruction and 16 in flight.
 __global__ void __launch_bounds__(256)
     paged_gather_kernel(const PagedEvict a, int* __restrict__ err_word) {
   pdl_wait();
-  const int lane = threadIdx.x & 31;
   const int per_head = (a.budget + 31) / 32;
   const long long w = static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
   const long long bh = w / per_head;
   if (bh >= static_cast<long long>(a.B) * a.pool.Hkv) return;
-  const int b = static_cast<int>(bh / a.pool.Hkv), h = static_cast<int>(bh % a.pool.Hkv);
-  const int slot = static_cast<int>(w - bh * per_head) * 32 + lane;
-  const int pos = slot < a.budget ? a.kept[bh * a.budget + slot] : -1;
-  long long src = -1, dst = -1;
-  if (pos >= 0) {
-    src = pool_row(a.pool, a.pool.table, a.pool.table_ld, a.pool.max_pages, b, h, pos);
-    dst = pool_row(a.pool, a.out_table, a.out_table_ld, a.out_pages, b, h, slot);
-    if (src < 0 || dst < 0) raise(err_word);
-  }
-  if (!__any_sync(0xffffffffu, dst >= 0)) return;
-  const int c = (lane & 7) * 8;
-#pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    uint4 kk[4], vv[4];
-    long long to[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = half * 16 + i * 4 + (lane >> 3);
-      const long long from = __shfl_sync(0xffffffffu, src, r);
-      to[i] = __shfl_sync(0xffffffffu, dst, r);
-      kk[i] = vv[i] = make_uint4(0, 0, 0, 0);   // a row without a page reads as zeros
-      if (from >= 0 && to[i] >= 0) {
-        kk[i] = *reinterpret_cast<const uint4*>(a.pool.k + from * 64 + c);
-        vv[i] = *reinterpret_cast<const uint4*>(a.pool.v + from * 64 + c);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (to[i] >= 0) {
-        *reinterpret_cast<uint4*>(a.pool.k + to[i] * 64 + c) = kk[i];
-        *reinterpret_cast<uint4*>(a.pool.v + to[i] * 64 + c) = vv[i];
-      }
-  }
+  const int slot = static_cast<int>(w - bh * per_head) * 32 + (threadIdx.x & 31);
+  gather_rows(a, static_cast<int>(bh / a.pool.Hkv), static_cast<int>(bh % a.pool.Hkv), slot,
+              slot < a.budget ? a.kept[bh * a.budget + slot] : -1, err_word);
 }
 
-template <int kThreads, int kR>
+template <int kThreads, int kR, bool kGather = false>
 cudaError_t launch_select(cudaStream_t stream, const PagedEvict& a, unsigned heads, int* err_word) {
-  return launch_dependent(paged_select_kernel<kThreads, kR>, dim3(heads), dim3(kThreads), 0, stream, 1,
+  return launch_dependent(paged_select_kernel<kThreads, kR, kGather>, dim3(heads), dim3(kThreads), 0, stream, 1,
                           a, err_word);
 }
 
@@ -355,6 +370,18 @@ cudaError_t launch_paged_evict(cudaStream_t stream, const PagedEvict& a, int* er
   // weights in registers as far as they go
   const long long cap = static_cast<long long>(a.pool.max_pages) * a.pool.page_size;
   cudaError_t e;
+  // One launch, each block moving its head's rows, but where that leaves SMs idle:
+  // few heads with many rows, or a third round of blocks (two fit an SM) that is
+  // nearly empty.  12 heads, 256 of 500 keys: 6.2 us against 8.1 in two launches; 512
+  // of 8192: 12.0 against 12.9; 1024 of 8192: 14.9 against 13.1, with 144 heads 24.7
+  // against 27.1, with 240 35.8 against 40.3, with 320 51.5 against 54.0 but 2048 of
+  // them 86.9 against 81.0, with 512 67.3 against 76.6.
+  const unsigned sms = static_cast<unsigned>(current_sm_count());
+  if (cap <= 8192 && a.budget <= 2048 && (heads > sms / 2 || a.budget <= 512) && (heads <= 2 * sms || heads > 3 * sms)) {
+    if (cap <= 1024) return launch_select<512, 2, true>(stream, a, heads, err_word);
+    return heads <= sms ? launch_select<1024, 8, true>(stream, a, heads, err_word)
+                        : launch_select<512, 16, true>(stream, a, heads, err_word);
+  }
   if (cap <= 1024)
     e = launch_select<256, 4>(stream, a, heads, err_word);
   else if (cap <= 8192)

@@ -502,6 +502,16 @@ def test_evict_long(L, budget):
     run_evict([L, L // 2], 2, 32, budget, 4, budget // 8, seed=L)
 
 
+@pytest.mark.parametrize("lens, Hkv, budget", [
+    ([8192], 2, 512), ([8000], 2, 2000), ([1000], 2, 600), ([1500, 1100], 64, 1200),
+    ([1200, 0, 700], 64, 600), ([300, 257, 100, 99, 1], 70, 100),
+    ([1100, 40, 1030, 500, 41, 39, 64, 1], 64, 40), ([600, 900, 1, 0], 45, 513)])
+def test_evict_few_and_many_heads(lens, Hkv, budget):
+    """Heads that leave SMs idle, fill them once or several times over, with one
+    block a head and with two launches."""
+    run_evict(lens, Hkv, 16, budget, 4, budget // 8, seed=budget)
+
+
 def test_evict_ties_and_unusual_weights():
     def all_equal(w):
         w.fill_(0.25)
