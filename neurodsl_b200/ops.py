@@ -663,6 +663,15 @@ def _int(v):
     return v if -_INT_MAX <= v <= _INT_MAX else (_INT_MAX if v > 0 else -1)
 
 
+def _empty(shape, dtype, device, stream):
+    """An output made for a call: on the call's stream, so that its memory is
+    free of work that other streams still have with it."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
 def _addr(t):
     return None if t is None else t.data_ptr()
 
@@ -696,14 +705,14 @@ def window_attn_fwd(Q, K, V, window, sinks=0, scale=None, out=None, out_dtype=to
     if Bk != B or Dk != D or V.shape != k_shape:
         raise ValueError(f"shape mismatch Q{tuple(Q.shape)} K{tuple(K.shape)} V{tuple(V.shape)}")
     if out is None:
-        out = torch.empty(q_shape, dtype=out_dtype, device=Q.device)
+        out = _empty(q_shape, out_dtype, Q.device, stream)
     _tensor(out, "out", None, 4, dev, False)
     if out.shape != q_shape:
         raise ValueError(f"out must be {tuple(q_shape)}, got {tuple(out.shape)}")
     if lse is None:
-        lse = torch.empty((B, H, Sq), dtype=_F32, device=Q.device)
+        lse = _empty((B, H, Sq), _F32, Q.device, stream)
     if row_max is None:
-        row_max = torch.empty((B, H, Sq), dtype=_F32, device=Q.device)
+        row_max = _empty((B, H, Sq), _F32, Q.device, stream)
     _vector(lse, "lse", _F32, B * H * Sq, dev)
     _vector(row_max, "row_max", _F32, B * H * Sq, dev)
     _call(_lib.load().nd_window_attn_fwd, dev, _stream_of(dev, stream), Q.data_ptr(),
@@ -773,12 +782,12 @@ def paged_decode_attn(q, k_pages, v_pages, block_table, lens, k_new=None, v_new=
         if k_new.shape != (B, Hkv, D) or v_new.shape != (B, Hkv, D):
             raise ValueError(f"k_new and v_new must be {(B, Hkv, D)}")
     if out is None:
-        out = torch.empty(q_shape, dtype=out_dtype, device=q.device)
+        out = _empty(q_shape, out_dtype, q.device, stream)
     _tensor(out, "out", None, 3, dev)
     if out.shape != q_shape:
         raise ValueError(f"out must be {tuple(q_shape)}, got {tuple(out.shape)}")
     if lse is None and want_lse:
-        lse = torch.empty((B, H), dtype=_F32, device=q.device)
+        lse = _empty((B, H), _F32, q.device, stream)
     if lse is not None:
         _vector(lse, "lse", _F32, B * H, dev)
     weights_ld = 0
@@ -853,15 +862,15 @@ def paged_kv_evict(k_pages, v_pages, block_table, lens, weights, out_table, budg
     out_pages, out_ld = _matrix(out_table, "out_table", _INT32, B, dev)
     _tensor(weights, "weights", _F32, 3, dev)
     if weights_out is None:
-        weights_out = torch.empty_like(weights)
+        weights_out = _empty(weights.shape, _F32, weights.device, stream)
     _tensor(weights_out, "weights_out", _F32, 3, dev)
     if weights.shape[:2] != (B, Hkv) or weights_out.shape[:2] != (B, Hkv):
         raise ValueError(f"weights and weights_out must be [{B}][{Hkv}][keys]")
     if kept is None:
-        kept = torch.empty((B, Hkv, max(0, int(budget))), dtype=_INT32, device=lens.device)
+        kept = _empty((B, Hkv, max(0, int(budget))), _INT32, lens.device, stream)
     _vector(kept, "kept", _INT32, B * Hkv * max(0, budget), dev)
     if new_lens is None:
-        new_lens = torch.empty((B,), dtype=_INT32, device=lens.device)
+        new_lens = _empty((B,), _INT32, lens.device, stream)
     _vector(new_lens, "new_lens", _INT32, B, dev)
     _call(_lib.load().nd_paged_kv_evict, dev, _stream_of(dev, stream), k_pages.data_ptr(),
           v_pages.data_ptr(), n_pages, page_size, block_table.data_ptr(), table_ld, max_pages,
@@ -891,7 +900,7 @@ def logits_penalty(logits, history=None, history_lens=None, repetition=None, pre
     rows = logits.shape[0]
     V, ld = _matrix(logits, "logits", None, rows, dev)
     if out is None:
-        out = torch.empty((rows, V), dtype=out_dtype or logits.dtype, device=logits.device)
+        out = _empty((rows, V), out_dtype or logits.dtype, logits.device, stream)
     out_V, out_ld = _matrix(out, "out", None, rows, dev)
     if out_V != V:
         raise ValueError(f"out must be {(rows, V)}, got {tuple(out.shape)}")
@@ -926,7 +935,7 @@ def logits_penalty(logits, history=None, history_lens=None, repetition=None, pre
         if mask.dim() == 2:
             mask_ld = mask.stride(0) if rows > 1 else words
     if idx is None and greedy:
-        idx = torch.empty((rows,), dtype=_INT32, device=logits.device)
+        idx = _empty((rows,), _INT32, logits.device, stream)
     if idx is not None:
         _vector(idx, "idx", _INT32, rows, dev)
     _call(_lib.load().nd_logits_penalty, dev, _stream_of(dev, stream), logits.data_ptr(),

@@ -206,3 +206,33 @@ def test_current_stream_and_capture():
         ops.logits_penalty(**args)
     s.synchronize()
     assert torch.equal(args["out"], want)
+
+
+@pytest.mark.parametrize("name, made", [("window_attn_fwd", ("out", "lse", "row_max")),
+                                        ("paged_decode_attn", ("out", "lse", "workspace")),
+                                        ("paged_kv_evict", ("weights_out", "kept", "new_lens")),
+                                        ("logits_penalty", ("out", "idx"))])
+def test_outputs_are_made_on_the_calls_stream(monkeypatch, name, made):
+    """Memory from another stream's pool may still be in use there."""
+    ops, _ = _ops()
+    args = arguments(name)
+    want = getattr(ops, name)(**args)
+    torch.cuda.synchronize()
+    args = arguments(name)      # weights and pages as they were
+    args.update(dict.fromkeys(made))
+    if "out" in made:
+        args["out_dtype"] = want[0].dtype
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    streams = []
+    for fn in ("empty", "zeros", "empty_like"):
+        def note(*a, real=getattr(torch, fn), **k):
+            streams.append(torch.cuda.current_stream())
+            return real(*a, **k)
+        monkeypatch.setattr(torch, fn, note)
+    got = getattr(ops, name)(**args, stream=s)
+    monkeypatch.undo()
+    assert len(streams) == len(made) and all(x == s for x in streams)
+    s.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
