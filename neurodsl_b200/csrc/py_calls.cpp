@@ -4,7 +4,7 @@
 // A serving step makes these calls once a layer with kernels of a few
 // microseconds, and the front end's argument checks and the foreign-function
 // call cost more than that: back to back, a decode that takes the device 7.4 us
-// took 12.5 a call and takes 7.4 here, a short store 9.8 and 3.5.  Each function
+// took 12.5 a call and 7.4 here, a short store 9.8 and 3.5.  Each function
 // here takes the arguments of its namesake in ops.py, checks that they are what
 // nearly every call passes (tensors of the right types on the current device,
 // outputs given, the current stream), and calls the C entry point, which
