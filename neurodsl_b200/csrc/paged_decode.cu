@@ -775,14 +775,15 @@ __global__ void __launch_bounds__(Shape<kRows, kTma>::kThreads, Shape<kRows, kTm
 
 // weights[b][h][j] += sum over the group's query heads of exp(s_j - lse), for
 // every visible key, in the heads' order.  A thread takes four keys of one
-// (sequence, kv head): the scores come in 16-byte pieces.
+// (sequence, kv head): the scores come in 16-byte pieces.  It lets no successor's
+// blocks in before its own are done: the next call's would stand in their way (67
+// us a call for 59 with 8 sequences of 32768 keys).
 constexpr int kWeightThreads = 256;
 constexpr int kWeightKeys = 4 * kWeightThreads;
 
 __global__ void __launch_bounds__(kWeightThreads)
     paged_weights_kernel(const Params p, float* __restrict__ weights, long long weights_ld) {
   pdl_wait();
-  pdl_trigger();
   const int b = blockIdx.y / p.Hkv, h = blockIdx.y % p.Hkv;
   const Span s = make_span(p, p.lens[b]);
   const int key0 = blockIdx.x * kWeightKeys + threadIdx.x * 4;
@@ -833,15 +834,9 @@ cudaError_t launch_typed(cudaStream_t stream, const Params& p, long long max_til
   long long grid = static_cast<long long>(current_sm_count()) * S::kCtas;
   if (grid > kMaxCtas) grid = kMaxCtas;
   if (grid > max_tiles) grid = max_tiles;
-  // Placed early, before the kernel before it has ended, a call starts 0.3 us
-  // sooner (7.4 -> 7.1 us for one sequence).  With weights it does not pay: the
-  // early blocks of the next call stand in the way of this call's second kernel
-  // (62.0 -> 67.0 us a call for 8 sequences of 32768 keys).
-  if (p.scores == nullptr)
-    return launch_dependent(kern, dim3(static_cast<unsigned>(grid)), dim3(S::kThreads), smem, stream, 1, p,
-                            tk, tv);
-  return launch_ex(kern, dim3(static_cast<unsigned>(grid)), dim3(S::kThreads), smem, stream, 1, true, p,
-                   tk, tv);
+  // placed early, before the kernel before it has ended: a call starts 0.3 us sooner
+  return launch_dependent(kern, dim3(static_cast<unsigned>(grid)), dim3(S::kThreads), smem, stream, 1, p, tk,
+                          tv);
 }
 
 long long scores_ld(long long max_len) { return (max_len + kTile - 1) / kTile * kTile; }
