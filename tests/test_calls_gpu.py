@@ -236,3 +236,41 @@ def test_outputs_are_made_on_the_calls_stream(monkeypatch, name, made):
     s.synchronize()
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+def test_two_threads_at_once():
+    """Each with a stream, a workspace and buffers of its own."""
+    import threading
+    ops, _ = _ops()
+    names = ["paged_decode_attn", "logits_penalty", "window_attn_fwd"]
+    want = {}
+    for name in names:
+        args = arguments(name)
+        args.pop("weights", None)
+        want[name] = [t.clone() for t in getattr(ops, name)(**args)]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work():
+        try:
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                sets = {}
+                for name in names:
+                    sets[name] = arguments(name)
+                    sets[name].pop("weights", None)
+                for _ in range(40):
+                    for name in names:
+                        got = getattr(ops, name)(**sets[name])
+                        if not all(torch.equal(a, b) for a, b in zip(got, want[name])):
+                            wrong.append(name)
+        except Exception as e:  # noqa: BLE001
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not wrong
