@@ -19,6 +19,7 @@ namespace nd {
 namespace {
 
 constexpr int kVec = 8;   // 16-byte pieces of a row
+constexpr int kMaxShared = 54 * 1024;   // weights in shared memory, beside the histogram
 
 __device__ __forceinline__ void raise(int* err_word) {
   if (err_word) atomicCAS(err_word, 0, kModelErrIndex);
@@ -144,8 +145,8 @@ __device__ __forceinline__ void gather_rows(const PagedEvict& a, int b, int h, i
 // One block per (sequence, kv head): which positions stay.  The first `sinks`
 // and the last `recent` always do; the rest of the budget goes to the largest
 // weights between, the lowest positions first among equals.  The weights stay in
-// registers (kR a thread; with kR = 0, for longer caches, they are read again
-// each time, from L2): every warp owns a contiguous span of positions, lane by
+// registers (kR a thread) or, for longer caches, in shared memory (kShared) or, for
+// the longest, are read again each time, from L2: every warp owns a contiguous span of positions, lane by
 // lane, so that ballots and one sum over the warps give each kept position its
 // slot.  The smallest weight that stays is found by its digits of 11, 11 and 10
 // bits, from the top of an order-preserving integer, with a histogram in shared
@@ -156,7 +157,7 @@ __device__ __forceinline__ void gather_rows(const PagedEvict& a, int b, int h, i
 //
 // kGather: the block then moves its rows itself (the launcher's rule), from the
 // positions left in the histogram's memory.
-template <int kThreads, int kR, bool kGather>
+template <int kThreads, int kR, bool kGather, bool kShared>
 __global__ void __launch_bounds__(kThreads, kThreads < 1024 ? 2 : 1)
     paged_select_kernel(const PagedEvict a, int* __restrict__ err_word) {
   constexpr int kW = kThreads / 32;
@@ -195,15 +196,25 @@ __global__ void __launch_bounds__(kThreads, kThreads < 1024 ? 2 : 1)
   };
   constexpr bool kKeep = kR > 0 && kR <= 16;   // the weights themselves in registers too
   uint32_t x[kR > 0 ? kR : 1];
-  float v[kR > 0 ? kR : 1];
+  constexpr int kStep = kKeep ? kR : 8;        // weights in flight a thread
+  float v[kKeep ? kR : kStep];
   if constexpr (kR > 0) {
 #pragma unroll
-    for (int r = 0; r < kR; ++r) v[r] = p0 + 32 * r < L ? w[p0 + 32 * r] : 0.f;
+    for (int r0 = 0; r0 < kR; r0 += kStep) {
 #pragma unroll
-    for (int r = 0; r < kR; ++r) x[r] = p0 + 32 * r >= lo && p0 + 32 * r < hi ? ordered(v[r]) : 0u;
+      for (int r = r0; r < r0 + kStep; ++r) v[kKeep ? r : r - r0] = p0 + 32 * r < L ? w[p0 + 32 * r] : 0.f;
+#pragma unroll
+      for (int r = r0; r < r0 + kStep; ++r)
+        x[r] = p0 + 32 * r >= lo && p0 + 32 * r < hi ? ordered(v[kKeep ? r : r - r0]) : 0u;
+    }
+  }
+  extern __shared__ uint32_t x_sm[];
+  if constexpr (kShared) {   // each thread reads its own again
+    for (int r = 0; r < rows; ++r) x_sm[p0 + 32 * r] = read(r);
   }
   auto weight = [&](int r) -> uint32_t {
     if constexpr (kR > 0) return x[r];
+    else if constexpr (kShared) return x_sm[p0 + 32 * r];
     else return read(r);
   };
 
@@ -211,7 +222,7 @@ __global__ void __launch_bounds__(kThreads, kThreads < 1024 ? 2 : 1)
   uint32_t threshold = 0;
   int above = 0;           // weights above the threshold
   if (!all && need > 0) {
-#pragma unroll
+#pragma unroll (kR > 16 ? 1 : 3)   // unrolled the 24 would spill
     for (int digit = 0; digit < 3; ++digit) {
       const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0;
       const uint32_t bins = digit == 2 ? 1023u : 2047u;
@@ -270,12 +281,14 @@ __global__ void __launch_bounds__(kThreads, kThreads < 1024 ? 2 : 1)
       sure_bits |= static_cast<uint32_t>(x[r] > t_up) << r;
       tie_bits |= static_cast<uint32_t>(x[r] == t_up) << r;
     }
-    // the positions that do not compete
-#pragma unroll
-    for (int r = 0; r < kR; ++r) {
-      const int p = p0 + 32 * r;
-      sure_bits |= static_cast<uint32_t>(p < L && (all || p < lo || p >= hi)) << r;
-    }
+    // the positions that do not compete: rows r with p0 + 32 r below a bound are
+    // the lowest bits
+    auto lowest = [&](int bound) {
+      const int m = min(max((bound - p0 + 31) >> 5, 0), 32);
+      return m < 32 ? (1u << m) - 1u : ~0u;
+    };
+    constexpr uint32_t kRows = kR < 32 ? (1u << kR) - 1u : ~0u;
+    sure_bits |= kRows & lowest(L) & (all ? ~0u : lowest(lo) | ~lowest(hi));
   }
   int n_sure = 0, n_tie = 0;
 #pragma unroll
@@ -344,10 +357,18 @@ __global__ void __launch_bounds__(256)
               slot < a.budget ? a.kept[bh * a.budget + slot] : -1, err_word);
 }
 
-template <int kThreads, int kR, bool kGather = false>
+template <int kThreads, int kR, bool kGather = false, bool kShared = false>
 cudaError_t launch_select(cudaStream_t stream, const PagedEvict& a, unsigned heads, int* err_word) {
-  return launch_dependent(paged_select_kernel<kThreads, kR, kGather>, dim3(heads), dim3(kThreads), 0, stream, 1,
-                          a, err_word);
+  auto kern = paged_select_kernel<kThreads, kR, kGather, kShared>;
+  size_t smem = 0;
+  if (kShared) {
+    const size_t cap = static_cast<size_t>(a.pool.max_pages) * a.pool.page_size;
+    smem = (cap + kThreads - 1) / kThreads * kThreads * sizeof(uint32_t);
+    static SmemOptIn opt_in;
+    const cudaError_t e = allow_smem(kern, static_cast<int>(smem), opt_in);
+    if (e != cudaSuccess) return e;
+  }
+  return launch_dependent(kern, dim3(heads), dim3(kThreads), smem, stream, 1, a, err_word);
 }
 
 }  // namespace
@@ -367,7 +388,9 @@ cudaError_t launch_paged_store(cudaStream_t stream, const __nv_bfloat16* src, lo
 cudaError_t launch_paged_evict(cudaStream_t stream, const PagedEvict& a, int* err_word) {
   const unsigned heads = static_cast<unsigned>(a.B * a.pool.Hkv);
   if (heads == 0) return cudaSuccess;
-  // weights in registers as far as they go
+  // Weights in registers as far as they go without spilling, then in shared memory:
+  // for 12 heads of 16000 keys cut to 2000 16.6 us (32 a thread: 42.0), of 24000
+  // 22.9 (42.5, from L2 41.0), of 32000 cut to 4000 48.2 (49.6, from L2 62.7).
   const long long cap = static_cast<long long>(a.pool.max_pages) * a.pool.page_size;
   cudaError_t e;
   // One launch, each block moving its head's rows, but where that leaves SMs idle:
@@ -386,8 +409,12 @@ cudaError_t launch_paged_evict(cudaStream_t stream, const PagedEvict& a, int* er
     e = launch_select<256, 4>(stream, a, heads, err_word);
   else if (cap <= 8192)
     e = launch_select<512, 16>(stream, a, heads, err_word);
-  else if (cap <= 32768)
-    e = launch_select<1024, 32>(stream, a, heads, err_word);
+  else if (cap <= 16384)
+    e = launch_select<1024, 16>(stream, a, heads, err_word);
+  else if (cap <= 24576)
+    e = launch_select<1024, 24>(stream, a, heads, err_word);
+  else if (cap <= kMaxShared)
+    e = launch_select<1024, 0, false, true>(stream, a, heads, err_word);
   else
     e = launch_select<1024, 0>(stream, a, heads, err_word);
   if (e != cudaSuccess) return e;

@@ -450,11 +450,11 @@ def choose(w, L, budget, sinks, recent):
     return np.concatenate([np.arange(sinks), best, np.arange(L - recent, L)])
 
 
-def run_evict(lens, Hkv, page, budget, sinks, recent, change=None, seed=0):
+def run_evict(lens, Hkv, page, budget, sinks, recent, change=None, seed=0, full=False):
     ops = _ops()
     B = len(lens)
     out_pages = -(-budget // page)
-    c = Cache(lens, Hkv, page, seed=seed, spare=B * (out_pages + 1))
+    c = Cache(lens, Hkv, page, seed=seed, spare=B * (out_pages + 1), extra_pages=0 if full else 2)
     w = torch.rand((B, Hkv, c.max_pages * page + 5), generator=c.g, device=DEV) ** 4
     w = torch.where(w < 0.05, torch.floor(w * 256) / 256, w)      # ties
     if change is not None:
@@ -510,6 +510,14 @@ def test_evict_few_and_many_heads(lens, Hkv, budget):
     """Heads that leave SMs idle, fill them once or several times over, with one
     block a head and with two launches."""
     run_evict(lens, Hkv, 16, budget, 4, budget // 8, seed=budget)
+
+
+@pytest.mark.parametrize("cap, budget", [(8192, 700), (16384, 3000), (24576, 500), (30000, 9000),
+                                         (55296, 4000), (55328, 4000)])
+def test_evict_where_the_weights_are_kept(cap, budget):
+    """Capacities up to the last position of each place for the weights, the
+    longest sequence filling it."""
+    run_evict([cap, cap - 33, budget + 1, 5], 2, 32, budget, 4, budget // 8, seed=cap, full=True)
 
 
 def test_evict_ties_and_unusual_weights():
