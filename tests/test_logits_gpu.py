@@ -277,3 +277,11 @@ def test_histories_of_different_tokens(V, n_hist):
     d = lambda a: torch.from_numpy(a).to(DEV)
     y, idx = _ops().logits_penalty(x, history=d(hist), repetition=d(rep), frequency=d(freq), out_dtype=torch.float32)
     check(y, idx, want, tol)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows, V, pad", [(3, 8191, 1), (5, 9001, 47), (2, 5, 2), (300, 2050, 3)])
+def test_padded_logits_and_a_tight_output(dtype, out_dtype, rows, V, pad):
+    """Rows whose place within 16 bytes differs between input and output."""
+    run(rows, V, 50, 5, True, dtype, out_dtype, seed=V, pad=pad, lens=True)
