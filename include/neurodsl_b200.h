@@ -523,7 +523,8 @@ int nd_paged_decode_workspace_size(int B, int H, int Hkv, int64_t max_len, int D
  *   window > 0: key j is seen when j >= lens[b] - window or j < sinks; 0: all.
  *   Pages without a visible key are not read, and their table entries may
  *   hold anything.
- *   out [B][H][64] in o_dtype; lse [B][H] fp32 or NULL.
+ *   out [B][H][64] in o_dtype; lse [B][H] fp32 or NULL.  A NaN or +inf among a
+ *   head's scores, or nothing above -inf, makes its row NaN.
  *   weights [B][Hkv][weights_ld] fp32 or NULL: weights[b][h][j] += the sum over
  *   the group's query heads of exp(s_j - lse), for every visible key j
  *   (weights_ld >= max_pages * page_size) — what nd_paged_kv_evict goes by.

@@ -7,7 +7,8 @@
 // j >= L - window or j < sinks (window 0: every j < L).  Per query head:
 //   s_j = scale * q.k_j,  out = sum_j exp(s_j - lse) v_j,
 //   lse = log sum_j exp(s_j)  over the visible j;
-// no visible key (L = 0) gives out = 0 and lse = -inf.
+// no visible key (L = 0) gives out = 0 and lse = -inf.  A score that is NaN or
+// +inf leaves no number in its head's row, as in the formula.
 //
 // Bound: HBM, 256 bytes per visible key and kv head (K and V rows of 64
 // bf16), each read once for all the query heads of the group.
@@ -650,7 +651,9 @@ __global__ void __launch_bounds__(Shape<kRows, kTma>::kThreads, Shape<kRows, kTm
     }
     named_bar_sync(1, kConsumers);
     const bool whole = head_start >= lo && head_end <= hi;
-    // The warps' shares of value d of row r, joined.
+    // The warps' shares of value d of row r, joined.  A share without a key above
+    // -inf has max -inf and sum 0 and is left out; one whose scores are NaN has
+    // that max too, but a sum that is NaN and has to come through.
     auto joined = [&](int r, int d, float& mm, float& ll, float& oo) {
       mm = -INFINITY;
 #pragma unroll
@@ -659,8 +662,8 @@ __global__ void __launch_bounds__(Shape<kRows, kTma>::kThreads, Shape<kRows, kTm
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         const float x = sm_m[w][r];
-        const float f = x == -INFINITY ? 0.f : fast_exp2(x - mm);
-        if (x != -INFINITY) {   // a share without keys may not even be written
+        const float f = fast_exp2(x - mm);
+        if (x != -INFINITY || sm_l[w][r] != 0.f) {   // values of a share left out may not even be written
           ll += sm_l[w][r] * f;
           oo += sm_o[w][r][d] * f;
         }
@@ -672,13 +675,13 @@ __global__ void __launch_bounds__(Shape<kRows, kTma>::kThreads, Shape<kRows, kTm
         float mm, ll, oo;
         joined(r, d, mm, ll, oo);
         const size_t row = static_cast<size_t>(c.b) * p.H + head0 + r;
-        const float y = ll > 0.f ? oo / ll : 0.f;
+        const float y = c.s.L > 0 ? oo / ll : 0.f;
         if constexpr (kOutF32)
           static_cast<float*>(p.out)[row * kD + d] = y;
         else
           static_cast<__nv_bfloat16*>(p.out)[row * kD + d] = __float2bfloat16_rn(y);
         if (d == 0) {
-          const float lse2 = ll > 0.f ? mm + log2f(ll) : -INFINITY;
+          const float lse2 = mm + log2f(ll);   // no key: -inf
           if (p.lse) p.lse[row] = lse2 * kLn2;
           if (p.scores) p.lse2[row] = lse2;
         }
@@ -739,8 +742,8 @@ __global__ void __launch_bounds__(Shape<kRows, kTma>::kThreads, Shape<kRows, kTm
             float top = mm;
 #pragma unroll
             for (int u = 0; u < 8; ++u) top = fmaxf(top, pm[u]);
-            if (top == -INFINITY) continue;
-            const float a = fast_exp2(mm - top);
+            const float base = top == -INFINITY ? 0.f : top;   // sums that are NaN stay so
+            const float a = fast_exp2(mm - base);
             ll *= a;
             oo.x *= a;
             oo.y *= a;
@@ -748,7 +751,7 @@ __global__ void __launch_bounds__(Shape<kRows, kTma>::kThreads, Shape<kRows, kTm
             oo.w *= a;
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
-              const float f = fast_exp2(pm[u] - top);
+              const float f = fast_exp2(pm[u] - base);
               ll += pl[u] * f;
               oo.x += po[u].x * f;
               oo.y += po[u].y * f;
@@ -759,8 +762,10 @@ __global__ void __launch_bounds__(Shape<kRows, kTma>::kThreads, Shape<kRows, kTm
           }
           *reinterpret_cast<float4*>(&sm_o[share][r][4 * l16]) = oo;
           if (l16 == 0) {
-            sm_l[share][r] = ll;
-            for (int w = share; w < kWarps; w += shares) sm_m[w][r] = w == share ? mm : -INFINITY;
+            for (int w = share; w < kWarps; w += shares) {
+              sm_m[w][r] = w == share ? mm : -INFINITY;
+              sm_l[w][r] = w == share ? ll : 0.f;
+            }
           }
         }
         named_bar_sync(1, kConsumers);

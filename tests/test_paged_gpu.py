@@ -637,3 +637,91 @@ def test_store_then_contiguous_decode_with_programmatic_launch():
             torch.cuda.synchronize()
             want = ops.kv_decode_attn(q, kc, vc, S)
         assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+
+
+def spoil(what, c, q):
+    """Numbers that are not finite in places that are seen."""
+    b = len(c.lens_list) - 1
+    L = c.lens_list[b]
+
+    def keys(first, n, value):
+        for j in range(first, first + n):
+            c.k[int(c.table[b, j // c.page]), 0, j % c.page, 0] = value
+    if what == "one query":
+        q[b, 0, 5] = math.nan
+    elif what == "one key":
+        keys(L - 2, 1, math.nan)
+    elif what == "first key":
+        keys(0, 1, math.nan)
+    elif what == "sixteen keys":       # all that one warp sees of a tile
+        keys(16, 16, math.nan)
+    elif what == "every key":
+        keys(0, L, math.nan)
+    elif what == "a tile and more":
+        keys(64, 80, math.nan)
+    elif what == "infinite key":       # +inf for the heads above zero there, -inf (weight 0) for the others
+        keys(20, 1, math.inf)
+    elif what == "infinite query":
+        q[b, 1, 0] = math.inf
+    else:                              # every score of every head -inf
+        q[b, :, 0] = 1.0
+        keys(0, L, -math.inf)
+
+
+@pytest.mark.parametrize("what", ["one query", "one key", "first key", "sixteen keys", "every key", "a tile and more",
+                                  "infinite key", "infinite query", "nothing left"])
+@pytest.mark.parametrize("lens, H, page", [([0, 200], 2, 16), ([300, 5000], 4, 16), ([40, 9000], 18, 20)])
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32])
+def test_scores_that_are_not_finite_are_not_lost(what, lens, H, page, out_dtype):
+    """By the definition a NaN among the scores, or +inf, or nothing above -inf,
+    leaves no number in the row (lse: NaN, and -inf for the last); a key of -inf
+    among others weighs nothing.  Only a sequence without keys is zeros."""
+    ops = _ops()
+    Hkv = 2
+    G = H // Hkv
+    c = Cache(lens, Hkv, page, seed=5)
+    q = _randn(_gen(7), len(lens), H, D)
+    spoil(what, c, q)
+    w = torch.rand((len(lens), Hkv, c.max_pages * page), generator=c.g, device=DEV)
+    w0 = w.clone()
+    out, lse = ops.paged_decode_attn(q, c.k, c.v, c.table, c.lens, out_dtype=out_dtype, weights=w)
+    assert ops.device_error() == 0
+    bad_heads = 0
+    for b, L in enumerate(lens):
+        if L == 0:
+            assert (out[b] == 0).all() and (lse[b] == -math.inf).all() and torch.equal(w[b], w0[b])
+            continue
+        for h in range(Hkv):
+            k, v = c.rows(c.k, b, h, L).double(), c.rows(c.v, b, h, L).double()
+            group_bad = False
+            want_w, tol_w = w0[b, h, :L].double(), torch.zeros(L, dtype=torch.float64, device=DEV)
+            for i in range(h * G, (h + 1) * G):
+                s = (q[b, i].double() * k).sum(-1) * 0.125
+                if s.isnan().any() or (s == math.inf).any():
+                    assert out[b, i].isnan().all() and lse[b, i].isnan(), (b, i)
+                    group_bad = True
+                    continue
+                seen = s > -math.inf
+                if not seen.any():
+                    assert out[b, i].isnan().all() and lse[b, i] == -math.inf, (b, i)
+                    group_bad = True
+                    continue
+                l = torch.logsumexp(s, -1)
+                p = torch.exp(s - l)
+                ref, A = p @ v, p @ v.abs()
+                E1 = (66 * 2.0**-24 * 0.125 * (q[b, i].double().abs() * k[seen].abs()).sum(-1).max()
+                      + 2.0**-22 * s[seen].abs().max()).item()
+                E = E1 + (L + 32) * 2.0**-23
+                tol = 3 * E * A
+                if out_dtype == torch.bfloat16:
+                    tol = tol + 2.0**-8 * (A + ref.abs()) * (1 + 2.0**-6)
+                assert ((out[b, i].double() - ref).abs() <= tol).all(), (b, i)
+                assert (lse[b, i].double() - l).abs() <= 2 * E + 2.0**-22 * (1 + l.abs()), (b, i)
+                want_w, tol_w = want_w + p, tol_w + 3 * E * p
+            bad_heads += group_bad
+            if group_bad:
+                assert w[b, h, :L].isnan().all(), (b, h)
+            else:
+                assert ((w[b, h, :L].double() - want_w).abs() <= tol_w + 2.0**-23 * want_w.abs()).all(), (b, h)
+            assert torch.equal(w[b, h, L:], w0[b, h, L:])
+    assert bad_heads >= 1 or what == "infinite key"      # there it is for the signs of q
