@@ -561,7 +561,8 @@ int nd_paged_kv_store(void *stream, const void *src, int64_t ld, int k_col, int 
  *   weights_out [B][Hkv][weights_out_ld] fp32, weights_out_ld >= budget: the
  *   kept keys' weights, then zeros; may not overlap weights.
  *   kept [B][Hkv][budget] int32: the positions that stay, then -1.
- *   new_lens [B] int32: min(lens[b], budget).
+ *   new_lens [B] int32: min(lens[b], budget); may be lens itself, and may not
+ *   overlap it otherwise.
  *   budget >= 1, sinks + recent <= budget <= max_out_pages * page_size.
  */
 int nd_paged_kv_evict(void *stream, void *k_pages, void *v_pages, int n_pages, int page_size,

@@ -1327,6 +1327,8 @@ __attribute__((visibility("default"))) int nd_paged_kv_evict(
   const float* wo_end = weights_out + static_cast<size_t>(B) * Hkv * weights_out_ld;
   if (weights_out < w_end && weights < wo_end)
     return fail(ND_ERR_INVALID_ARG, "%s: weights_out overlaps weights", fn);
+  if (new_lens != lens && new_lens < lens + B && lens < new_lens + B)
+    return fail(ND_ERR_INVALID_ARG, "%s: new_lens may be lens, but not overlap it otherwise", fn);
   rc = check_current_device(nullptr);
   if (rc) return rc;
   nd::PagedEvict a = {};

@@ -142,6 +142,12 @@ __device__ __forceinline__ void gather_rows(const PagedEvict& a, int b, int h, i
   }
 }
 
+// A length between 0 and what the table holds.
+__device__ __forceinline__ int cut(const PagedEvict& a, int L) {
+  const long long cap = static_cast<long long>(a.pool.max_pages) * a.pool.page_size;
+  return L < 0 ? 0 : L > cap ? static_cast<int>(cap) : L;
+}
+
 // One block per (sequence, kv head): which positions stay.  The first `sinks`
 // and the last `recent` always do; the rest of the budget goes to the largest
 // weights between, the lowest positions first among equals.  The weights stay in
@@ -156,7 +162,8 @@ __device__ __forceinline__ void gather_rows(const PagedEvict& a, int b, int h, i
 // keys, against 16.5 with these.)
 //
 // kGather: the block then moves its rows itself (the launcher's rule), from the
-// positions left in the histogram's memory.
+// positions left in the histogram's memory, and writes the new length, which is
+// then not where the other heads' blocks read the old one.
 template <int kThreads, int kR, bool kGather, bool kShared>
 __global__ void __launch_bounds__(kThreads, kThreads < 1024 ? 2 : 1)
     paged_select_kernel(const PagedEvict a, int* __restrict__ err_word) {
@@ -176,7 +183,7 @@ __global__ void __launch_bounds__(kThreads, kThreads < 1024 ? 2 : 1)
   int L = a.lens[b];
   if (L < 0 || L > cap) {
     if (threadIdx.x == 0) raise(err_word);
-    L = L < 0 ? 0 : static_cast<int>(cap);
+    L = cut(a, L);
   }
   const float* w = a.weights + static_cast<size_t>(blockIdx.x) * a.weights_ld;
   float* w_out = a.weights_out + static_cast<size_t>(blockIdx.x) * a.weights_out_ld;
@@ -342,9 +349,11 @@ __global__ void __launch_bounds__(kThreads, kThreads < 1024 ? 2 : 1)
   } else {
     for (long long i = z + threadIdx.x; i < a.weights_out_ld; i += kThreads) w_out[i] = 0.f;
   }
-  if (h == 0 && threadIdx.x == 0) a.new_lens[b] = n;
+  if (kGather && h == 0 && threadIdx.x == 0) a.new_lens[b] = n;
 }
 
+// The rows of all heads, and the new lengths: every selection has read the old ones
+// by now, so they may be written in their place.
 __global__ void __launch_bounds__(256)
     paged_gather_kernel(const PagedEvict a, int* __restrict__ err_word) {
   pdl_wait();
@@ -353,8 +362,9 @@ __global__ void __launch_bounds__(256)
   const long long bh = w / per_head;
   if (bh >= static_cast<long long>(a.B) * a.pool.Hkv) return;
   const int slot = static_cast<int>(w - bh * per_head) * 32 + (threadIdx.x & 31);
-  gather_rows(a, static_cast<int>(bh / a.pool.Hkv), static_cast<int>(bh % a.pool.Hkv), slot,
-              slot < a.budget ? a.kept[bh * a.budget + slot] : -1, err_word);
+  const int b = static_cast<int>(bh / a.pool.Hkv), h = static_cast<int>(bh % a.pool.Hkv);
+  if (h == 0 && slot == 0) a.new_lens[b] = min(cut(a, a.lens[b]), a.budget);   // one thread a sequence
+  gather_rows(a, b, h, slot, slot < a.budget ? a.kept[bh * a.budget + slot] : -1, err_word);
 }
 
 template <int kThreads, int kR, bool kGather = false, bool kShared = false>
@@ -399,8 +409,9 @@ cudaError_t launch_paged_evict(cudaStream_t stream, const PagedEvict& a, int* er
   // of 8192: 12.0 against 12.9; 1024 of 8192: 14.9 against 13.1, with 144 heads 24.7
   // against 27.1, with 240 35.8 against 40.3, with 320 51.5 against 54.0 but 2048 of
   // them 86.9 against 81.0, with 512 67.3 against 76.6.
+  // Lengths that are written in place take two launches.
   const unsigned sms = static_cast<unsigned>(current_sm_count());
-  if (cap <= 8192 && a.budget <= 2048 && (heads > sms / 2 || a.budget <= 512) && (heads <= 2 * sms || heads > 3 * sms)) {
+  if (a.new_lens != a.lens && cap <= 8192 && a.budget <= 2048 && (heads > sms / 2 || a.budget <= 512) && (heads <= 2 * sms || heads > 3 * sms)) {
     if (cap <= 1024) return launch_select<512, 2, true>(stream, a, heads, err_word);
     return heads <= sms ? launch_select<1024, 8, true>(stream, a, heads, err_word)
                         : launch_select<512, 16, true>(stream, a, heads, err_word);

@@ -61,7 +61,7 @@ struct PagedEvict {
   float* weights_out;           // [B][Hkv][weights_out_ld]
   long long weights_out_ld;
   int* kept;                    // [B][Hkv][budget]
-  int* new_lens;                // [B]
+  int* new_lens;                // [B], may be lens
 };
 cudaError_t launch_paged_evict(cudaStream_t stream, const PagedEvict& a, int* err_word);
 

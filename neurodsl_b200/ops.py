@@ -847,6 +847,8 @@ def paged_kv_evict(k_pages, v_pages, block_table, lens, weights, out_table, budg
     out_table's pages, which must be none of the source pages.
 
     weights [B][Hkv][keys] fp32 as paged_decode_attn accumulates them.
+    new_lens may be `lens` itself.
+
     Returns (kept [B][Hkv][budget] int32 positions, -1 past the last;
     new_lens [B]; weights_out [B][Hkv][keys], the kept keys' weights first,
     zeros behind them)."""

@@ -725,3 +725,30 @@ def test_scores_that_are_not_finite_are_not_lost(what, lens, H, page, out_dtype)
                 assert ((w[b, h, :L].double() - want_w).abs() <= tol_w + 2.0**-23 * want_w.abs()).all(), (b, h)
             assert torch.equal(w[b, h, L:], w0[b, h, L:])
     assert bad_heads >= 1 or what == "infinite key"      # there it is for the signs of q
+
+
+@pytest.mark.parametrize("lens, Hkv, budget", [([500, 300, 40], 2, 100), ([700] * 5, 70, 300), ([900, 20, 1100], 300, 200),
+                                               ([5000, 9000], 3, 2500), ([-4, 10**8, 77], 90, 30)])
+def test_evict_writes_the_lengths_in_place(lens, Hkv, budget):
+    """new_lens = lens: every head of a sequence goes by the old length."""
+    ops = _ops()
+    page, B = 16, len(lens)
+    fit = [1200 if L > 10**6 else max(L, 0) for L in lens]
+    out_pages = -(-budget // page)
+    c = Cache(fit, Hkv, page, seed=budget, spare=B * out_pages, extra_pages=0)
+    c.lens = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    w = torch.rand((B, Hkv, c.max_pages * page), generator=c.g, device=DEV)
+    ot = torch.tensor(c.free[:B * out_pages], dtype=torch.int32, device=DEV).view(B, out_pages)
+    k0, v0 = c.k.clone(), c.v.clone()
+    want = ops.paged_kv_evict(c.k, c.v, c.table, c.lens, w, ot, budget, sinks=2, recent=9)
+    ops.device_error()
+    k1, v1 = c.k.clone(), c.v.clone()
+    c.k.copy_(k0)
+    c.v.copy_(v0)
+    got = ops.paged_kv_evict(c.k, c.v, c.table, c.lens, w, ot, budget, sinks=2, recent=9, new_lens=c.lens)
+    assert got[1] is c.lens and torch.equal(c.lens, want[1])
+    assert c.lens.tolist() == [min(L, budget) for L in fit]
+    assert torch.equal(got[0], want[0]) and torch.equal(got[2], want[2])
+    assert torch.equal(c.k.view(torch.int16), k1.view(torch.int16))
+    assert torch.equal(c.v.view(torch.int16), v1.view(torch.int16))
+    assert ops.device_error() == (16 if lens != fit else 0)

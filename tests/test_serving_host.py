@@ -194,3 +194,16 @@ def test_the_calls_extension_leaves_everything_uncommon_to_the_checks():
         assert fn() is None and fn(*[host] * (n + 1)) is None
     with pytest.raises(TypeError):
         calls.bind(1, 2)
+
+
+def test_paged_evict_refuses_lengths_that_overlap():
+    """Lengths written over others that are still to be read; the same lengths in
+    place are fine (here: as far as the missing device)."""
+    m, lib = _lib()
+    at = lambda i: ctypes.c_void_p(0x300000 + 4 * i)  # noqa: E731
+    for i in (1, -1):
+        assert evict(lib, lens=at(0), new_lens=at(i)) == m.ND_ERR_INVALID_ARG
+        assert b"new_lens" in lib.nd_last_error_string()
+    for i in (0, 2, -2):
+        evict(lib, lens=at(0), new_lens=at(i), D=64, kept=None)      # refused for kept alone
+        assert b"new_lens" not in lib.nd_last_error_string()
