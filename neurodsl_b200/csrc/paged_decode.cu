@@ -56,6 +56,7 @@
 #include "model_ops.h"
 #include "paged_kv.h"
 #include "ptx.cuh"
+#include "ring.cuh"
 #include "tma.h"
 
 namespace nd {
@@ -86,7 +87,6 @@ constexpr int kPartialRow = kD + 4;             // acc[64], max, sum (16-byte ro
 constexpr int kHeadCost = 3;                    // what a head costs beside its tiles, in tiles
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr int kDevErrTimeoutPaged = 6;          // a tile did not arrive in time
 
 struct Params {
   const __nv_bfloat16* q;
@@ -117,6 +117,7 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool t
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n)
                : "memory");
 }
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 // This thread's copies so far arrive on `bar` when they have landed.
 __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -329,14 +330,7 @@ __device__ __forceinline__ void produce(const Params& p, const CUtensorMap* tm_k
   look_up(c);
   uint64_t policy = 0;
   if constexpr (kTma) asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
-  bool ok = true;
-  int it = 0;
-  for (; at < hi; ++it) {
-    const int s = it % kStages;
-    if (it >= kStages && !warp_wait(&bars->empty[s], ((it / kStages) - 1) & 1, abort_flag)) {
-      ok = false;
-      break;
-    }
+  auto fill = [&](int s) {
     uint8_t* dst = ring + s * kStageBytes;
     if constexpr (kTma) {
       const bool go = row != -2;
@@ -365,13 +359,16 @@ __device__ __forceinline__ void produce(const Params& p, const CUtensorMap* tm_k
     }
     at += next_tile(p, heads, c);
     if (at < hi) look_up(c);
-  }
-  if (!ok) {
-    raise_abort(abort_flag, p.err_word, kDevErrTimeoutPaged);
-    // what was issued lands before the CTA may exit
-    for (int i = it > kStages ? it - kStages : 0; i < it; ++i)
-      (void)warp_wait(&bars->full[i % kStages], (i / kStages) & 1, abort_flag);
-  }
+  };
+  ring_produce<kStages>(
+      [&]() { return at < hi; },
+      [&](int s, uint32_t parity) { return warp_wait(&bars->empty[s], parity, abort_flag); }, fill,
+      [&]() { raise_abort(abort_flag, p.err_word, kDevErrTimeoutPaged); },
+      [&](int s, uint32_t parity) {
+        // the pieces by thread: another warp's may never have been sent off
+        if constexpr (kTma) mbar_landed(&bars->full[s], parity);
+        else cp_async_wait_all();
+      });
 }
 
 template <int kRows, bool kOutF32, bool kTma>
@@ -446,7 +443,7 @@ __global__ void __launch_bounds__(Shape<kRows, kTma>::kThreads, Shape<kRows, kTm
     }
   };
   load_q(c.b, c.hp);
-  bool ok = true;          // after a lost tile the rest runs on without waiting
+  bool ok = true;          // no tile has failed to come
   int it = 0;              // tiles taken from the ring
   long long at = lo;
   long long head_start = lo - c.j;
@@ -491,7 +488,12 @@ __global__ void __launch_bounds__(Shape<kRows, kTma>::kThreads, Shape<kRows, kTm
       const uint32_t off = st * kStageBytes;
       const int key0 = c.key_tile() * kTile + warp * kKeysPerWarp;
       if (k + 1 < n) ++c.j;
-      ok = ok && warp_wait(&bars.full[st], (it / kStages) & 1, abort_flag);
+      if (!ring_take<kStages>(
+              ok, it, [&](int s, uint32_t parity) { return warp_wait(&bars.full[s], parity, abort_flag); },
+              [&]() { raise_abort(abort_flag, p.err_word, kDevErrTimeoutPaged); })) {
+        it += n - k;
+        break;
+      }
       const bool full = all_visible(p, c.s, key0, kKeysPerWarp);
       const int fresh = c.s.L - 1 - key0;          // the new token's row of the 16
       const bool app = append && fresh >= 0 && fresh < kKeysPerWarp;
@@ -632,6 +634,12 @@ __global__ void __launch_bounds__(Shape<kRows, kTma>::kThreads, Shape<kRows, kTm
       }
     }
     at = seg_end;
+    // a head that lacks a tile has no result: NaN through all joins, which go on so
+    // that the workspace stays as it has to be
+    if (!ok) {
+#pragma unroll
+      for (int r = 0; r < kR; ++r) l[r] = __int_as_float(0x7fffffff);
+    }
 
     // ---- the head's end in this range: join the warps
     named_bar_sync(1, kConsumers);   // the previous head's readers are done

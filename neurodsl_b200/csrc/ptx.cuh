@@ -29,6 +29,7 @@ enum DeviceError : int {
   kDevErrTimeoutSoftmax = 3,
   kDevErrTimeoutEpilogue = 4,
   kDevErrTimeoutComm = 5,       // a peer rank's flag did not arrive in time
+  kDevErrTimeoutPaged = 6,      // a tile of the paged decode did not arrive in time
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
@@ -132,6 +133,14 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity,
       if (globaltimer() - t0 > ND_WAIT_TIMEOUT_NS) return false;
     }
   }
+}
+
+// Bounded wait for this role's own copies before the block may end: also after
+// another role has given up.
+__device__ __forceinline__ void mbar_landed(uint64_t* bar, uint32_t parity) {
+  const uint64_t t0 = globaltimer();
+  for (uint32_t it = 1; !mbar_try_wait(bar, parity); ++it)
+    if ((it & 31u) == 0 && globaltimer() - t0 > ND_WAIT_TIMEOUT_NS) return;
 }
 
 // Bounded wait by a full warp, with a warp-uniform result and the warp
