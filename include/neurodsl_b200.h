@@ -519,7 +519,8 @@ int nd_paged_decode_workspace_size(int B, int H, int Hkv, int64_t max_len, int D
  *   included; 0: a row of zeros with lse -inf.
  *   k_new, v_new [B][Hkv][64] bf16 or both NULL: the token at position
  *   lens[b] - 1, used for that key and written into its page (which no other
- *   sequence may read or write in the same call).
+ *   sequence may read or write in the same call).  A kernel behind such a call
+ *   starts when it has ended, whatever nd_set_pdl says.
  *   window > 0: key j is seen when j >= lens[b] - window or j < sinks; 0: all.
  *   Pages without a visible key are not read, and their table entries may
  *   hold anything.

@@ -399,7 +399,10 @@ __global__ void __launch_bounds__(Shape<kRows, kTma>::kThreads, Shape<kRows, kTm
     tma_prefetch_desc(&tm_v);
   }
   pdl_wait();
-  pdl_trigger();
+  // A call that appends writes the cache, and the contiguous decode attention, with
+  // programmatic launch on, reads cached rows before it waits: what follows starts
+  // when this kernel is done.
+  if (p.k_new == nullptr) pdl_trigger();
   __syncthreads();
 
   Cursor c;

@@ -752,3 +752,32 @@ def test_evict_writes_the_lengths_in_place(lens, Hkv, budget):
     assert torch.equal(c.k.view(torch.int16), k1.view(torch.int16))
     assert torch.equal(c.v.view(torch.int16), v1.view(torch.int16))
     assert ops.device_error() == (16 if lens != fit else 0)
+
+
+@pytest.mark.parametrize("with_weights", [False, True])
+def test_append_then_contiguous_decode_with_programmatic_launch(with_weights):
+    """The row that a paged decode appends is one of those that a contiguous decode
+    right behind it reads before it waits."""
+    ops = _ops()
+    g = _gen(6)
+    B, H, L_max, L = 8, 12, 2048, 2000
+    kc, vc = _randn(g, B, H, L_max, D), _randn(g, B, H, L_max, D)
+    table = torch.arange(B, dtype=torch.int32, device=DEV)[:, None].contiguous()
+    lens = torch.full((B,), L, dtype=torch.int32, device=DEV)
+    q, kn, vn = _randn(g, B, H, D), 4 * _randn(g, B, H, D), 4 * _randn(g, B, H, D)
+    q2 = kn.clone()          # attends mostly to the appended row
+    ws = ops.paged_decode_workspace(B, H, H, L_max, weights=with_weights)
+    w = torch.zeros((B, H, L_max), device=DEV) if with_weights else None
+    want = None
+    for _ in range(5):
+        kc[:, :, L - 1] = 0
+        vc[:, :, L - 1] = 0
+        with ops.pdl(True):
+            ops.paged_decode_attn(q, kc, vc, table, lens, k_new=kn, v_new=vn, weights=w, workspace=ws)
+            out, lse = ops.kv_decode_attn(q2, kc, vc, L + 1)
+        if want is None:
+            torch.cuda.synchronize()
+            assert torch.equal(kc[:, :, L - 1], kn) and torch.equal(vc[:, :, L - 1], vn)
+            want = ops.kv_decode_attn(q2, kc, vc, L + 1)
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+    assert ops.device_error() == 0
