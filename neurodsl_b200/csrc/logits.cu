@@ -237,12 +237,17 @@ __global__ void __launch_bounds__(kThreads, 4)
         n_hist = n_hist < 0 ? 0 : a.n_history;
       }
       // The first to enter a token sends for the word that holds its logit and
-      // takes it off the map.
+      // takes it off the map.  Half a word beyond an end of the row is none of the
+      // caller's: there the two bytes alone are read.
       auto enter = [&](int t, bool biased) {
         int s = slot_of(t, table), k;
         while ((k = atomicCAS(&key[s], -1, t)) != -1 && (k & ~kBiased) != t) s = after(s, table);
         if (k == -1) {
-          cp_async4(smem_u32(value + s), reinterpret_cast<const void*>(reinterpret_cast<uintptr_t>(in + t) & ~uintptr_t{3}));
+          const uintptr_t at = reinterpret_cast<uintptr_t>(in + t);
+          if (sizeof(TI) == 2 && (at & 2 ? t == 0 : t == a.V - 1))
+            value[s] = static_cast<uint32_t>(*reinterpret_cast<const unsigned short*>(at)) << (at & 2 ? 16 : 0);
+          else
+            cp_async4(smem_u32(value + s), reinterpret_cast<const void*>(at & ~uintptr_t{3}));
           const uint32_t bit = 1u << (t & 31);
           if (!(atomicAnd(&bits[(t >> 5) - w0], ~bit) & bit)) atomicAdd(&count[s], kForbidden);
         }

@@ -285,3 +285,27 @@ def test_histories_of_different_tokens(V, n_hist):
 def test_padded_logits_and_a_tight_output(dtype, out_dtype, rows, V, pad):
     """Rows whose place within 16 bytes differs between input and output."""
     run(rows, V, 50, 5, True, dtype, out_dtype, seed=V, pad=pad, lens=True)
+
+
+@pytest.mark.parametrize("dtype, out_dtype, in_place", [
+    (torch.bfloat16, torch.bfloat16, False), (torch.bfloat16, torch.bfloat16, True),
+    (torch.bfloat16, torch.float32, False), (torch.float32, torch.bfloat16, False)])
+@pytest.mark.parametrize("V", [1, 2, 3, 8, 33, 4097])
+def test_listed_tokens_at_the_ends_of_a_row(dtype, out_dtype, in_place, V):
+    """Wherever in a word the row begins and ends; what lies beside it is none of
+    the call's."""
+    rng = np.random.default_rng(V)
+    ids = np.array([[0, V - 1]], np.int32)
+    hist = np.array([[V - 1, 0, V - 1]], np.int32)
+    bias, freq = np.array([[1.5, -2.5]], np.float32), np.full(1, 0.25, np.float32)
+    d = lambda a: torch.from_numpy(a).to(DEV)
+    for first in range(4):
+        buf = torch.full((first + V + 4,), math.nan, device=DEV).to(dtype)
+        x = buf[first:first + V].view(1, V)
+        x.copy_(torch.from_numpy(rng.standard_normal((1, V)).astype(np.float32)))
+        want, tol = reference(x.float().cpu().numpy(), hist, None, None, None, freq, ids, bias, None)
+        out, idx = _ops().logits_penalty(x, history=d(hist), frequency=d(freq), bias_ids=d(ids), bias=d(bias),
+                                         out=x if in_place else None, out_dtype=out_dtype)
+        check(out, idx, want, tol)
+        assert buf[:first].isnan().all() and buf[first + V:].isnan().all()
+    assert _ops().device_error() == 0
