@@ -586,6 +586,7 @@ int nd_paged_kv_evict(void *stream, void *k_pages, void *v_pages, int n_pages, i
  *   otherwise.
  *   history [rows][history_ld] int32 or NULL: n_history entries a row, the
  *   first history_lens[row] of them used (NULL: all), negative ones skipped.
+ *   With n_history 0 the pointer is not read; NULL takes no penalties.
  *   repetition (> 0), presence, frequency [rows] fp32 or NULL (left out).
  *   bias_ids, bias [rows][n_bias] or both NULL: negative ids are skipped, a
  *   token listed twice takes both biases.

@@ -1408,9 +1408,9 @@ __attribute__((visibility("default"))) int nd_logits_penalty(
   a.ld = ld;
   a.rows = rows;
   a.V = V;
-  a.history = n_history > 0 ? history : nullptr;
+  a.history = history;
   a.history_ld = history_ld;
-  a.n_history = n_history;
+  a.n_history = history != nullptr ? n_history : 0;
   a.history_lens = history_lens;
   a.repetition = repetition;
   a.presence = presence;

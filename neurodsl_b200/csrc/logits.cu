@@ -177,10 +177,10 @@ __global__ void __launch_bounds__(kThreads, 4)
     for (int u = 0; u < 4; ++u) t[u] = i + u * kThreads < n ? list[i + u * kThreads] : -1;
   };
   int th[4], tb[4];
-  read(hist, hist ? a.n_history : 0, threadIdx.x, th);
+  read(hist, a.n_history, threadIdx.x, th);
   read(ids, n_bias, threadIdx.x, tb);
-  int n_hist = hist ? a.n_history : 0;
-  if (hist && a.history_lens) n_hist = a.history_lens[row];
+  int n_hist = a.n_history;
+  if (a.history_lens) n_hist = a.history_lens[row];
   float rep = 1.f, pres = 0.f, freq = 0.f;
   if (a.repetition) rep = a.repetition[row];
   if (a.presence) pres = a.presence[row];
@@ -229,13 +229,13 @@ __global__ void __launch_bounds__(kThreads, 4)
       if (i * kThreads < gz - ga - static_cast<int>(threadIdx.x)) next[i].template load<kVec>(src + i * kThreads * kN);
     cp_async_wait_all();
     __syncthreads();
+    if (n_hist < 0 || n_hist > a.n_history) {
+      if (threadIdx.x == 0 && err_word) atomicCAS(err_word, 0, kModelErrIndex);
+      n_hist = n_hist < 0 ? 0 : a.n_history;
+    }
     if (lists) {
       // ---- the listed tokens of the part.  The tables hold more entries than that:
       // the launcher sizes them by the lists, or else by the part.
-      if (n_hist < 0 || n_hist > a.n_history) {
-        if (threadIdx.x == 0 && err_word) atomicCAS(err_word, 0, kModelErrIndex);
-        n_hist = n_hist < 0 ? 0 : a.n_history;
-      }
       // The first to enter a token sends for the word that holds its logit and
       // takes it off the map.  Half a word beyond an end of the row is none of the
       // caller's: there the two bytes alone are read.
@@ -489,7 +489,7 @@ cudaError_t launch_typed(cudaStream_t stream, const LogitsPenalty& a, int* err_w
   // longer than that.  (Small tables leave the L1 cache to the loads in flight:
   // with 26 KB more a row the stream took 27 us for 23.)
   constexpr int kMost = kMaxTable / 4 * 3;
-  const long long n_bias = a.bias_ids ? a.n_bias : 0, n = (a.history ? a.n_history : 0) + n_bias;
+  const long long n_bias = a.bias_ids ? a.n_bias : 0, n = a.n_history + n_bias;
   auto entries = [](long long m) {
     return 2 * m < kMaxTable ? (2 * static_cast<int>(m) + 3) / 4 * 4 : kMaxTable;
   };

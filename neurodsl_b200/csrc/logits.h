@@ -10,9 +10,9 @@ struct LogitsPenalty {
   bool in_f32;
   long long ld;
   int rows, V;
-  const int* history;          // [rows][history_ld] or null; negative: no token
+  const int* history;          // [rows][history_ld]; negative: no token
   long long history_ld;
-  int n_history;
+  int n_history;               // 0 without a history
   const int* history_lens;     // [rows] or null (n_history)
   const float* repetition;     // [rows] or null
   const float* presence;

@@ -293,8 +293,10 @@ PyObject* logits_penalty(PyObject*, PyObject* const* v, Py_ssize_t n) {
     }
     const int r = narrow(rows, a), nv = narrow(V, a), nh = hist == nullptr ? 0 : narrow(hist->size(1), a);
     const int nb = bias == nullptr ? 0 : narrow(bias->size(1), a);
+    // a history without entries has no memory; it is still a history, and not read
+    const void* h = hist != nullptr && nh == 0 ? ptr(x) : ptr(hist);
     return status(a, [&](void* s) {
-      return f_logits(s, ptr(x), dtype(*x), ld, r, nv, ptr<int32_t>(hist), h_ld, nh, ptr<int32_t>(hl), ptr<float>(rep),
+      return f_logits(s, ptr(x), dtype(*x), ld, r, nv, static_cast<const int32_t*>(h), h_ld, nh, ptr<int32_t>(hl), ptr<float>(rep),
                       ptr<float>(pres), ptr<float>(freq), ptr<int32_t>(ids), ptr<float>(bias), nb, ptr<uint32_t>(mask),
                       m_ld, ptr(out), dtype(*out), out_ld, ptr<int32_t>(idx));
     });

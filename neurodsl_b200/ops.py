@@ -907,8 +907,11 @@ def logits_penalty(logits, history=None, history_lens=None, repetition=None, pre
     if out_V != V:
         raise ValueError(f"out must be {(rows, V)}, got {tuple(out.shape)}")
     n_hist = hist_ld = 0
+    hist_addr = None
     if history is not None:
         n_hist, hist_ld = _matrix(history, "history", _INT32, rows, dev)
+        # a history without entries has no memory; it is still a history, and not read
+        hist_addr = history.data_ptr() if n_hist else logits.data_ptr()
     if history_lens is not None:
         _vector(history_lens, "history_lens", _INT32, rows, dev)
     if repetition is not None:
@@ -941,7 +944,7 @@ def logits_penalty(logits, history=None, history_lens=None, repetition=None, pre
     if idx is not None:
         _vector(idx, "idx", _INT32, rows, dev)
     _call(_lib.load().nd_logits_penalty, dev, _stream_of(dev, stream), logits.data_ptr(),
-          _DT[logits.dtype], ld, rows, V, _addr(history), hist_ld, n_hist, _addr(history_lens),
+          _DT[logits.dtype], ld, rows, V, hist_addr, hist_ld, n_hist, _addr(history_lens),
           _addr(repetition), _addr(presence), _addr(frequency), _addr(bias_ids), _addr(bias),
           n_bias, _addr(mask), mask_ld, out.data_ptr(), _DT[out.dtype], out_ld, _addr(idx))
     return out, idx

@@ -309,3 +309,30 @@ def test_listed_tokens_at_the_ends_of_a_row(dtype, out_dtype, in_place, V):
         check(out, idx, want, tol)
         assert buf[:first].isnan().all() and buf[first + V:].isnan().all()
     assert _ops().device_error() == 0
+
+
+@pytest.mark.parametrize("direct", [True, False])
+def test_an_empty_history(monkeypatch, direct):
+    """[rows][0], as before the first token: nothing is penalised; a length that is
+    not 0 is reported like any other outside [0, n]."""
+    from neurodsl_b200 import _lib
+    ops = _ops()
+    if not direct:
+        monkeypatch.setattr(_lib, "calls", False)
+    x = torch.randn((3, 500), device=DEV)
+    empty = torch.empty((3, 0), dtype=torch.int32, device=DEV)
+    half = torch.full((3,), 0.5, device=DEV)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    for lens, code in ((None, 0), (i32([0, 0, 0]), 0), (i32([0, 1, 0]), 16), (i32([-1, 0, 0]), 16)):
+        out, idx = torch.empty_like(x), i32([9, 9, 9])
+        ops.logits_penalty(x, history=empty, history_lens=lens, repetition=1 + half, presence=half, frequency=half,
+                           out=out, idx=idx)
+        assert torch.equal(out, x) and torch.equal(idx.long(), x.argmax(1))
+        assert ops.device_error() == code
+    out, _ = ops.logits_penalty(x, history=empty, presence=half, bias_ids=i32([[7], [8], [9]]), bias=2 * half[:, None])
+    want = x.clone()
+    for r in range(3):
+        want[r, 7 + r] += 1
+    assert torch.equal(out, want)
+    with pytest.raises(RuntimeError):
+        ops.logits_penalty(x, presence=half)
