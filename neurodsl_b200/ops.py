@@ -571,8 +571,10 @@ def add_layernorm(x, p, bias=None, gamma=None, beta=None, eps=1e-5, s_out=None, 
 _BF16, _F32, _INT32 = torch.bfloat16, torch.float32, torch.int32
 _I64x3 = ctypes.c_int64 * 3
 _INT_MAX = 2**31 - 1
-_cuda_device = torch._C._cuda_getDevice          # the current device's number
-_raw_stream = torch._C._cuda_getCurrentRawStream  # a device's current stream as an int
+# the current device's number, a device's current stream as an int (a torch built
+# without CUDA has neither, and no tensor that a call would take)
+_cuda_device = getattr(torch._C, "_cuda_getDevice", None)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _device_of(t, name):

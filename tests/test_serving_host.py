@@ -207,3 +207,26 @@ def test_paged_evict_refuses_lengths_that_overlap():
     for i in (0, 2, -2):
         evict(lib, lens=at(0), new_lens=at(i), D=64, kept=None)      # refused for kept alone
         assert b"new_lens" not in lib.nd_last_error_string()
+
+
+def test_ops_imports_where_torch_was_built_without_cuda():
+    """As before the serving operators: only the calls need a GPU."""
+    import os
+    import subprocess
+    import sys
+    pytest.importorskip("torch")
+    program = """
+import torch
+for name in dir(torch._C):
+    if name.startswith("_cuda_"):
+        delattr(torch._C, name)
+import neurodsl_b200.ops as ops, neurodsl_b200.graph
+try:
+    ops.logits_penalty(torch.zeros(1, 4))
+except TypeError as e:
+    print("refused:", e)
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", program], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr
+    assert "refused: logits must be a CUDA tensor" in r.stdout
