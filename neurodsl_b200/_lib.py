@@ -6,7 +6,9 @@ load, every operation raises; nothing falls back to another implementation.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
+import sys
 import threading
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
@@ -139,15 +141,23 @@ def load(path: str = LIB_PATH):
     return _lib
 
 
+def calls_path():
+    """Where the extension for this interpreter and this torch is: it reads tensors
+    through torch's inline accessors, so its name says which it was built for."""
+    import torch
+    return os.path.join(_PKG, f"_calls.{sys.implementation.cache_tag}.torch-{torch.__version__}.so")
+
+
 def load_calls():
     """The extension that makes the serving operators' calls (csrc/py_calls.cpp)
-    bound to the library's entry points.  False where it was not built or this
-    interpreter's torch cannot load it: the same entry points are then called
-    through ctypes."""
+    bound to the library's entry points.  False where it was not built for this
+    interpreter and torch: the same entry points are then called through ctypes."""
     global calls
     lib = load()
+    spec = importlib.util.spec_from_file_location(__package__ + "._calls", calls_path())
     try:
-        from . import _calls
+        _calls = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(_calls)
     except ImportError:
         calls = False
     else:

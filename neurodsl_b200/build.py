@@ -15,13 +15,15 @@ import os
 import shutil
 import subprocess
 import sys
+import warnings
+
+from . import _lib
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libneurodsl_b200.so")
-CALLS = os.path.join(PKG, "_calls.so")
 SOURCES = ["abi.cu", "tma.cu", "flash_fwd.cu", "kv_decode.cu", "gemm.cu", "layernorm.cu", "model_ops.cu",
            "tp_comm.cu", "elementwise.cu", "paged_decode.cu", "paged_kv.cu", "logits.cu"]
 
@@ -87,29 +89,46 @@ def build(force: bool = False, verbose: bool = False, extra_flags=None) -> str:
     return LIB
 
 
-def build_calls(force: bool = False) -> str:
-    """neurodsl_b200/_calls.so: the CPython extension that makes the serving
-    operators' calls (csrc/py_calls.cpp), against this interpreter and its torch."""
-    src = os.path.join(CSRC, "py_calls.cpp")
-    if not force and not _stale(CALLS, [src, os.path.join(ROOT, "include", "neurodsl_b200.h")]):
-        return CALLS
+def build_calls(force: bool = False):
+    """neurodsl_b200/_calls.<interpreter>.<torch>.so: the CPython extension that
+    makes the serving operators' calls (csrc/py_calls.cpp), against this interpreter
+    and its torch.  None, with a warning, where there is no torch, no C++ compiler or
+    none of their headers: ctypes then makes the calls."""
     import sysconfig
-
-    import torch
-    from torch.utils.cpp_extension import include_paths
+    try:
+        import torch
+        from torch.utils.cpp_extension import include_paths
+    except ImportError as e:
+        return _no_calls(e)
+    target = _lib.calls_path()
+    src = os.path.join(CSRC, "py_calls.cpp")
+    if not force and not _stale(target, [src, os.path.join(ROOT, "include", "neurodsl_b200.h")]):
+        return target
+    cxx = os.environ.get("CXX", "g++")
+    if shutil.which(cxx) is None:
+        return _no_calls(f"no C++ compiler ({cxx})")
+    for header, dirs in (("Python.h", [sysconfig.get_paths()["include"]]),
+                         ("torch/csrc/autograd/python_variable.h", include_paths())):
+        if not any(os.path.exists(os.path.join(d, header)) for d in dirs):
+            return _no_calls(f"no {header}")
     cuda = os.path.dirname(os.path.dirname(nvcc()))
     libs = os.path.join(os.path.dirname(torch.__file__), "lib")
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+    cmd = [cxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            "-I", os.path.join(ROOT, "include"), "-isystem", sysconfig.get_paths()["include"],
            "-isystem", os.path.join(cuda, "include")]
     for d in include_paths():
         cmd += ["-isystem", d]
-    cmd += [src, "-o", CALLS, "-L", libs, "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    cmd += [src, "-o", target, "-L", libs, "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError("building _calls.so failed:\n" + r.stdout + r.stderr)
-    return CALLS
+        raise RuntimeError("building the calls' extension failed:\n" + r.stdout + r.stderr)
+    return target
+
+
+def _no_calls(why):
+    warnings.warn(f"the calls' extension is not built: {why}", stacklevel=3)
+    return None
 
 
 def main():

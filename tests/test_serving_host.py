@@ -230,3 +230,40 @@ except TypeError as e:
     r = subprocess.run([sys.executable, "-c", program], cwd=root, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr
     assert "refused: logits must be a CUDA tensor" in r.stdout
+
+
+def test_the_calls_extension_is_of_this_interpreter_and_torch(monkeypatch, tmp_path):
+    """One built for another torch is neither taken for fresh nor loaded; the calls
+    then go through ctypes."""
+    import sys
+    torch = pytest.importorskip("torch")
+    from neurodsl_b200 import build
+    m, lib = _lib()
+    assert m.load_calls()
+    mine = m.calls_path()
+    assert build.build_calls() == mine
+    monkeypatch.setattr(torch, "__version__", "1.13.0")
+    assert m.calls_path() != mine
+    monkeypatch.setattr(m, "calls", None)
+    assert m.load_calls() is False
+    made = []
+    monkeypatch.setattr(build.subprocess, "run", lambda cmd, **kw: made.append(cmd) or type("R", (), dict(returncode=0)))
+    assert build.build_calls() == m.calls_path()
+    assert len(made) == 1 and m.calls_path() in made[0]
+    monkeypatch.setattr(torch, "__version__", mine.split("torch-")[1][:-3])
+    monkeypatch.setattr(sys.implementation, "cache_tag", "cpython-27")
+    assert m.calls_path() != mine
+
+
+def test_a_build_without_a_compiler_or_headers(monkeypatch):
+    """The library alone is enough: a warning, no error."""
+    pytest.importorskip("torch")
+    import torch.utils.cpp_extension as ext
+    from neurodsl_b200 import build
+    with monkeypatch.context() as c:
+        c.setenv("CXX", "/nowhere/c++")
+        with pytest.warns(UserWarning, match="no C.. compiler"):
+            assert build.build_calls(force=True) is None
+    monkeypatch.setattr(ext, "include_paths", lambda *a, **k: ["/nowhere"])
+    with pytest.warns(UserWarning, match="python_variable.h"):
+        assert build.build_calls(force=True) is None
