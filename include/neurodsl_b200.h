@@ -481,7 +481,8 @@ int nd_gemm_allreduce_add_layernorm(void *stream, const void *A, const void *W, 
  *   Keys and values below Sk have to be finite: a masked one weighs exactly 0,
  *   and 0 times an infinity is NaN.
  *   lse, row_max [B][H][Sq] fp32 or NULL.  The weights are rounded to bf16
- *   for the second product, whatever o_dtype.
+ *   for the second product, some of them twice, whatever o_dtype: an fp32 O is
+ *   within 2^-7 of the sum of weight times |value|.
  */
 int nd_window_attn_fwd(void *stream, const void *Q, const int64_t *q_strides, const void *K,
                        const int64_t *k_strides, const void *V, const int64_t *v_strides, void *O,

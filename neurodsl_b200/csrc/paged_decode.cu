@@ -602,18 +602,21 @@ __global__ void __launch_bounds__(Shape<kRows, kTma>::kThreads, Shape<kRows, kTm
             l[r] += pr;
           }
       }
-      // O^T += V^T P^T.  P goes to the matrix unit in bf16 (relative error
-      // 2^-9 a weight, below the bf16 output's own rounding).  An fp32 output
-      // takes P as three bf16 terms, which carry all 24 bits, and adds each
+      // O^T += V^T P^T.  The matrix unit takes P in bf16: as two terms for a bf16
+      // output (off by 2^-16 of a weight, far below the output's own rounding, as the
+      // contiguous decode's fp32 weights are; one term, off by 2^-8, takes 38.1 us for
+      // 38.3 with 64 ragged sequences, and 38.9 for 39.9 with 16 heads a kv head).
+      // An fp32 output takes three terms, which carry all 24 bits, and adds each
       // step's product in fp32 arithmetic: the matrix unit's own accumulation
       // cuts off low bits, a bias that grows with the number of steps.
-      uint32_t pb[kR][kOutF32 ? 3 : 1][2];
+      constexpr int kTerms = kOutF32 ? 3 : 2;
+      uint32_t pb[kR][kTerms][2];
 #pragma unroll
       for (int r = 0; r < kR; ++r)
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int x = 0; x < (kOutF32 ? 3 : 1); ++x) {
+          for (int x = 0; x < kTerms; ++x) {
             const uint32_t w = pack_bf16x2(sc[t][2 * r], sc[t][2 * r + 1]);
             pb[r][x][t] = w;
             sc[t][2 * r] -= __uint_as_float(w << 16);     // what the rounding left
@@ -626,12 +629,14 @@ __global__ void __launch_bounds__(Shape<kRows, kTma>::kThreads, Shape<kRows, kTm
           if constexpr (kOutF32) {
             float x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int y = 2; y >= 0; --y)
+            for (int y = kTerms - 1; y >= 0; --y)
               mma_bf16(x, vf[i][0], vf[i][1], vf[i][2], vf[i][3], pb[r][y][0], pb[r][y][1]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[r][i][e] += x[e];
           } else {
-            mma_bf16(o[r][i], vf[i][0], vf[i][1], vf[i][2], vf[i][3], pb[r][0][0], pb[r][0][1]);
+#pragma unroll
+            for (int y = kTerms - 1; y >= 0; --y)
+              mma_bf16(o[r][i], vf[i][0], vf[i][1], vf[i][2], vf[i][3], pb[r][y][0], pb[r][y][1]);
           }
         }
       }

@@ -781,3 +781,25 @@ def test_append_then_contiguous_decode_with_programmatic_launch(with_weights):
             want = ops.kv_decode_attn(q2, kc, vc, L + 1)
         assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
     assert ops.device_error() == 0
+
+
+@pytest.mark.parametrize("lens, H, Hkv, page", [([300, 64, 17], 12, 12, 16), ([900, 5000], 8, 2, 64), ([700], 18, 2, 20)])
+def test_bf16_output_is_rounded_once(lens, H, Hkv, page):
+    """A bf16 output keeps its weights to 2^-16 (two bf16 terms, the second of what
+    the first leaves: 2^-8 of 2^-8), as the contiguous decode keeps them in fp32: off by
+    its own rounding and the module's fp32 bounds, however small it is beside sum p |v|."""
+    c = Cache(lens, Hkv, page, seed=3)
+    q = _randn(_gen(2), len(lens), H, D)
+    out, _ = _ops().paged_decode_attn(q, c.k, c.v, c.table, c.lens)
+    G = H // Hkv
+    for b, L in enumerate(lens):
+        for h in range(Hkv):
+            k, v = c.rows(c.k, b, h, L).double(), c.rows(c.v, b, h, L).double()
+            qq = q[b, h * G:(h + 1) * G].double()
+            s = qq @ k.T * 0.125
+            p = torch.softmax(s, -1)
+            ref, A = p @ v, p @ v.abs()
+            E1 = (66 * 2.0**-24 * 0.125 * (qq.abs() @ k.abs().T).max() + 2.0**-22 * s.abs().max()).item()
+            E = E1 + (L + 32) * 2.0**-23
+            tol = (3 * E + 2.0**-16) * A + 2.0**-8 * ref.abs() * (1 + 2.0**-6)
+            assert ((out[b, h * G:(h + 1) * G].double() - ref).abs() <= tol).all(), (b, h)
