@@ -712,7 +712,9 @@ def _dispatch_paged_decode_attn(dev, output_buffer, inputs, attrs, out_sym, out_
     ws = out_node.aux_data.get("decode_workspace")
     if ws is None or ws.numel() < need:
         ws = torch.zeros(need, dtype=torch.uint8, device=dev.torch_device)
-        out_node.aux_data["decode_workspace"] = ws
+        # one made inside a capture is zeros only where the captured graph runs
+        if not torch.cuda.is_current_stream_capturing():
+            out_node.aux_data["decode_workspace"] = ws
     out, lse = ops.paged_decode_attn(_bf16_rows(q).view(B, H, D), kp, vp, table, lens, k_new=kn,
                                      v_new=vn, window=int(attrs.get("window", 0)),
                                      sinks=int(attrs.get("sinks", 0)), scale=1.0 / math.sqrt(D),

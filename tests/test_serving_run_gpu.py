@@ -234,3 +234,36 @@ def test_operator_graph():
     with pytest.raises(g_.NeuroDSLError):
         g_.addrule(g, g_.GraphRule("bad", ["q", "k", "v"], "window_attention", {"n_heads": 3, "window": 4}))
         g_.demand(g, "bad")
+
+
+def test_operator_graph_captured_before_its_first_run():
+    """A node first demanded inside a capture keeps no workspace from there: its
+    zeros are only written when the captured graph runs."""
+    from neurodsl_b200 import graph as g_
+    ops = _ops()
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(4)
+    rn = lambda *s: torch.randn(s, generator=gen, device=DEV).to(torch.bfloat16)
+    B, H, page, max_pages = 2, 2, 16, 400
+    q, kp, vp = rn(B, H * D), rn(B * max_pages, H, page, D), rn(B * max_pages, H, page, D)
+    table = torch.arange(B * max_pages, dtype=torch.int32, device=DEV).view(B, max_pages)
+    lens = torch.tensor([6400, 5000], dtype=torch.int32, device=DEV)
+    want, _ = ops.paged_decode_attn(q.view(B, H, D), kp, vp, table, lens, out_dtype=torch.float32)
+    g = g_.NeuroGraph()
+    for n, x in (("q", q), ("kp", kp), ("vp", vp), ("table", table), ("lens", lens)):
+        g_.set_(g, n, x)
+    g_.addrule(g, g_.GraphRule("d", ["q", "kp", "vp", "table", "lens"], "paged_decode_attn", {"n_heads": H}))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = g_.demand(g, "d")
+    node = g.nodes["default"]["d"]
+    for x in node.aux_data.values():      # what the capture alone has "written" may hold anything
+        if isinstance(x, torch.Tensor):
+            x.fill_(1)
+    g_.set_(g, "q", q)
+    assert torch.equal(g_.demand(g, "d").view(B, H, D), want)
+    for _ in range(3):
+        graph.replay()
+        assert torch.equal(captured.view(B, H, D), want)
+    assert ops.device_error() == 0
