@@ -57,7 +57,10 @@
 // hands its row sums and accumulator over through shared memory.  So twice as
 // many SMs work, and each takes two K/V tiles in little more than the time of
 // one (509 queries against 4099 keys, B=2, H=16, window 1024: 27.1 us in items of
-// 256 rows, 20.4 with one group a tile, 18.3 so).
+// 256 rows, 20.4 with one group a tile, 17.9 so).  The weights enter the second product
+// as one bf16 term in every form and for every output type, off by 2^-8 each, and by
+// as much again where a row's offset rises between a tile's halves: tensor memory is
+// full (scores, weights and output of two query tiles), with no room for a second term.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <limits.h>
@@ -172,7 +175,7 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
 // x = n + f with n = round(x) (the 1.5·2^23 magic-add rounding, exact for
 // |x| < 2^22) and f in [-0.5, 0.5]; 2^f from a degree-3 minimax polynomial
 // (coefficients computed for this kernel with the Remez exchange algorithm,
-// minimising relative error on [-0.5, 0.5]: max 7.5e-5, far below the 2^-9
+// minimising relative error on [-0.5, 0.5]: max 7.5e-5, far below the 2^-8
 // rounding of the bf16 probabilities); 2^n is added into the exponent field.
 constexpr float kExpC0 = 0.99992806f;
 constexpr float kExpC1 = 0.69326097f;

@@ -11,7 +11,7 @@
 // +inf leaves no number in its head's row, as in the formula.
 //
 // Bound: HBM, 256 bytes per visible key and kv head (K and V rows of 64
-// bf16), each read once for all the query heads of the group.
+// bf16), each read once for up to 16 query heads of the group.
 //
 // Split: the visible keys of a (sequence, kv head) are cut into tiles of 64,
 // and the tiles of all heads, laid end to end, are dealt out in equal
@@ -19,7 +19,7 @@
 // sequence both keep every SM busy, whatever the lengths; a head counts as
 // kHeadCost tiles more than it has, for the joins at its end (without that the
 // CTAs that drew the short heads finished last: 47.5 us for 64 sequences of 32 to
-// 2048 keys, 12 heads, where it now takes 38.6, 81 % of the copy bandwidth).
+// 2048 keys, 12 heads, where it now takes 38.4, 81 % of the copy bandwidth).
 // Every CTA sums the lengths itself: they live on the device, and a host-side
 // plan would need a synchronisation.  A head wholly inside one range is written at once; a head
 // cut by range borders leaves partials (max, sum, unnormalised output) in the
@@ -34,9 +34,9 @@
 // more (the largest power of two that divides it, up to the tile), one TMA box
 // each with the 128-byte swizzle; else 16-byte cp.async pieces into the same
 // layout, by four warps (two beside 16 query heads, whose consumers need the
-// registers).  64 sequences of 2048 keys, 12 heads: 68.6 us at pages of 64 rows,
-// 71.0 at 16, 75.6 at 24 (by pieces 119.8 with one warp); by pieces 86.4 at 100
-// (98.3 in boxes of 4), 94.7 at 7, 119.4 at 1.
+// registers).  64 sequences of 2048 keys, 12 heads: 67.8 us at pages of 64 rows,
+// 70.2 at 16, 77.4 at 24 (by pieces with one warp 1.6 times as long); by pieces 88.5
+// at 100 (in boxes of 4 a seventh longer), 97.2 at 7, 120.7 at 1.
 //
 // S = Q K^T takes Q as the 16-row operand of mma.m16n8k16 (query head = row)
 // and K's rows as they lie (ldmatrix).  The scores' fragment is then, packed to
@@ -222,8 +222,8 @@ __device__ __forceinline__ int next_tile(const Params& p, int heads, Cursor& c) 
 
 // What every warp works out for itself: the cost of all heads, how many CTAs
 // share it, and this CTA's range [lo, hi) of it.  A head of n tiles takes
-// n + kHeadCost places, its tiles the first n.  (No barrier: the five warps of
-// a CTA read the same few lengths.)
+// n + kHeadCost places, its tiles the first n.  (No barrier: the warps of a CTA
+// read the same few lengths.)
 struct Plan {
   long long total, lo, hi;
   int n_cta;

@@ -694,7 +694,9 @@ def window_attn_fwd(Q, K, V, window, sinks=0, scale=None, out=None, out_dtype=to
     p sees key j when j <= p and (j > p - window or j < sinks).
 
     Returns (O, lse, row_max) like flash_attn_fwd, and like there Q, K, V and
-    `out` may be strided views (a fused projection, a longer cache)."""
+    `out` may be strided views (a fused projection, a longer cache).  All Sk keys and
+    values have to be finite, padding too: a masked value weighs 0, and 0 times an
+    infinity is NaN."""
     if out is not None and stream is None and _quick(
             "window_attn_fwd", Q, K, V, window, sinks, scale, out, lse, row_max):
         return out, lse, row_max
@@ -745,7 +747,7 @@ def paged_decode_workspace_size(B, H, Hkv, max_len, weights=False, D=64):
 def paged_decode_workspace(B, H, Hkv, max_len, weights=False, device=None):
     """A zero-filled workspace for paged_decode_attn calls of up to these
     sizes (max_len: pages a sequence times page_size; weights: for calls that
-    accumulate them).  Every call leaves it ready for the next; calls that may
+    accumulate them, 4 bytes more for every query head and key of the table).  Every call leaves it ready for the next; calls that may
     run at the same time, two captured graphs' among them, need one each."""
     n = paged_decode_workspace_size(B, H, Hkv, max_len, weights)
     return torch.zeros(n, dtype=torch.uint8, device=device if device is not None else "cuda")
